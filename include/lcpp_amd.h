@@ -52,7 +52,9 @@ typedef enum lcpp_dtype LCPP_ENUM_INT {
     LCPP_FLOAT32 = 2,
     LCPP_INT64 = 3,
     LCPP_UINT64 = 4,
-    LCPP_FLOAT64 = 5
+    LCPP_FLOAT64 = 5,
+    LCPP_BFLOAT16 = 6, /* these two: lcpp_layer_norm_*, lcpp_dropout, lcpp_recurrence_* only */
+    LCPP_FLOAT16 = 7
 } lcpp_dtype;
 
 /* Reduction operators and element transforms of lcpp_reduce_transform (the
@@ -69,6 +71,13 @@ typedef enum lcpp_transform LCPP_ENUM_INT {
     LCPP_XFORM_ABS = 2,    /* identity for unsigned types */
     LCPP_XFORM_SQUARE = 3  /* integers wrap */
 } lcpp_transform;
+
+/* How lcpp_recurrence_* take the decay a and the drive b of a step from its gate g and input x. */
+typedef enum lcpp_gate LCPP_ENUM_INT {
+    LCPP_GATE_DECAY = 0,  /* a = g, b = x */
+    LCPP_GATE_LOG = 1,    /* a = exp(g), b = x */
+    LCPP_GATE_SIGMOID = 2 /* a = sigmoid(g), b = (1 - a) x */
+} lcpp_gate;
 
 typedef enum lcpp_status LCPP_ENUM_INT {
     LCPP_OK = 0,
@@ -340,6 +349,96 @@ int lcpp_segment_reduce_argmin_fixed(lcpp_dtype t, void *temp, size_t temp_bytes
 int lcpp_segment_reduce_argmax_fixed(lcpp_dtype t, void *temp, size_t temp_bytes, const void *in, void *out,
                                      uint32_t *index_out, uint64_t num_segments, uint32_t segment_size,
                                      void *stream);
+
+/* ---------------------------------------------------------------------
+ * Layer norm, dropout, gated linear recurrence (no counterpart in the
+ * reference): the operators of a recurrent language model's residual block,
+ * next to the reductions and scans they are made of.
+ *
+ * t: LCPP_FLOAT32, LCPP_BFLOAT16 or LCPP_FLOAT16 for activations and their
+ * gradients; statistics, states and random-bit counters are float32 / 64-bit
+ * integers as declared.  Everything is computed in 32 bits and rounded once,
+ * to nearest even, when it is stored.  Rows have unit stride along their
+ * columns; *_stride is the distance between rows in elements, of any size for
+ * inputs (0 repeats a row) and at least cols for outputs.  Pointers need the
+ * alignment of one element only.  Outputs may lie exactly in the place of an
+ * input of the same type and stride (but `sum` not in that of `out`); other
+ * overlaps give wrong results.  rows < 2^32, cols <= 2^30.
+ * ------------------------------------------------------------------- */
+/* out[r] = (in[r] - mean) * rstd * weight + bias with each row's mean and rstd = 1 / sqrt(var +
+ * eps), var over cols.  weight, bias: `cols` values of type wt (t or LCPP_FLOAT32), NULL for 1 and
+ * 0.  mean, rstd: one value per row, NULL where the backward pass does not follow. */
+int lcpp_layer_norm_forward(lcpp_dtype t, lcpp_dtype wt, const void *in, uint64_t in_stride, const void *weight,
+                            const void *bias, float eps, void *out, uint64_t out_stride, float *mean, float *rstd,
+                            uint64_t rows, uint64_t cols, void *stream);
+/* sum = residual + dropout(in), stored in type t, and the layer norm of what is stored. */
+int lcpp_layer_norm_add_forward(lcpp_dtype t, lcpp_dtype wt, const void *in, uint64_t in_stride, const void *residual,
+                                uint64_t residual_stride, double p, uint64_t seed, uint64_t offset,
+                                const uint64_t *offset_dev, const void *weight, const void *bias, float eps, void *sum,
+                                uint64_t sum_stride, void *out, uint64_t out_stride, float *mean, float *rstd,
+                                uint64_t rows, uint64_t cols, void *stream);
+/* Partial sums of the weight's and bias's gradients: up to 512 rows of 2 cols floats. */
+int lcpp_layer_norm_backward_temp_bytes(lcpp_dtype t, uint64_t rows, uint64_t cols, size_t *bytes);
+/* The gradients of lcpp_layer_norm_forward from that of `out`, its input and its statistics.
+ * grad_weight, grad_bias: `cols` values of type wt, each NULL if not wanted (temp is needed for
+ * either); for rows = 0 they are set to 0.  Sums over rows are made in a fixed order: a call gives
+ * the same bits every time. */
+int lcpp_layer_norm_backward(lcpp_dtype t, lcpp_dtype wt, void *temp, size_t temp_bytes, const void *grad_out,
+                             uint64_t grad_out_stride, const void *in, uint64_t in_stride, const void *weight,
+                             const float *mean, const float *rstd, void *grad_in, uint64_t grad_in_stride,
+                             void *grad_weight, void *grad_bias, uint64_t rows, uint64_t cols, void *stream);
+/* The gradients of lcpp_layer_norm_add_forward.  grad_sum: what reaches `sum` by other ways (the
+ * residual path), NULL for none.  grad_residual = the sum's whole gradient, grad_in = its dropout
+ * with the forward call's p, seed and offset; each NULL if not wanted. */
+int lcpp_layer_norm_add_backward(lcpp_dtype t, lcpp_dtype wt, void *temp, size_t temp_bytes, const void *grad_out,
+                                 uint64_t grad_out_stride, const void *grad_sum, uint64_t grad_sum_stride,
+                                 const void *sum, uint64_t sum_stride, const void *weight, const float *mean,
+                                 const float *rstd, double p, uint64_t seed, uint64_t offset,
+                                 const uint64_t *offset_dev, void *grad_residual, uint64_t grad_residual_stride,
+                                 void *grad_in, uint64_t grad_in_stride, void *grad_weight, void *grad_bias,
+                                 uint64_t rows, uint64_t cols, void *stream);
+/* out = (kept ? in * 65536 / (65536 - cut) : 0) [+ residual], cut = round(65536 p).  An element is
+ * kept where its 16 random bits are >= cut: bits 16 (c % 2) .. +16 of word (c % 8) / 2 of Philox
+ * 4x32 with 7 rounds, counter (c / 8, row, offset, offset >> 32), key (seed, seed >> 32), c the
+ * column.  No mask is stored: the backward pass is the same call on the gradient, without the
+ * residual.  offset_dev: a device counter added to offset when the kernel runs (a captured graph
+ * can advance it between replays), or NULL.  0 <= p <= 1. */
+int lcpp_dropout(lcpp_dtype t, const void *in, uint64_t in_stride, const void *residual, uint64_t residual_stride,
+                 void *out, uint64_t out_stride, uint64_t rows, uint64_t cols, double p, uint64_t seed,
+                 uint64_t offset, const uint64_t *offset_dev, void *stream);
+
+/* h_t = a_t h_{t-1} + b_t for every channel of every sequence, a and b from the gate and the input
+ * (lcpp_gate), out_t = h_t.  Row t of sequence s is `channels` values at s * seq + t * row of each
+ * tensor.  begin, end == NULL: every sequence has max_length rows.  Otherwise sequence s is rows
+ * begin[s] .. end[s] of tensors of `rows` rows (the seq strides are not used), empty if end <=
+ * begin and cut at max_length, which sizes the launch; rows of no sequence are left alone.
+ * initial (NULL: 0), final_state: the states before the first and after the last row, float32
+ * [sequences][channels]; an empty sequence's final state is its initial one.  checkpoints: what
+ * the backward pass needs, float32 [sequences][lcpp_recurrence_checkpoint_rows][channels], or NULL. */
+int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes);
+int lcpp_recurrence_checkpoint_rows(uint64_t max_length, uint64_t *rows);
+int lcpp_recurrence_forward(lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, const void *gate,
+                            uint64_t gate_row, uint64_t gate_seq, const void *in, uint64_t in_row, uint64_t in_seq,
+                            void *out, uint64_t out_row, uint64_t out_seq, const float *initial, float *final_state,
+                            float *checkpoints, uint64_t sequences, uint64_t max_length, uint64_t channels,
+                            const uint32_t *begin, const uint32_t *end, uint64_t rows, void *stream);
+/* The gradients of gate, input and initial state (NULL if not wanted) from those of `out` and of
+ * the final state (NULL: 0), with the forward call's checkpoints and the same sequences. */
+int lcpp_recurrence_backward(lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, const void *gate,
+                             uint64_t gate_row, uint64_t gate_seq, const void *in, uint64_t in_row, uint64_t in_seq,
+                             const float *checkpoints, const void *grad_out, uint64_t grad_out_row,
+                             uint64_t grad_out_seq, void *grad_gate, uint64_t grad_gate_row, uint64_t grad_gate_seq,
+                             void *grad_in, uint64_t grad_in_row, uint64_t grad_in_seq, const float *grad_final,
+                             float *grad_initial, uint64_t sequences, uint64_t max_length, uint64_t channels,
+                             const uint32_t *begin, const uint32_t *end, uint64_t rows, void *stream);
+/* One token for each of `sequences`: h = a h + b, out = h, on the states [num_slots][channels] of a
+ * pool, read at state_in and written at state_out (which may be the same) in row slots[s], or row s
+ * if slots is NULL.  A slot outside 0 .. num_slots - 1 marks padding: no state changes, out is 0.
+ * No two sequences may name the same slot. */
+int lcpp_recurrence_step(lcpp_dtype t, lcpp_gate g, const void *gate, uint64_t gate_stride, const void *in,
+                         uint64_t in_stride, const float *state_in, float *state_out, const int32_t *slots,
+                         uint64_t num_slots, void *out, uint64_t out_stride, uint64_t sequences, uint64_t channels,
+                         void *stream);
 
 /* ---------------------------------------------------------------------
  * Instrumentation (no counterpart in the reference).  When enabled, every

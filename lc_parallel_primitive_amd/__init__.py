@@ -25,6 +25,7 @@ from ._capi import (  # noqa: F401
     profile_enable,
     profile_read,
 )
+from .device_block import DeviceDropout, DeviceGatedRecurrence, DeviceLayerNorm  # noqa: F401
 from .device import DeviceRadixSort, DeviceReduce, DeviceScan, DeviceSegmentReduce  # noqa: F401
 
 __all__ = [
@@ -32,6 +33,9 @@ __all__ = [
     "DeviceScan",
     "DeviceRadixSort",
     "DeviceSegmentReduce",
+    "DeviceLayerNorm",
+    "DeviceDropout",
+    "DeviceGatedRecurrence",
     "LcppError",
     "lib",
     "lib_path",

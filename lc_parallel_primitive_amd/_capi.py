@@ -9,8 +9,10 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 lib_path = os.path.join(_PKG, "liblcpp_amd.so")
 
 LCPP_INT32, LCPP_UINT32, LCPP_FLOAT32, LCPP_INT64, LCPP_UINT64, LCPP_FLOAT64 = range(6)
+LCPP_BFLOAT16, LCPP_FLOAT16 = 6, 7  # the layer norm, dropout and recurrence only
 LCPP_OPS = {"sum": 0, "min": 1, "max": 2}
 LCPP_TRANSFORMS = {"identity": 0, "negate": 1, "abs": 2, "square": 3}
+LCPP_GATES = {"decay": 0, "log": 1, "sigmoid": 2}
 LCPP_DTYPES = {
     "int32": LCPP_INT32,
     "uint32": LCPP_UINT32,
@@ -25,6 +27,8 @@ _c_size_p = ctypes.POINTER(ctypes.c_size_t)
 _vp = ctypes.c_void_p
 _u64 = ctypes.c_uint64
 _i = ctypes.c_int
+_f = ctypes.c_float
+_d = ctypes.c_double
 SIGNATURES = {
     "lcpp_version": (_i, []),
     "lcpp_status_string": (ctypes.c_char_p, [_i]),
@@ -68,6 +72,22 @@ SIGNATURES = {
     "lcpp_segment_reduce_argmax": (_i, [_i, _vp, ctypes.c_size_t, _vp, _vp, _vp, _u64, _vp, _vp, _vp]),
     "lcpp_segment_reduce_argmin_fixed": (_i, [_i, _vp, ctypes.c_size_t, _vp, _vp, _vp, _u64, ctypes.c_uint32, _vp]),
     "lcpp_segment_reduce_argmax_fixed": (_i, [_i, _vp, ctypes.c_size_t, _vp, _vp, _vp, _u64, ctypes.c_uint32, _vp]),
+    "lcpp_layer_norm_forward": (_i, [_i, _i, _vp, _u64, _vp, _vp, _f, _vp, _u64, _vp, _vp, _u64, _u64, _vp]),
+    "lcpp_layer_norm_add_forward": (_i, [_i, _i, _vp, _u64, _vp, _u64, _d, _u64, _u64, _vp, _vp, _vp, _f, _vp, _u64, _vp, _u64,
+                                         _vp, _vp, _u64, _u64, _vp]),
+    "lcpp_layer_norm_backward_temp_bytes": (_i, [_i, _u64, _u64, _c_size_p]),
+    "lcpp_layer_norm_backward": (_i, [_i, _i, _vp, ctypes.c_size_t, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _vp, _u64, _vp, _vp,
+                                      _u64, _u64, _vp]),
+    "lcpp_layer_norm_add_backward": (_i, [_i, _i, _vp, ctypes.c_size_t, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _d, _u64,
+                                          _u64, _vp, _vp, _u64, _vp, _u64, _vp, _vp, _u64, _u64, _vp]),
+    "lcpp_dropout": (_i, [_i, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _d, _u64, _u64, _vp, _vp]),
+    "lcpp_recurrence_temp_bytes": (_i, [_u64, _u64, _u64, _c_size_p]),
+    "lcpp_recurrence_checkpoint_rows": (_i, [_u64, ctypes.POINTER(_u64)]),
+    "lcpp_recurrence_forward": (_i, [_i, _i, _vp, ctypes.c_size_t] + [_vp, _u64, _u64] * 3 + [_vp, _vp, _vp, _u64, _u64, _u64, _vp,
+                                     _vp, _u64, _vp]),
+    "lcpp_recurrence_backward": (_i, [_i, _i, _vp, ctypes.c_size_t] + [_vp, _u64, _u64] * 2 + [_vp] + [_vp, _u64, _u64] * 3
+                                 + [_vp, _vp, _u64, _u64, _u64, _vp, _vp, _u64, _vp]),
+    "lcpp_recurrence_step": (_i, [_i, _i, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _u64, _u64, _vp]),
     "lcpp_temp_status": (_i, [_vp, ctypes.c_size_t, _vp]),
     "lcpp_temp_status_record": (_i, [_vp, ctypes.c_size_t, _vp, _vp]),
     "lcpp_device_status_decode": (_i, [ctypes.c_uint32]),
@@ -132,6 +152,26 @@ def dtype_code(dtype) -> int:
     code = LCPP_DTYPES[name]
     try:
         _codes[dtype] = code
+    except TypeError:  # not hashable
+        pass
+    return code
+
+
+_float_codes: dict = {}
+
+
+def float_code(dtype) -> int:
+    """lcpp_dtype of a floating type of activations: float32, bfloat16 or float16."""
+    try:
+        return _float_codes[dtype]
+    except (KeyError, TypeError):
+        pass
+    name = str(dtype).replace("torch.", "").replace("numpy.", "")
+    code = {"float32": LCPP_FLOAT32, "bfloat16": LCPP_BFLOAT16, "float16": LCPP_FLOAT16}.get(name)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}: float32, bfloat16 or float16")
+    try:
+        _float_codes[dtype] = code
     except TypeError:  # not hashable
         pass
     return code

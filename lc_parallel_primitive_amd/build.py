@@ -19,7 +19,7 @@ LIB = os.path.join(PKG, "liblcpp_amd.so")
 DATAGEN_LIB = os.path.join(PKG, "liblcpp_datagen.so")
 
 LIB_SOURCES = ["runtime.hip", "reduce.hip", "scan.hip", "radix_sort.hip", "small_sort.hip", "tie_repair.hip", "segment_reduce.hip",
-               "scan_by_key.hip", "reduce_by_key.hip"]
+               "scan_by_key.hip", "reduce_by_key.hip", "layer_norm.hip", "dropout.hip", "recurrence.hip"]
 DATAGEN_SOURCES = ["datagen.hip"]
 
 ARCH = os.environ.get("LCPP_OFFLOAD_ARCH", "gfx950")

@@ -1,0 +1,669 @@
+// layer_norm.hip — layer norm over rows, forward and backward, alone or with
+// the residual sum and dropout before it.
+//
+//   s = x, or s = residual + dropout(x), stored in the rows' type
+//   mean = sum(s) / n,  rstd = 1 / sqrt(sum((s - mean)^2) / n + eps)
+//   y = (s - mean) rstd w + b
+//
+// With u = (s - mean) rstd and v = dy w, the gradients are
+//   ds = rstd (v - sum(v) / n - u sum(v u) / n)   [+ the gradient that reaches s elsewhere]
+//   dw = sum over rows of dy u,  db = sum over rows of dy
+//   dresidual = ds,  dx = dropout(ds) with the forward pass's random bits
+#include <algorithm>
+
+#include "tensor.hpp"
+
+namespace lcpp {
+namespace {
+
+// Sums of one or two values over the NT threads of a row's group; every thread
+// of the group gets them.  A group of several waves meets in LDS, and all groups
+// of the workgroup meet at the same barrier; `slot` alternates between the calls
+// of one row, so that one barrier a call is enough.
+template <int NT, int WAVES, int V>
+__device__ __forceinline__ void group_sum(float (&x)[V], float (*lds)[WAVES][2], int slot)
+{
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = wave_reduce_dpp(x[v], SumOp());
+    if constexpr (NT > kWave) {
+        constexpr int GW = NT / kWave;
+        const uint32_t wave = threadIdx.x / kWave;
+        if (lane_id() == 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) lds[slot][wave][v] = x[v];
+        }
+        __syncthreads();
+        const uint32_t first = wave / GW * GW;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < GW; ++w) s += lds[slot][first + w][v];
+            x[v] = s;
+        }
+    }
+}
+
+struct NormArgs {
+    const void *in, *residual, *weight, *bias;
+    void *sum, *out;
+    uint64_t in_stride, residual_stride, sum_stride, out_stride;
+    float *mean, *rstd;
+    uint32_t rows, cols;
+    float eps;
+    DropArgs drop;
+};
+
+// s of one octet: the input, or residual + dropout(input) rounded to the rows'
+// type, which is also stored.
+template <class T, bool ADD>
+__device__ __forceinline__ Octet<T> norm_input(const NormArgs &a, uint64_t offset, uint32_t row, uint32_t col)
+{
+    Octet<T> x = load_octet(static_cast<const T *>(a.in) + row * a.in_stride, col, a.cols);
+    if constexpr (ADD) {
+        const Octet<T> r = load_octet(static_cast<const T *>(a.residual) + row * a.residual_stride, col, a.cols);
+        float v[kOctet];
+#pragma unroll
+        for (int i = 0; i < kOctet; ++i) v[i] = x[i];
+        if (a.drop.cut) drop_octet(v, row, col / kOctet, offset, a.drop);
+#pragma unroll
+        for (int i = 0; i < kOctet; ++i) {
+            v[i] += r[i];
+            x.v[i] = (T)v[i];
+        }
+        store_octet(static_cast<T *>(a.sum) + row * a.sum_stride, col, a.cols, v);
+    }
+    return x;
+}
+
+template <class T, class W>
+__device__ __forceinline__ void norm_output(const NormArgs &a, uint32_t row, uint32_t col, const Octet<T> &x, float mean,
+                                            float rstd)
+{
+    float y[kOctet];
+#pragma unroll
+    for (int i = 0; i < kOctet; ++i) y[i] = (x[i] - mean) * rstd;
+    if (a.weight) {
+        const Octet<W> w = load_octet(static_cast<const W *>(a.weight), col, a.cols);
+#pragma unroll
+        for (int i = 0; i < kOctet; ++i) y[i] *= w[i];
+    }
+    if (a.bias) {
+        const Octet<W> b = load_octet(static_cast<const W *>(a.bias), col, a.cols);
+#pragma unroll
+        for (int i = 0; i < kOctet; ++i) y[i] += b[i];
+    }
+    store_octet(static_cast<T *>(a.out) + row * a.out_stride, col, a.cols, y);
+}
+
+// Rows whose octets fit the registers of NT threads, K each: read once, the mean
+// first and then the squares around it, so a row far from 0 loses nothing.
+template <class T, class W, int NT, int K, int THREADS, bool ADD>
+__global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
+{
+    constexpr int WAVES = THREADS / kWave;
+    __shared__ float lds[2][WAVES][2];
+    constexpr int RG = THREADS / NT;
+    const uint32_t t = threadIdx.x % NT;
+    const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
+    // (the workgroup's groups make the same number of rounds: they share barriers)
+    for (uint64_t base = (uint64_t)blockIdx.x * RG; base < a.rows; base += (uint64_t)gridDim.x * RG) {
+        const uint64_t row64 = base + threadIdx.x / NT;
+        const bool live = row64 < a.rows;
+        const uint32_t row = (uint32_t)row64;
+        Octet<T> x[K];
+        float sum[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t col = (t + k * NT) * kOctet;
+            if (live && col < a.cols) {
+                x[k] = norm_input<T, ADD>(a, offset, row, col);
+#pragma unroll
+                for (int i = 0; i < kOctet; ++i) sum[0] += x[k][i];
+            }
+        }
+        group_sum<NT, WAVES>(sum, lds, 0);
+        const float mean = sum[0] / (float)a.cols;
+        float sq[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t col = (t + k * NT) * kOctet;
+            if (live && col < a.cols) {
+#pragma unroll
+                for (int i = 0; i < kOctet; ++i) {
+                    const float d = x[k][i] - mean;
+                    if (col + i < a.cols) sq[0] += d * d;
+                }
+            }
+        }
+        group_sum<NT, WAVES>(sq, lds, 1);
+        const float rstd = 1.0f / sqrtf(sq[0] / (float)a.cols + a.eps);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t col = (t + k * NT) * kOctet;
+            if (live && col < a.cols) norm_output<T, W>(a, row, col, x[k], mean, rstd);
+        }
+        if (live && t == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+// Longer rows: a workgroup reads its row three times (from the caches).
+constexpr int kLongThreads = 1024;
+template <class T, class W, bool ADD>
+__global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(NormArgs a)
+{
+    constexpr int WAVES = kLongThreads / kWave;
+    __shared__ float lds[2][WAVES][2];
+    const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *s = ADD ? static_cast<const T *>(a.sum) + row * a.sum_stride
+                         : static_cast<const T *>(a.in) + row * a.in_stride;
+        float sum[1] = {0.0f};
+        for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
+            const Octet<T> x = norm_input<T, ADD>(a, offset, row, col);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) sum[0] += x[i];
+        }
+        group_sum<kLongThreads, WAVES>(sum, lds, 0);
+        const float mean = sum[0] / (float)a.cols;
+        float sq[1] = {0.0f};
+        // (each thread reads back the sums that it stored itself)
+        for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
+            const Octet<T> x = load_octet(s, col, a.cols);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) {
+                const float d = x[i] - mean;
+                if (col + i < a.cols) sq[0] += d * d;
+            }
+        }
+        group_sum<kLongThreads, WAVES>(sq, lds, 1);
+        const float rstd = 1.0f / sqrtf(sq[0] / (float)a.cols + a.eps);
+        for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet)
+            norm_output<T, W>(a, row, col, load_octet(s, col, a.cols), mean, rstd);
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- backward
+struct NormGradArgs {
+    const void *grad_out, *grad_sum, *in, *weight;
+    void *grad_in, *grad_branch;  // ds, and dx where it is not ds
+    uint64_t go_stride, gs_stride, in_stride, gi_stride, gb_stride;
+    const float *mean, *rstd;
+    float *partial;    // [workgroup][dw, db][cols]; null: neither is wanted
+    uint32_t *status;  // the temp storage's status word, cleared here (may be null)
+    uint32_t rows, cols;
+    DropArgs drop;
+};
+
+// One octet's dy w (v), u, and its shares of dw and db.
+template <class T, class W>
+__device__ __forceinline__ void norm_grad_terms(const Octet<T> &dy, const Octet<T> &s, const float (&w)[kOctet],
+                                                float mean, float rstd, float (&v)[kOctet], float (&u)[kOctet])
+{
+#pragma unroll
+    for (int i = 0; i < kOctet; ++i) {
+        u[i] = (s[i] - mean) * rstd;
+        v[i] = dy[i] * w[i];
+    }
+}
+template <class W>
+__device__ __forceinline__ void norm_weight(const void *weight, uint32_t col, uint32_t cols, float (&w)[kOctet])
+{
+    if (weight) {
+        const Octet<W> o = load_octet(static_cast<const W *>(weight), col, cols);
+#pragma unroll
+        for (int i = 0; i < kOctet; ++i) w[i] = o[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kOctet; ++i) w[i] = 1.0f;
+    }
+}
+// ds of an octet from the row's sums, and what is stored of it.
+template <class T, bool ADD>
+__device__ __forceinline__ void norm_grad_output(const NormGradArgs &a, uint64_t offset, uint32_t row, uint32_t col,
+                                                 const float (&v)[kOctet], const float (&u)[kOctet], float mean_v,
+                                                 float mean_vu, float rstd)
+{
+    float d[kOctet];
+#pragma unroll
+    for (int i = 0; i < kOctet; ++i) d[i] = rstd * (v[i] - mean_v - u[i] * mean_vu);
+    if constexpr (ADD) {
+        if (a.grad_sum) {
+            const Octet<T> g = load_octet(static_cast<const T *>(a.grad_sum) + row * a.gs_stride, col, a.cols);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) d[i] += g[i];
+        }
+    }
+    if (a.grad_in) store_octet(static_cast<T *>(a.grad_in) + row * a.gi_stride, col, a.cols, d);
+    if constexpr (ADD) {
+        if (a.grad_branch) {
+            if (a.drop.cut) drop_octet(d, row, col / kOctet, offset, a.drop);
+            store_octet(static_cast<T *>(a.grad_branch) + row * a.gb_stride, col, a.cols, d);
+        }
+    }
+}
+
+// THREADS / NT rows at a time; a thread keeps the same columns for all of its
+// workgroup's rows, so dw and db are sums in its registers, one partial sum per
+// workgroup at the end.
+template <class T, class W, int NT, int K, int THREADS, bool ADD>
+__global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
+{
+    constexpr int WAVES = THREADS / kWave, RG = THREADS / NT;
+    __shared__ float lds[2][WAVES][2];
+    __shared__ float fold[RG > 1 ? NT * K * kOctet : 1];
+    const uint32_t t = threadIdx.x % NT, group = threadIdx.x / NT;
+    const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
+    const float inv = 1.0f / (float)a.cols;
+    float dw[K][kOctet] = {}, db[K][kOctet] = {};
+    int slot = 0;
+    if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+    // (the workgroup's groups make the same number of rounds: they share barriers)
+    for (uint64_t base = (uint64_t)blockIdx.x * RG; base < a.rows; base += (uint64_t)gridDim.x * RG, slot ^= 1) {
+        const uint64_t row64 = base + group;
+        const bool live = row64 < a.rows;
+        const uint32_t row = live ? (uint32_t)row64 : a.rows - 1;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        Octet<T> dy[K], s[K];
+        float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t col = (t + k * NT) * kOctet;
+            if (live && col < a.cols) {
+                dy[k] = load_octet(static_cast<const T *>(a.grad_out) + row * a.go_stride, col, a.cols);
+                s[k] = load_octet(static_cast<const T *>(a.in) + row * a.in_stride, col, a.cols);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t col = (t + k * NT) * kOctet;
+            if (live && col < a.cols) {
+                float w[kOctet], v[kOctet], u[kOctet];
+                norm_weight<W>(a.weight, col, a.cols, w);
+                norm_grad_terms<T, W>(dy[k], s[k], w, mean, rstd, v, u);
+#pragma unroll
+                for (int i = 0; i < kOctet; ++i) {
+                    // (past the row's end dy and v are 0, u is not)
+                    sums[0] += v[i];
+                    sums[1] += v[i] * u[i];
+                    dw[k][i] += dy[k][i] * u[i];
+                    db[k][i] += dy[k][i];
+                }
+            }
+        }
+        group_sum<NT, WAVES>(sums, lds, slot);
+        const float mean_v = sums[0] * inv, mean_vu = sums[1] * inv;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t col = (t + k * NT) * kOctet;
+            if (live && col < a.cols) {
+                float w[kOctet], v[kOctet], u[kOctet];
+                norm_weight<W>(a.weight, col, a.cols, w);
+                norm_grad_terms<T, W>(dy[k], s[k], w, mean, rstd, v, u);
+                norm_grad_output<T, ADD>(a, offset, row, col, v, u, mean_v, mean_vu, rstd);
+            }
+        }
+    }
+    if (!a.partial) return;
+    float *part = a.partial + (uint64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+    for (int half = 0; half < 2; ++half, part += a.cols) {
+        float(&x)[K][kOctet] = half ? db : dw;
+        if constexpr (RG > 1) {
+            // the groups add to the columns' sums one after the other, in a fixed order
+            for (uint32_t g = 0; g < RG; ++g) {
+                if (group == g) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k)
+#pragma unroll
+                        for (int i = 0; i < kOctet; ++i) {
+                            float &f = fold[(i * K + k) * NT + t];
+                            f = g ? f + x[k][i] : x[k][i];
+                            x[k][i] = f;
+                        }
+                }
+                __syncthreads();
+            }
+        }
+        if (group == RG - 1) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const uint32_t col = (t + k * NT) * kOctet;
+                if (col < a.cols) store_octet(part, col, a.cols, x[k]);
+            }
+        }
+    }
+}
+
+// Longer rows, ds: a workgroup reads its row twice (the second time from the caches).
+template <class T, class W, bool ADD>
+__global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(NormGradArgs a)
+{
+    constexpr int WAVES = kLongThreads / kWave;
+    __shared__ float lds[2][WAVES][2];
+    const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
+    const float inv = 1.0f / (float)a.cols;
+    if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+    int slot = 0;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x, slot ^= 1) {
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        const T *dy = static_cast<const T *>(a.grad_out) + row * a.go_stride;
+        const T *s = static_cast<const T *>(a.in) + row * a.in_stride;
+        float sums[2] = {0.0f, 0.0f};
+        float w[kOctet], v[kOctet], u[kOctet];
+        for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
+            norm_weight<W>(a.weight, col, a.cols, w);
+            norm_grad_terms<T, W>(load_octet(dy, col, a.cols), load_octet(s, col, a.cols), w, mean, rstd, v, u);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) {
+                sums[0] += v[i];
+                sums[1] += v[i] * u[i];
+            }
+        }
+        group_sum<kLongThreads, WAVES>(sums, lds, slot);
+        for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
+            norm_weight<W>(a.weight, col, a.cols, w);
+            norm_grad_terms<T, W>(load_octet(dy, col, a.cols), load_octet(s, col, a.cols), w, mean, rstd, v, u);
+            norm_grad_output<T, ADD>(a, offset, row, col, v, u, sums[0] * inv, sums[1] * inv, rstd);
+        }
+    }
+}
+// Longer rows, dw and db: a workgroup takes 2048 columns of every gridDim.y-th
+// row.  It runs before ds is written, which may go where dy or s lies.
+constexpr int kColThreads = 256;
+template <class T>
+__global__ __launch_bounds__(kColThreads) void norm_backward_cols_kernel(NormGradArgs a)
+{
+    const uint32_t col = (blockIdx.x * kColThreads + threadIdx.x) * kOctet;
+    if (col >= a.cols) return;
+    float dw[kOctet] = {}, db[kOctet] = {};
+    for (uint64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const Octet<T> dy = load_octet(static_cast<const T *>(a.grad_out) + row * a.go_stride, col, a.cols);
+        const Octet<T> s = load_octet(static_cast<const T *>(a.in) + row * a.in_stride, col, a.cols);
+        const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+        for (int i = 0; i < kOctet; ++i) {
+            dw[i] += dy[i] * ((s[i] - mean) * rstd);
+            db[i] += dy[i];
+        }
+    }
+    float *part = a.partial + (uint64_t)blockIdx.y * 2 * a.cols;
+    store_octet(part, col, a.cols, dw);
+    store_octet(part + a.cols, col, a.cols, db);
+}
+
+// dw and db from the partial sums: 64 columns per workgroup, each wave every
+// 16th partial sum, always in the same order.
+constexpr int kFoldWaves = 16;
+template <class W>
+__global__ __launch_bounds__(kFoldWaves *kWave) void norm_fold_kernel(const float *partial, uint32_t parts, uint32_t cols,
+                                                                      W *grad_weight, W *grad_bias)
+{
+    __shared__ float lds[kFoldWaves][kWave];
+    const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const uint32_t col = blockIdx.x * kWave + lane;
+    W *out = blockIdx.y ? grad_bias : grad_weight;
+    if (!out) return;
+    float sum = 0.0f;
+    if (col < cols) {
+        const float *p = partial + (uint64_t)blockIdx.y * cols + col;
+#pragma unroll 4
+        for (uint32_t i = wave; i < parts; i += kFoldWaves) sum += p[(uint64_t)i * 2 * cols];
+    }
+    lds[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && col < cols) {
+#pragma unroll
+        for (int w = 1; w < kFoldWaves; ++w) sum += lds[w][lane];
+        out[col] = from_f32<W>(sum);
+    }
+}
+
+// ---------------------------------------------------------------- launches
+// (a launch has less than 2^32 threads: with more rows, workgroups take several)
+constexpr uint64_t kMaxGroups = 1u << 20;
+
+// NT threads with K octets each for a row of `octets`: the smallest group of
+// waves that holds it.  f(NT, K) as integral constants; false if the row is longer.
+template <class F>
+bool norm_forward_shape(uint32_t octets, F f)
+{
+    using std::integral_constant;
+    if (octets <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (octets <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    else if (octets <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    else if (octets <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    else if (octets <= 1024) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    else if (octets <= 2048) f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    else if (octets <= 4096) f(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+    else return false;
+    return true;
+}
+template <class F>
+bool norm_backward_shape(uint32_t octets, F f)
+{
+    using std::integral_constant;
+    if (octets <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (octets <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    else if (octets <= 256) f(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+    else if (octets <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    else if (octets <= 1024) f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    else if (octets <= 2048) f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    else return false;
+    return true;
+}
+
+template <class T, class W, bool ADD>
+int norm_forward_launch(const NormArgs &a, hipStream_t s)
+{
+    const uint32_t octets = (uint32_t)ceil_div(a.cols, kOctet);
+    const char *name = ADD ? "layer_norm_add_forward" : "layer_norm_forward";
+    const bool fits = norm_forward_shape(octets, [&](auto nt, auto k) {
+        constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
+        constexpr int THREADS = NT > 256 ? NT : 256;
+        const uint32_t grid = (uint32_t)std::min<uint64_t>(ceil_div(a.rows, THREADS / NT), kMaxGroups);
+        LCPP_LAUNCH(name, s, norm_forward_kernel<T, W, NT, K, THREADS, ADD><<<grid, THREADS, 0, s>>>(a));
+    });
+    if (!fits) LCPP_LAUNCH(name, s, norm_forward_long_kernel<T, W, ADD><<<(uint32_t)std::min<uint64_t>(a.rows, kMaxGroups), kLongThreads, 0, s>>>(a));
+    LCPP_CHECK_LAUNCH();
+    return LCPP_OK;
+}
+
+// Partial sums of dw and db: at most one for each of two workgroups per CU.
+constexpr uint64_t kMaxParts = 512;
+uint64_t norm_parts(uint64_t rows) { return rows < kMaxParts ? rows : kMaxParts; }
+uint64_t norm_backward_temp(uint64_t rows, uint64_t cols)
+{
+    return rows && cols ? kStatusBytes + align_up(norm_parts(rows) * 2 * cols * sizeof(float), 256) : 0;
+}
+
+template <class T, class W, bool ADD>
+int norm_backward_launch(const NormGradArgs &a, W *grad_weight, W *grad_bias, hipStream_t s)
+{
+    const uint32_t octets = (uint32_t)ceil_div(a.cols, kOctet);
+    const char *name = ADD ? "layer_norm_add_backward" : "layer_norm_backward";
+    uint32_t parts = 0;
+    const bool fits = norm_backward_shape(octets, [&](auto nt, auto k) {
+        constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
+        constexpr int THREADS = NT > 512 ? NT : 512;
+        parts = (uint32_t)std::min<uint64_t>(ceil_div(a.rows, THREADS / NT), kMaxParts);
+        LCPP_LAUNCH(name, s, norm_backward_kernel<T, W, NT, K, THREADS, ADD><<<parts, THREADS, 0, s>>>(a));
+    });
+    if (!fits) {
+        if (a.partial) {
+            parts = (uint32_t)std::min<uint64_t>(norm_parts(a.rows), 128);
+            const dim3 grid((uint32_t)ceil_div(octets, kColThreads), parts);
+            LCPP_LAUNCH("layer_norm_backward_cols", s, norm_backward_cols_kernel<T><<<grid, kColThreads, 0, s>>>(a));
+        }
+        LCPP_LAUNCH(name, s, norm_backward_long_kernel<T, W, ADD><<<(uint32_t)std::min<uint64_t>(a.rows, kMaxGroups), kLongThreads, 0, s>>>(a));
+    }
+    if (a.partial)
+        LCPP_LAUNCH("layer_norm_fold", s,
+                    norm_fold_kernel<W><<<dim3((uint32_t)ceil_div(a.cols, kWave), 2), kFoldWaves * kWave, 0, s>>>(
+                        a.partial, parts, a.cols, grad_weight, grad_bias));
+    LCPP_CHECK_LAUNCH();
+    return LCPP_OK;
+}
+
+template <class W>
+__global__ void norm_zero_kernel(W *x, W *y, uint32_t n)
+{
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+        if (x) x[i] = (W)0.0f;
+        if (y) y[i] = (W)0.0f;
+    }
+}
+
+// The rows' type, and the weights' type, which is the same or float32.
+template <class F>
+int norm_dispatch(lcpp_dtype t, lcpp_dtype wt, F f)
+{
+    if (wt != t && wt != LCPP_FLOAT32) return LCPP_ERR_UNSUPPORTED_DTYPE;
+    return float_dispatch(t, [&](auto x) -> int {
+        using T = decltype(x);
+        if (wt == t) return f(x, x);
+        if constexpr (!std::is_same_v<T, float>) return f(x, float());
+        return LCPP_ERR_UNSUPPORTED_DTYPE;
+    });
+}
+
+bool norm_pointer(const void *p, size_t size, bool needed) { return p ? elem_ok(p, size) : !needed; }
+
+int norm_forward(lcpp_dtype t, lcpp_dtype wt, bool add, const NormArgs &a, uint64_t rows, uint64_t cols, hipStream_t s)
+{
+    const size_t e = float_size(t), we = float_size(wt);
+    if (!e || !we || (wt != t && wt != LCPP_FLOAT32)) return LCPP_ERR_UNSUPPORTED_DTYPE;
+    if (rows > kMaxRows || cols > kMaxCols) return LCPP_ERR_INVALID_ARG;
+    if (rows == 0 || cols == 0) return LCPP_OK;
+    if (!elem_ok(a.in, e) || !elem_ok(a.out, e) || !rows_apart(a.out_stride, rows, cols)) return LCPP_ERR_INVALID_ARG;
+    if (!norm_pointer(a.weight, we, false) || !norm_pointer(a.bias, we, false)) return LCPP_ERR_INVALID_ARG;
+    if (!norm_pointer(a.mean, 4, false) || !norm_pointer(a.rstd, 4, false)) return LCPP_ERR_INVALID_ARG;
+    if (!(a.eps >= 0.0f)) return LCPP_ERR_INVALID_ARG;
+    if (add && (!elem_ok(a.residual, e) || !elem_ok(a.sum, e) || !rows_apart(a.sum_stride, rows, cols)))
+        return LCPP_ERR_INVALID_ARG;
+    return norm_dispatch(t, wt, [&](auto x, auto w) -> int {
+        using T = decltype(x);
+        using W = decltype(w);
+        return add ? norm_forward_launch<T, W, true>(a, s) : norm_forward_launch<T, W, false>(a, s);
+    });
+}
+
+int norm_backward(lcpp_dtype t, lcpp_dtype wt, bool add, void *temp, size_t temp_bytes, NormGradArgs &a,
+                  void *grad_weight, void *grad_bias, uint64_t rows, uint64_t cols, hipStream_t s)
+{
+    const size_t e = float_size(t), we = float_size(wt);
+    if (!e || !we || (wt != t && wt != LCPP_FLOAT32)) return LCPP_ERR_UNSUPPORTED_DTYPE;
+    if (rows > kMaxRows || cols > kMaxCols) return LCPP_ERR_INVALID_ARG;
+    if (cols == 0) return LCPP_OK;
+    if (!norm_pointer(grad_weight, we, false) || !norm_pointer(grad_bias, we, false)) return LCPP_ERR_INVALID_ARG;
+    if (rows == 0) {  // sums over no rows
+        if (!grad_weight && !grad_bias) return LCPP_OK;
+        // (the temp query is 0 for no rows: temp holds no status word)
+        return norm_dispatch(t, wt, [&](auto, auto w) -> int {
+            using W = decltype(w);
+            LCPP_LAUNCH("layer_norm_zero", s,
+                        norm_zero_kernel<W><<<(uint32_t)std::min<uint64_t>(ceil_div(cols, 256), 1024), 256, 0, s>>>(
+                            static_cast<W *>(grad_weight), static_cast<W *>(grad_bias), (uint32_t)cols));
+            LCPP_CHECK_LAUNCH();
+            return LCPP_OK;
+        });
+    }
+    if (!elem_ok(a.grad_out, e) || !elem_ok(a.in, e) || !elem_ok(a.mean, 4) || !elem_ok(a.rstd, 4))
+        return LCPP_ERR_INVALID_ARG;
+    if (!norm_pointer(a.weight, we, false) || !norm_pointer(a.grad_sum, e, false)) return LCPP_ERR_INVALID_ARG;
+    if (!norm_pointer(a.grad_in, e, !add) || !norm_pointer(a.grad_branch, e, false)) return LCPP_ERR_INVALID_ARG;
+    if (a.grad_in && !rows_apart(a.gi_stride, rows, cols)) return LCPP_ERR_INVALID_ARG;
+    if (a.grad_branch && !rows_apart(a.gb_stride, rows, cols)) return LCPP_ERR_INVALID_ARG;
+    if (grad_weight || grad_bias) {
+        if (temp_bytes < norm_backward_temp(rows, cols)) return LCPP_ERR_TEMP_TOO_SMALL;
+        if (!temp || (reinterpret_cast<uintptr_t>(temp) & 255)) return LCPP_ERR_INVALID_ARG;
+        a.partial = reinterpret_cast<float *>(static_cast<char *>(temp) + kStatusBytes);
+    }
+    if (temp && temp_bytes >= kStatusBytes && !(reinterpret_cast<uintptr_t>(temp) & 255))
+        a.status = static_cast<uint32_t *>(temp);
+    return norm_dispatch(t, wt, [&](auto x, auto w) -> int {
+        using T = decltype(x);
+        using W = decltype(w);
+        W *gw = static_cast<W *>(grad_weight), *gb = static_cast<W *>(grad_bias);
+        return add ? norm_backward_launch<T, W, true>(a, gw, gb, s) : norm_backward_launch<T, W, false>(a, gw, gb, s);
+    });
+}
+
+}  // namespace
+}  // namespace lcpp
+
+using namespace lcpp;
+
+extern "C" int lcpp_layer_norm_forward(lcpp_dtype t, lcpp_dtype wt, const void *in, uint64_t in_stride,
+                                       const void *weight, const void *bias, float eps, void *out, uint64_t out_stride,
+                                       float *mean, float *rstd, uint64_t rows, uint64_t cols, void *stream)
+{
+    NormArgs a = {};
+    a.in = in, a.weight = weight, a.bias = bias, a.out = out;
+    a.in_stride = in_stride, a.out_stride = out_stride;
+    a.mean = mean, a.rstd = rstd, a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.eps = eps;
+    return norm_forward(t, wt, false, a, rows, cols, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lcpp_layer_norm_add_forward(lcpp_dtype t, lcpp_dtype wt, const void *in, uint64_t in_stride,
+                                           const void *residual, uint64_t residual_stride, double p, uint64_t seed,
+                                           uint64_t offset, const uint64_t *offset_dev, const void *weight,
+                                           const void *bias, float eps, void *sum, uint64_t sum_stride, void *out,
+                                           uint64_t out_stride, float *mean, float *rstd, uint64_t rows, uint64_t cols,
+                                           void *stream)
+{
+    NormArgs a = {};
+    if (!drop_args(p, seed, offset, offset_dev, &a.drop)) return LCPP_ERR_INVALID_ARG;
+    a.in = in, a.residual = residual, a.weight = weight, a.bias = bias, a.sum = sum, a.out = out;
+    a.in_stride = in_stride, a.residual_stride = residual_stride, a.sum_stride = sum_stride, a.out_stride = out_stride;
+    a.mean = mean, a.rstd = rstd, a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.eps = eps;
+    return norm_forward(t, wt, true, a, rows, cols, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lcpp_layer_norm_backward_temp_bytes(lcpp_dtype t, uint64_t rows, uint64_t cols, size_t *bytes)
+{
+    if (!bytes || rows > kMaxRows || cols > kMaxCols) return LCPP_ERR_INVALID_ARG;
+    if (!float_size(t)) return LCPP_ERR_UNSUPPORTED_DTYPE;
+    *bytes = norm_backward_temp(rows, cols);
+    return LCPP_OK;
+}
+
+extern "C" int lcpp_layer_norm_backward(lcpp_dtype t, lcpp_dtype wt, void *temp, size_t temp_bytes, const void *grad_out,
+                                        uint64_t grad_out_stride, const void *in, uint64_t in_stride, const void *weight,
+                                        const float *mean, const float *rstd, void *grad_in, uint64_t grad_in_stride,
+                                        void *grad_weight, void *grad_bias, uint64_t rows, uint64_t cols, void *stream)
+{
+    NormGradArgs a = {};
+    a.grad_out = grad_out, a.in = in, a.weight = weight, a.grad_in = grad_in;
+    a.go_stride = grad_out_stride, a.in_stride = in_stride, a.gi_stride = grad_in_stride;
+    a.mean = mean, a.rstd = rstd, a.rows = (uint32_t)rows, a.cols = (uint32_t)cols;
+    return norm_backward(t, wt, false, temp, temp_bytes, a, grad_weight, grad_bias, rows, cols,
+                         static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lcpp_layer_norm_add_backward(lcpp_dtype t, lcpp_dtype wt, void *temp, size_t temp_bytes,
+                                            const void *grad_out, uint64_t grad_out_stride, const void *grad_sum,
+                                            uint64_t grad_sum_stride, const void *sum, uint64_t sum_stride,
+                                            const void *weight, const float *mean, const float *rstd, double p,
+                                            uint64_t seed, uint64_t offset, const uint64_t *offset_dev,
+                                            void *grad_residual, uint64_t grad_residual_stride, void *grad_in,
+                                            uint64_t grad_in_stride, void *grad_weight, void *grad_bias, uint64_t rows,
+                                            uint64_t cols, void *stream)
+{
+    NormGradArgs a = {};
+    if (!drop_args(p, seed, offset, offset_dev, &a.drop)) return LCPP_ERR_INVALID_ARG;
+    a.grad_out = grad_out, a.grad_sum = grad_sum, a.in = sum, a.weight = weight;
+    a.grad_in = grad_residual, a.grad_branch = grad_in;
+    a.go_stride = grad_out_stride, a.gs_stride = grad_sum_stride, a.in_stride = sum_stride;
+    a.gi_stride = grad_residual_stride, a.gb_stride = grad_in_stride;
+    a.mean = mean, a.rstd = rstd, a.rows = (uint32_t)rows, a.cols = (uint32_t)cols;
+    return norm_backward(t, wt, true, temp, temp_bytes, a, grad_weight, grad_bias, rows, cols,
+                         static_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,667 @@
+// recurrence.hip — the gated linear recurrence h_t = a_t h_{t-1} + b_t over long
+// sequences, per channel, its gradient, and its step for single tokens.
+//
+//   gate "decay":    a = g,          b = x
+//   gate "log":      a = exp(g),     b = x
+//   gate "sigmoid":  a = sigmoid(g), b = (1 - a) x = sigmoid(-g) x
+//
+// A step is the affine map h -> a h + b, and maps compose: rows r..s together
+// are h -> A h + H with A the product of their a and H what they make of h = 0.
+// So time is cut into tiles of kTileRows rows, a workgroup for each tile and 64
+// lanes' channels: every wave takes kRows rows and folds them to (A, H), the waves
+// meet in LDS, tiles by decoupled look-back, and with h before its first row in
+// hand every wave runs through its rows, which wait in registers: the inputs
+// are read once.
+//
+// Backward, with dh_t the whole gradient of h_t and e_t = a_t dh_t what of it
+// reaches h_{t-1}:
+//   dh_t = dy_t + e_{t+1},   e_t = a_t e_{t+1} + a_t dy_t
+// which is a recurrence of the same form from the last row to the first, with the
+// same products A; e past the last row is the gradient of the final state, and e
+// of the first row is the gradient of the initial state.  The gate's gradient
+// needs h_{t-1}: the forward pass keeps the state before each tile (one row in
+// kTileRows, in 32 bits) and the backward tile runs through its rows again, which
+// is exact to 32 bits and reads no output.
+//   "decay":    dg = dh h_{t-1},                   dx = dh
+//   "log":      dg = dh h_{t-1} a,                 dx = dh
+//   "sigmoid":  dg = dh (h_{t-1} - x) a (1 - a),   dx = dh (1 - a)
+#include <algorithm>
+
+#include "lookback.hpp"
+#include "tensor.hpp"
+
+namespace lcpp {
+namespace {
+
+constexpr int kRows = 16;   // rows of a wave
+constexpr int kWaves = 8;   // waves of a full tile
+constexpr int kTileRows = kRows * kWaves;
+
+struct RowsIn {
+    const void *p;
+    uint64_t row, seq;  // strides in elements (seq 0 with begin and end)
+};
+struct RowsOut {
+    void *p;
+    uint64_t row, seq;
+};
+struct RecArgs {
+    RowsIn gate, in, grad_out;
+    RowsOut out, grad_gate, grad_in;
+    const float *initial, *grad_final;     // [sequence][channel]
+    float *final_state, *grad_initial;     // [sequence][channel]
+    float *checkpoints;                    // [sequence][tile][channel]
+    const uint32_t *begin, *end;           // null: sequence s begins at its stride, with max_length rows
+    uint64_t rows;                         // with begin and end: rows of the tensors
+    uint32_t sequences, tiles, groups, channels, max_length;
+    uint64_t *words;                       // [sequence][tile][group][lane channels]
+    WaitCtl ctl;
+};
+
+// ---------------------------------------------------------------- gates
+struct GateDecay {
+    static constexpr bool kShare = false;  // b is x itself
+    __device__ static __forceinline__ void eval(float g, float &a, float &share) { a = g, share = 1.0f; }
+    __device__ static __forceinline__ float grad(float dh, float before, float, float, float) { return dh * before; }
+};
+struct GateLog {
+    static constexpr bool kShare = false;
+    __device__ static __forceinline__ void eval(float g, float &a, float &share) { a = __expf(g), share = 1.0f; }
+    __device__ static __forceinline__ float grad(float dh, float before, float, float a, float) { return dh * before * a; }
+};
+struct GateSigmoid {
+    static constexpr bool kShare = true;
+    // 1 - a is computed as sigmoid(-g): as a difference it would lose what a has
+    // near 1.  exp(-|g|) cannot overflow.
+    __device__ static __forceinline__ void eval(float g, float &a, float &share)
+    {
+        const float e = __expf(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+        a = g >= 0.0f ? r : er;
+        share = g >= 0.0f ? er : r;
+    }
+    __device__ static __forceinline__ float grad(float dh, float before, float x, float a, float share)
+    {
+        return dh * (before - x) * (a * share);
+    }
+};
+
+// ---------------------------------------------------------------- tiles
+// Where a workgroup's lanes work.  A lane has C channels; the last lanes of a
+// last group are moved back so that they lie inside the row, and compute and
+// store what their neighbours do (the same values).  Every access is in bounds
+// as long as there are C channels.
+struct Place {
+    uint32_t seq, tile, len, channel;
+    bool active;
+    uint64_t row;  // of the tensors' rows that the sequence begins at (with offsets)
+};
+template <int C>
+__device__ __forceinline__ bool find_place(const RecArgs &a, bool reverse, Place &p)
+{
+    const uint32_t b = blockIdx.x;
+    const uint32_t group = b % a.groups, rest = b / a.groups;
+    p.seq = rest % a.sequences;
+    const uint32_t k = rest / a.sequences;
+    p.row = 0;
+    p.len = a.max_length;
+    if (a.begin) {
+        const uint64_t first = a.begin[p.seq];
+        const uint64_t end = a.end[p.seq] < a.rows ? a.end[p.seq] : a.rows;
+        const uint64_t n = end > first ? end - first : 0;
+        p.row = first;
+        p.len = n < a.max_length ? (uint32_t)n : a.max_length;
+    }
+    const uint32_t tiles = (p.len + kTileRows - 1) / kTileRows;
+    if (k >= tiles && !(k == 0 && tiles == 0)) return false;
+    p.tile = reverse && tiles ? tiles - 1 - k : k;
+    const uint32_t c = group * (kWave * C) + lane_id() * C;
+    p.active = c < a.channels;
+    p.channel = c + C <= a.channels ? c : a.channels - C;
+    return true;
+}
+template <class T>
+__device__ __forceinline__ const T *row_in(const RowsIn &t, const Place &p)
+{
+    return static_cast<const T *>(t.p) + p.row * t.row + p.seq * t.seq + p.channel;
+}
+
+template <class T>
+__device__ __forceinline__ T *row_out(const RowsOut &t, const Place &p)
+{
+    return static_cast<T *>(t.p) + p.row * t.row + p.seq * t.seq + p.channel;
+}
+
+// The packed look-back word of a channel: the map (A, H) of a tile (PARTIAL), or
+// the state after it (INCLUSIVE), in one 64-bit store.  The upper half is A's
+// bits inverted, so cleared memory is a NaN with all bits set, which no tile
+// publishes (a NaN A is stored as 0x7FC00000); another such NaN marks a state.
+constexpr uint32_t kWordState = 1;
+__device__ __forceinline__ uint64_t word_map(float A, float H)
+{
+    const uint32_t bits = A == A ? __builtin_bit_cast(uint32_t, A) : 0x7FC00000u;
+    return (uint64_t)~bits << 32 | __builtin_bit_cast(uint32_t, H);
+}
+__device__ __forceinline__ uint64_t word_state(float h)
+{
+    return (uint64_t)kWordState << 32 | __builtin_bit_cast(uint32_t, h);
+}
+
+template <int C>
+struct Chan {
+    float v[C];
+};
+
+// What the tiles before this one (in the order of the walk) make of the
+// sequence's first state.  Called by one wave; `words` are those of this tile's
+// channels, `step` is the distance to the next tile's.
+template <int C>
+__device__ __forceinline__ Chan<C> look_back(const uint64_t *words, int64_t step, uint32_t before, const WaitCtl &ctl)
+{
+    Chan<C> A, H;
+    bool done[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) A.v[c] = 1.0f, H.v[c] = 0.0f, done[c] = false;
+    uint32_t spins = 0;
+    for (uint32_t k = 1; k <= before;) {
+        uint64_t w[C];
+        bool ready = true;
+#pragma unroll
+        for (int c = 0; c < C; ++c) w[c] = ld_relaxed(words + (int64_t)k * step + c);
+#pragma unroll
+        for (int c = 0; c < C; ++c) ready = ready && (done[c] || (uint32_t)(w[c] >> 32) != 0);
+        if (ballot(!ready) != 0) {
+            if (++spins < ctl.spin_limit) {
+                __builtin_amdgcn_s_sleep(1);
+                continue;
+            }
+            if (lane_id() == 0) report_timeout(ctl);
+            break;
+        }
+        bool all = true;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const uint32_t up = (uint32_t)(w[c] >> 32);
+            const float low = __builtin_bit_cast(float, (uint32_t)w[c]);
+            if (!done[c]) {
+                H.v[c] += A.v[c] * low;
+                A.v[c] *= __builtin_bit_cast(float, ~up);
+                done[c] = up == kWordState;
+            }
+            all = all && done[c];
+        }
+        if (ballot(!all) == 0) break;
+        ++k;
+    }
+    return H;
+}
+
+template <class T, int C>
+__device__ __forceinline__ void store_chan(T *p, const Chan<C> &x)
+{
+    store_pack<C>(p, x.v);
+}
+
+template <class T, class G, int C, int W>
+__global__ __launch_bounds__(W *kWave) void rec_forward_kernel(RecArgs a)
+{
+    __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave];
+    Place p;
+    if (!find_place<C>(a, false, p)) return;
+    const uint32_t wave = threadIdx.x / kWave, lane = lane_id();
+    const uint64_t state_at = (uint64_t)p.seq * a.channels + p.channel;
+    const uint32_t first = p.tile * kTileRows + wave * kRows;
+    const uint32_t last = p.len ? p.len - 1 : 0;
+    const T *gp = row_in<T>(a.gate, p), *xp = row_in<T>(a.in, p);
+
+    Pack<T, C> gr[kRows], xr[kRows];
+    if (p.len) {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const uint64_t t = first + r < last ? first + r : last;  // (rows past the end are not used)
+            gr[r] = load_pack<C>(gp + t * a.gate.row);
+            xr[r] = load_pack<C>(xp + t * a.in.row);
+        }
+    }
+    Chan<C> ga[kRows], gb[kRows], A, H;
+#pragma unroll
+    for (int c = 0; c < C; ++c) A.v[c] = 1.0f, H.v[c] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const bool in = first + r < p.len;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float al, share;
+            G::eval(gr[r][c], al, share);
+            ga[r].v[c] = in ? al : 1.0f;
+            gb[r].v[c] = in ? (G::kShare ? share * xr[r][c] : xr[r][c]) : 0.0f;
+            H.v[c] = ga[r].v[c] * H.v[c] + gb[r].v[c];
+            A.v[c] *= ga[r].v[c];
+        }
+    }
+    s_A[wave][lane] = A;
+    s_H[wave][lane] = H;
+    __syncthreads();
+    if (wave == 0) {
+        const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
+        const uint32_t group = blockIdx.x % a.groups;
+        uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.tile) * tile_words + (uint64_t)group * kWave * C + lane * C;
+        const bool more = ((uint64_t)p.tile + 1) * kTileRows < p.len;  // a tile follows
+        Chan<C> tA = A, tH = H;
+#pragma unroll
+        for (int w = 1; w < W; ++w)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                tH.v[c] = s_A[w][lane].v[c] * tH.v[c] + s_H[w][lane].v[c];
+                tA.v[c] *= s_A[w][lane].v[c];
+            }
+        const bool publish = blockIdx.x != a.ctl.withhold;
+        Chan<C> h;
+        if (p.tile == 0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) h.v[c] = a.initial ? a.initial[state_at + c] : 0.0f;
+        } else {
+            if (more && publish) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) st_relaxed(words + c, word_map(tA.v[c], tH.v[c]));
+            }
+            h = look_back<C>(words, -(int64_t)tile_words, p.tile, a.ctl);
+        }
+        Chan<C> after;
+#pragma unroll
+        for (int c = 0; c < C; ++c) after.v[c] = tA.v[c] * h.v[c] + tH.v[c];
+        if (more && publish) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) st_relaxed(words + c, word_state(after.v[c]));
+        }
+        if (p.active) {
+            if (a.checkpoints && p.len)
+                store_chan(a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels + p.channel, h);
+            if (a.final_state && !p.len) store_chan(a.final_state + state_at, h);
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const Chan<C> wA = s_A[w][lane], wH = s_H[w][lane];
+            s_H[w][lane] = h;
+#pragma unroll
+            for (int c = 0; c < C; ++c) h.v[c] = wA.v[c] * h.v[c] + wH.v[c];
+        }
+    }
+    __syncthreads();
+    Chan<C> h = s_H[wave][lane];
+    T *yp = row_out<T>(a.out, p);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) h.v[c] = ga[r].v[c] * h.v[c] + gb[r].v[c];
+        if (first + r < p.len && p.active) store_pack<C>(yp + (uint64_t)(first + r) * a.out.row, h.v);
+    }
+    // (rows past the end left h as it was)
+    if (a.final_state && p.active && p.len && first <= last && last - first < kRows)
+        store_chan(a.final_state + state_at, h);
+}
+
+// The same tiles from the last to the first.  h before the tile is the forward
+// pass's checkpoint, so only e is looked back for.
+template <class T, class G, int C, int W>
+__global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
+{
+    __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_E[W][kWave];
+    Place p;
+    if (!find_place<C>(a, true, p)) return;
+    const uint32_t wave = threadIdx.x / kWave, lane = lane_id();
+    const uint64_t state_at = (uint64_t)p.seq * a.channels + p.channel;
+    if (p.len == 0) {  // nothing lies between the final and the initial state
+        if (wave == 0 && a.grad_initial && p.active) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                a.grad_initial[state_at + c] = a.grad_final ? a.grad_final[state_at + c] : 0.0f;
+        }
+        return;
+    }
+    const uint32_t first = p.tile * kTileRows + wave * kRows;
+    const uint32_t last = p.len - 1;
+    const T *gp = row_in<T>(a.gate, p), *xp = row_in<T>(a.in, p), *dyp = row_in<T>(a.grad_out, p);
+
+    Pack<T, C> gr[kRows], xr[kRows], dyr[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const uint64_t t = first + r < last ? first + r : last;  // (rows past the end are not used)
+        gr[r] = load_pack<C>(gp + t * a.gate.row);
+        xr[r] = load_pack<C>(xp + t * a.in.row);
+        dyr[r] = load_pack<C>(dyp + t * a.grad_out.row);
+    }
+    // the wave's rows as one map, forward (A, H) and backward (A, E)
+    Chan<C> A, H, E;
+#pragma unroll
+    for (int c = 0; c < C; ++c) A.v[c] = 1.0f, H.v[c] = 0.0f, E.v[c] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        if (first + r < p.len) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float al, share;
+                G::eval(gr[r][c], al, share);
+                H.v[c] = al * H.v[c] + (G::kShare ? share * xr[r][c] : xr[r][c]);
+                A.v[c] *= al;
+                // e before the rows: the last row's share comes first, times all a up to it
+                E.v[c] += A.v[c] * dyr[r][c];
+            }
+        }
+    }
+    s_A[wave][lane] = A;
+    s_H[wave][lane] = H;
+    s_E[wave][lane] = E;
+    __syncthreads();
+    if (wave == 0) {
+        const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
+        const uint32_t group = blockIdx.x % a.groups;
+        const uint32_t tiles = (p.len + kTileRows - 1) / kTileRows;
+        uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.tile) * tile_words + (uint64_t)group * kWave * C + lane * C;
+        const bool publish = p.tile > 0 && blockIdx.x != a.ctl.withhold;
+        Chan<C> tA, tE;
+#pragma unroll
+        for (int c = 0; c < C; ++c) tA.v[c] = 1.0f, tE.v[c] = 0.0f;
+#pragma unroll
+        for (int w = W - 1; w >= 0; --w)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                tE.v[c] = s_A[w][lane].v[c] * tE.v[c] + s_E[w][lane].v[c];
+                tA.v[c] *= s_A[w][lane].v[c];
+            }
+        Chan<C> e;
+        if (p.tile + 1 == tiles) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) e.v[c] = a.grad_final ? a.grad_final[state_at + c] : 0.0f;
+        } else {
+            if (publish) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) st_relaxed(words + c, word_map(tA.v[c], tE.v[c]));
+            }
+            e = look_back<C>(words, (int64_t)tile_words, tiles - 1 - p.tile, a.ctl);
+        }
+        Chan<C> before;
+#pragma unroll
+        for (int c = 0; c < C; ++c) before.v[c] = tA.v[c] * e.v[c] + tE.v[c];
+        if (publish) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) st_relaxed(words + c, word_state(before.v[c]));
+        }
+        if (p.tile == 0 && a.grad_initial && p.active) store_chan(a.grad_initial + state_at, before);
+#pragma unroll
+        for (int w = W - 1; w >= 0; --w) {
+            const Chan<C> wA = s_A[w][lane], wE = s_E[w][lane];
+            s_E[w][lane] = e;
+#pragma unroll
+            for (int c = 0; c < C; ++c) e.v[c] = wA.v[c] * e.v[c] + wE.v[c];
+        }
+        const float *saved = a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels + p.channel;
+        Chan<C> h;
+#pragma unroll
+        for (int c = 0; c < C; ++c) h.v[c] = saved[c];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const Chan<C> wA = s_A[w][lane], wH = s_H[w][lane];
+            s_H[w][lane] = h;
+#pragma unroll
+            for (int c = 0; c < C; ++c) h.v[c] = wA.v[c] * h.v[c] + wH.v[c];
+        }
+    }
+    __syncthreads();
+    Chan<C> h = s_H[wave][lane], e = s_E[wave][lane], before[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        before[r] = h;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float al, share;
+            G::eval(gr[r][c], al, share);
+            h.v[c] = al * h.v[c] + (G::kShare ? share * xr[r][c] : xr[r][c]);
+        }
+    }
+    T *dgp = row_out<T>(a.grad_gate, p), *dxp = row_out<T>(a.grad_in, p);
+#pragma unroll
+    for (int r = kRows - 1; r >= 0; --r) {
+        if (first + r < p.len) {
+            float dg[C], dx[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float al, share;
+                G::eval(gr[r][c], al, share);
+                const float dh = dyr[r][c] + e.v[c];
+                dg[c] = G::grad(dh, before[r].v[c], xr[r][c], al, share);
+                dx[c] = G::kShare ? dh * share : dh;
+                e.v[c] = al * dh;
+            }
+            if (p.active) {
+                store_pack<C>(dgp + (uint64_t)(first + r) * a.grad_gate.row, dg);
+                store_pack<C>(dxp + (uint64_t)(first + r) * a.grad_in.row, dx);
+            }
+        }
+    }
+}
+
+// One token for each of some sequences: h = a h + b on the states of a pool, at
+// slots that the caller names (or one behind the other).  A slot outside the
+// pool (a batch's padding) leaves every state alone and gives 0.
+struct StepArgs {
+    const void *gate, *in;
+    void *out;
+    uint64_t gate_stride, in_stride, out_stride;
+    const float *state_in;
+    float *state_out;
+    const int32_t *slots;
+    uint64_t num_slots;
+    uint64_t items;  // octets of all sequences
+    uint32_t channels, row_octets;
+};
+constexpr int kStepThreads = 256;
+template <class T, class G>
+__global__ __launch_bounds__(kStepThreads) void rec_step_kernel(StepArgs a)
+{
+    const uint64_t stride = (uint64_t)gridDim.x * kStepThreads;
+    for (uint64_t item = (uint64_t)blockIdx.x * kStepThreads + threadIdx.x; item < a.items; item += stride) {
+        const uint64_t seq = item / a.row_octets;
+        const uint32_t col = (uint32_t)(item - seq * a.row_octets) * kOctet;
+        const int64_t slot = a.slots ? (int64_t)a.slots[seq] : (int64_t)seq;
+        float y[kOctet] = {};
+        if (slot >= 0 && (uint64_t)slot < a.num_slots) {
+            const Octet<T> g = load_octet(static_cast<const T *>(a.gate) + seq * a.gate_stride, col, a.channels);
+            const Octet<T> x = load_octet(static_cast<const T *>(a.in) + seq * a.in_stride, col, a.channels);
+            const Octet<float> h = load_octet(a.state_in + (uint64_t)slot * a.channels, col, a.channels);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) {
+                float al, share;
+                G::eval(g[i], al, share);
+                y[i] = al * h[i] + (G::kShare ? share * x[i] : x[i]);
+            }
+            store_octet(a.state_out + (uint64_t)slot * a.channels, col, a.channels, y);
+        }
+        store_octet(static_cast<T *>(a.out) + seq * a.out_stride, col, a.channels, y);
+    }
+}
+
+// ---------------------------------------------------------------- launches
+template <class F>
+int gate_dispatch(lcpp_gate g, F f)
+{
+    switch (g) {
+    case LCPP_GATE_DECAY: return f(GateDecay());
+    case LCPP_GATE_LOG: return f(GateLog());
+    case LCPP_GATE_SIGMOID: return f(GateSigmoid());
+    default: return LCPP_ERR_INVALID_ARG;
+    }
+}
+
+// Channels of a lane: two, so that a wave's row is 256 or 512 bytes; one where
+// 64 lanes cover the channels.
+uint32_t rec_lane_channels(uint64_t channels) { return channels <= kWave ? 1 : 2; }
+struct RecShape {
+    uint64_t tiles, groups, words;
+};
+bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, RecShape *r)
+{
+    if (sequences > 0xFFFFFFFFull || max_length > 0x7FFFFFFFull || channels > kMaxCols) return false;
+    const uint64_t lanes = kWave * rec_lane_channels(channels);
+    r->groups = ceil_div(channels, lanes);
+    r->tiles = std::max<uint64_t>(ceil_div(max_length, kTileRows), 1);
+    // workgroups are numbered in 32 bits, and a launch has less than 2^32 threads
+    const uint64_t most = 0xFFFFFFFFull / (kWaves * kWave);
+    if (r->groups && (r->tiles > most / r->groups || sequences > most / (r->groups * r->tiles))) return false;
+    r->words = r->tiles > 1 ? sequences * r->tiles * r->groups * lanes : 0;
+    return true;
+}
+uint64_t rec_temp_bytes(const RecShape &r)
+{
+    return r.words ? kStatusBytes + align_up(r.words * sizeof(uint64_t), 256) : 0;
+}
+
+template <class T, class G, int C, int W>
+int rec_launch_waves(bool forward, const RecArgs &a, hipStream_t s)
+{
+    const uint32_t grid = a.sequences * a.tiles * a.groups;
+    if (forward) LCPP_LAUNCH("recurrence_forward", s, rec_forward_kernel<T, G, C, W><<<grid, W * kWave, 0, s>>>(a));
+    else LCPP_LAUNCH("recurrence_backward", s, rec_backward_kernel<T, G, C, W><<<grid, W * kWave, 0, s>>>(a));
+    LCPP_CHECK_LAUNCH();
+    return LCPP_OK;
+}
+// Sequences of one tile take no more waves than have rows.
+template <class T, class G, int C>
+int rec_launch(bool forward, const RecArgs &a, hipStream_t s)
+{
+    if (a.max_length <= kRows) return rec_launch_waves<T, G, C, 1>(forward, a, s);
+    if (a.max_length <= 4 * kRows) return rec_launch_waves<T, G, C, 4>(forward, a, s);
+    return rec_launch_waves<T, G, C, kWaves>(forward, a, s);
+}
+
+int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, RecArgs &a, uint64_t sequences,
+            uint64_t max_length, uint64_t channels, uint64_t rows, hipStream_t s)
+{
+    const size_t e = float_size(t);
+    if (!e) return LCPP_ERR_UNSUPPORTED_DTYPE;
+    if (g != LCPP_GATE_DECAY && g != LCPP_GATE_LOG && g != LCPP_GATE_SIGMOID) return LCPP_ERR_INVALID_ARG;
+    RecShape r;
+    if (!rec_shape(sequences, max_length, channels, &r) || (!a.begin) != (!a.end)) return LCPP_ERR_INVALID_ARG;
+    if (sequences == 0 || channels == 0) return LCPP_OK;
+    if (a.begin && (!elem_ok(a.begin, 4) || !elem_ok(a.end, 4))) return LCPP_ERR_INVALID_ARG;
+    auto optional = [](const void *p) { return !p || elem_ok(p, 4); };
+    if (!optional(a.initial) || !optional(a.final_state) || !optional(a.grad_final) || !optional(a.grad_initial) ||
+        !optional(a.checkpoints))
+        return LCPP_ERR_INVALID_ARG;
+    const bool some = max_length != 0 && (!a.begin || rows != 0);  // (else only the states are copied)
+    const uint64_t total = a.begin ? rows : max_length;
+    auto out_ok = [&](const RowsOut &o) {
+        return elem_ok(o.p, e) && rows_apart(o.row, total, channels) &&
+               (a.begin || rows_apart(o.seq, sequences, channels));
+    };
+    if (some) {
+        if (!elem_ok(a.gate.p, e) || !elem_ok(a.in.p, e)) return LCPP_ERR_INVALID_ARG;
+        if (forward ? !out_ok(a.out) : !(elem_ok(a.grad_out.p, e) && out_ok(a.grad_gate) && out_ok(a.grad_in) && a.checkpoints))
+            return LCPP_ERR_INVALID_ARG;
+    }
+    if (r.words) {
+        if (temp_bytes < rec_temp_bytes(r)) return LCPP_ERR_TEMP_TOO_SMALL;
+        if (!temp || (reinterpret_cast<uintptr_t>(temp) & 255)) return LCPP_ERR_INVALID_ARG;
+    }
+    a.sequences = (uint32_t)sequences, a.tiles = (uint32_t)r.tiles, a.groups = (uint32_t)r.groups;
+    a.channels = (uint32_t)channels, a.max_length = some ? (uint32_t)max_length : 0, a.rows = rows;
+    if (a.begin) a.gate.seq = a.in.seq = a.grad_out.seq = a.out.seq = a.grad_gate.seq = a.grad_in.seq = 0;
+    uint64_t *head = static_cast<uint64_t *>(temp);
+    if (r.words) {
+        a.words = head + kStatusBytes / 8;
+        a.ctl = wait_ctl(static_cast<uint32_t *>(temp));
+        const int rc = lb_init(head, kStatusBytes / 8 + r.words, s, "recurrence_init");
+        if (rc != LCPP_OK) return rc;
+    } else {
+        a.ctl = wait_ctl(nullptr);  // one tile a sequence: nothing waits
+    }
+    return float_dispatch(t, [&](auto x) -> int {
+        using T = decltype(x);
+        return gate_dispatch(g, [&](auto gate) {
+            using G = decltype(gate);
+            return rec_lane_channels(channels) == 1 ? rec_launch<T, G, 1>(forward, a, s) : rec_launch<T, G, 2>(forward, a, s);
+        });
+    });
+}
+
+}  // namespace
+}  // namespace lcpp
+
+using namespace lcpp;
+
+extern "C" int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes)
+{
+    RecShape r;
+    if (!bytes || !rec_shape(sequences, max_length, channels, &r)) return LCPP_ERR_INVALID_ARG;
+    *bytes = rec_temp_bytes(r);
+    return LCPP_OK;
+}
+
+extern "C" int lcpp_recurrence_checkpoint_rows(uint64_t max_length, uint64_t *rows)
+{
+    if (!rows || max_length > 0x7FFFFFFFull) return LCPP_ERR_INVALID_ARG;
+    *rows = std::max<uint64_t>(ceil_div(max_length, kTileRows), 1);
+    return LCPP_OK;
+}
+
+extern "C" int lcpp_recurrence_forward(lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, const void *gate,
+                                       uint64_t gate_row, uint64_t gate_seq, const void *in, uint64_t in_row,
+                                       uint64_t in_seq, void *out, uint64_t out_row, uint64_t out_seq,
+                                       const float *initial, float *final_state, float *checkpoints, uint64_t sequences,
+                                       uint64_t max_length, uint64_t channels, const uint32_t *begin,
+                                       const uint32_t *end, uint64_t rows, void *stream)
+{
+    RecArgs a = {};
+    a.gate = {gate, gate_row, gate_seq}, a.in = {in, in_row, in_seq}, a.out = {out, out_row, out_seq};
+    a.initial = initial, a.final_state = final_state, a.checkpoints = checkpoints, a.begin = begin, a.end = end;
+    return rec_run(true, t, g, temp, temp_bytes, a, sequences, max_length, channels, rows,
+                   static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lcpp_recurrence_backward(lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, const void *gate,
+                                        uint64_t gate_row, uint64_t gate_seq, const void *in, uint64_t in_row,
+                                        uint64_t in_seq, const float *checkpoints, const void *grad_out,
+                                        uint64_t grad_out_row, uint64_t grad_out_seq, void *grad_gate,
+                                        uint64_t grad_gate_row, uint64_t grad_gate_seq, void *grad_in,
+                                        uint64_t grad_in_row, uint64_t grad_in_seq, const float *grad_final,
+                                        float *grad_initial, uint64_t sequences, uint64_t max_length, uint64_t channels,
+                                        const uint32_t *begin, const uint32_t *end, uint64_t rows, void *stream)
+{
+    RecArgs a = {};
+    a.gate = {gate, gate_row, gate_seq}, a.in = {in, in_row, in_seq}, a.grad_out = {grad_out, grad_out_row, grad_out_seq};
+    a.grad_gate = {grad_gate, grad_gate_row, grad_gate_seq}, a.grad_in = {grad_in, grad_in_row, grad_in_seq};
+    a.checkpoints = const_cast<float *>(checkpoints), a.grad_final = grad_final, a.grad_initial = grad_initial;
+    a.begin = begin, a.end = end;
+    return rec_run(false, t, g, temp, temp_bytes, a, sequences, max_length, channels, rows,
+                   static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lcpp_recurrence_step(lcpp_dtype t, lcpp_gate g, const void *gate, uint64_t gate_stride, const void *in,
+                                    uint64_t in_stride, const float *state_in, float *state_out, const int32_t *slots,
+                                    uint64_t num_slots, void *out, uint64_t out_stride, uint64_t sequences,
+                                    uint64_t channels, void *stream)
+{
+    const size_t e = float_size(t);
+    if (!e) return LCPP_ERR_UNSUPPORTED_DTYPE;
+    if (g != LCPP_GATE_DECAY && g != LCPP_GATE_LOG && g != LCPP_GATE_SIGMOID) return LCPP_ERR_INVALID_ARG;
+    if (sequences > kMaxRows || channels > kMaxCols || num_slots > kMaxRows) return LCPP_ERR_INVALID_ARG;
+    if (sequences == 0 || channels == 0) return LCPP_OK;
+    if (!elem_ok(gate, e) || !elem_ok(in, e) || !elem_ok(out, e) || !rows_apart(out_stride, sequences, channels))
+        return LCPP_ERR_INVALID_ARG;
+    if (!elem_ok(state_in, 4) || !elem_ok(state_out, 4) || (slots && !elem_ok(slots, 4)) || (!slots && num_slots < sequences))
+        return LCPP_ERR_INVALID_ARG;
+    StepArgs a = {gate, in, out, gate_stride, in_stride, out_stride, state_in, state_out, slots, num_slots, 0, 0, 0};
+    a.channels = (uint32_t)channels;
+    a.row_octets = (uint32_t)ceil_div(channels, kOctet);
+    a.items = sequences * a.row_octets;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(ceil_div(a.items, kStepThreads), 1u << 20);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return float_dispatch(t, [&](auto x) -> int {
+        using T = decltype(x);
+        return gate_dispatch(g, [&](auto kind) -> int {
+            using G = decltype(kind);
+            LCPP_LAUNCH("recurrence_step", s, rec_step_kernel<T, G><<<grid, kStepThreads, 0, s>>>(a));
+            LCPP_CHECK_LAUNCH();
+            return LCPP_OK;
+        });
+    });
+}
