@@ -33,8 +33,8 @@
 namespace lcpp {
 namespace {
 
-constexpr int kRows = 16;   // rows of a wave
-constexpr int kWaves = 8;   // waves of a full tile
+constexpr int kRows = 16;  // rows of a wave
+constexpr int kWaves = 8;  // waves of a full tile
 constexpr int kTileRows = kRows * kWaves;
 
 struct RowsIn {
@@ -54,7 +54,7 @@ struct RecArgs {
     const uint32_t *begin, *end;           // null: sequence s begins at its stride, with max_length rows
     uint64_t rows;                         // with begin and end: rows of the tensors
     uint32_t sequences, tiles, groups, channels, max_length;
-    uint64_t *words;                       // [sequence][tile][group][lane channels]
+    uint64_t *words;                       // [sequence][tile of the walk][group][lane's channels]
     WaitCtl ctl;
 };
 
@@ -91,17 +91,21 @@ struct GateSigmoid {
 // store what their neighbours do (the same values).  Every access is in bounds
 // as long as there are C channels.
 struct Place {
-    uint32_t seq, tile, len, channel;
+    uint32_t seq, tile, len, channel, group;
+    uint32_t walk;  // tiles of the sequence before this one in the walk
     bool active;
     uint64_t row;  // of the tensors' rows that the sequence begins at (with offsets)
 };
+// Workgroups are numbered tile by tile, in a tile sequence by sequence, in a
+// sequence group by group, so a tile waits only on workgroups dispatched before
+// its own; `reverse` counts tiles from the sequence's end.
 template <int C>
 __device__ __forceinline__ bool find_place(const RecArgs &a, bool reverse, Place &p)
 {
-    const uint32_t b = blockIdx.x;
-    const uint32_t group = b % a.groups, rest = b / a.groups;
-    p.seq = rest % a.sequences;
+    const uint32_t rest = blockIdx.x / a.groups;
+    p.group = blockIdx.x - rest * a.groups;
     const uint32_t k = rest / a.sequences;
+    p.seq = rest - k * a.sequences;
     p.row = 0;
     p.len = a.max_length;
     if (a.begin) {
@@ -113,22 +117,26 @@ __device__ __forceinline__ bool find_place(const RecArgs &a, bool reverse, Place
     }
     const uint32_t tiles = (p.len + kTileRows - 1) / kTileRows;
     if (k >= tiles && !(k == 0 && tiles == 0)) return false;
+    p.walk = k;
     p.tile = reverse && tiles ? tiles - 1 - k : k;
-    const uint32_t c = group * (kWave * C) + lane_id() * C;
+    const uint32_t c = p.group * (kWave * C) + lane_id() * C;
     p.active = c < a.channels;
     p.channel = c + C <= a.channels ? c : a.channels - C;
     return true;
 }
+// (the wave's number as a scalar, so that row addresses are scalars too and a
+// lane holds nothing but its channel's offset)
+__device__ __forceinline__ uint32_t wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
 template <class T>
-__device__ __forceinline__ const T *row_in(const RowsIn &t, const Place &p)
+__device__ __forceinline__ const T *row_in(const RowsIn &t, const Place &p, uint64_t row)
 {
-    return static_cast<const T *>(t.p) + p.row * t.row + p.seq * t.seq + p.channel;
+    return static_cast<const T *>(t.p) + ((p.row + row) * t.row + p.seq * t.seq);
 }
 
 template <class T>
-__device__ __forceinline__ T *row_out(const RowsOut &t, const Place &p)
+__device__ __forceinline__ T *row_out(const RowsOut &t, const Place &p, uint64_t row)
 {
-    return static_cast<T *>(t.p) + p.row * t.row + p.seq * t.seq + p.channel;
+    return static_cast<T *>(t.p) + ((p.row + row) * t.row + p.seq * t.seq);
 }
 
 // The packed look-back word of a channel: the map (A, H) of a tile (PARTIAL), or
@@ -151,11 +159,11 @@ struct Chan {
     float v[C];
 };
 
-// What the tiles before this one (in the order of the walk) make of the
-// sequence's first state.  Called by one wave; `words` are those of this tile's
-// channels, `step` is the distance to the next tile's.
+// What the tiles before this one in the walk make of the sequence's first state:
+// their maps composed up to the nearest state.  One wave calls it; `words` are
+// those of this tile's channels, `step` is the distance to the tile before it.
 template <int C>
-__device__ __forceinline__ Chan<C> look_back(const uint64_t *words, int64_t step, uint32_t before, const WaitCtl &ctl)
+__device__ __forceinline__ Chan<C> look_back(const uint64_t *words, uint64_t step, uint32_t before, const WaitCtl &ctl)
 {
     Chan<C> A, H;
     bool done[C];
@@ -163,27 +171,27 @@ __device__ __forceinline__ Chan<C> look_back(const uint64_t *words, int64_t step
     for (int c = 0; c < C; ++c) A.v[c] = 1.0f, H.v[c] = 0.0f, done[c] = false;
     uint32_t spins = 0;
     for (uint32_t k = 1; k <= before;) {
+        words -= step;
         uint64_t w[C];
-        bool ready = true;
+        for (;;) {
+            bool ready = true;
 #pragma unroll
-        for (int c = 0; c < C; ++c) w[c] = ld_relaxed(words + (int64_t)k * step + c);
+            for (int c = 0; c < C; ++c) w[c] = ld_relaxed(words + c);
 #pragma unroll
-        for (int c = 0; c < C; ++c) ready = ready && (done[c] || (uint32_t)(w[c] >> 32) != 0);
-        if (ballot(!ready) != 0) {
-            if (++spins < ctl.spin_limit) {
-                __builtin_amdgcn_s_sleep(1);
-                continue;
+            for (int c = 0; c < C; ++c) ready = ready && (done[c] || (uint32_t)(w[c] >> 32) != 0);
+            if (ballot(!ready) == 0) break;
+            if (++spins >= ctl.spin_limit) {
+                if (lane_id() == 0) report_timeout(ctl);
+                return H;
             }
-            if (lane_id() == 0) report_timeout(ctl);
-            break;
+            __builtin_amdgcn_s_sleep(8);
         }
         bool all = true;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const uint32_t up = (uint32_t)(w[c] >> 32);
-            const float low = __builtin_bit_cast(float, (uint32_t)w[c]);
             if (!done[c]) {
-                H.v[c] += A.v[c] * low;
+                H.v[c] += A.v[c] * __builtin_bit_cast(float, (uint32_t)w[c]);
                 A.v[c] *= __builtin_bit_cast(float, ~up);
                 done[c] = up == kWordState;
             }
@@ -195,6 +203,20 @@ __device__ __forceinline__ Chan<C> look_back(const uint64_t *words, int64_t step
     return H;
 }
 
+// One wave publishes its tile's map, and then the state after it.
+template <int C>
+__device__ __forceinline__ void publish_map(uint64_t *words, const Chan<C> &A, const Chan<C> &H)
+{
+#pragma unroll
+    for (int c = 0; c < C; ++c) st_relaxed(words + c, word_map(A.v[c], H.v[c]));
+}
+template <int C>
+__device__ __forceinline__ void publish_state(uint64_t *words, const Chan<C> &A, const Chan<C> &H, const Chan<C> &h)
+{
+#pragma unroll
+    for (int c = 0; c < C; ++c) st_relaxed(words + c, word_state(A.v[c] * h.v[c] + H.v[c]));
+}
+
 template <class T, int C>
 __device__ __forceinline__ void store_chan(T *p, const Chan<C> &x)
 {
@@ -202,102 +224,111 @@ __device__ __forceinline__ void store_chan(T *p, const Chan<C> &x)
 }
 
 template <class T, class G, int C, int W>
-__global__ __launch_bounds__(W *kWave) void rec_forward_kernel(RecArgs a)
+__global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) void rec_forward_kernel(RecArgs a)
 {
-    __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave];
+    __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_carry[kWave];
     Place p;
     if (!find_place<C>(a, false, p)) return;
-    const uint32_t wave = threadIdx.x / kWave, lane = lane_id();
+    const uint32_t wave = wave_id(), lane = lane_id();
     const uint64_t state_at = (uint64_t)p.seq * a.channels + p.channel;
     const uint32_t first = p.tile * kTileRows + wave * kRows;
     const uint32_t last = p.len ? p.len - 1 : 0;
-    const T *gp = row_in<T>(a.gate, p), *xp = row_in<T>(a.in, p);
+    const bool more = ((uint64_t)p.tile + 1) * kTileRows < p.len;  // a tile follows
+    const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
+    uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.walk) * tile_words + (uint64_t)p.group * kWave * C + lane * C;
 
-    Pack<T, C> gr[kRows], xr[kRows];
-    if (p.len) {
+    Chan<C> ga[kRows], gb[kRows], A, H;
+    {
+        Pack<T, C> gr[kRows], xr[kRows];
+        if (p.len) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const uint64_t t = first + r < last ? first + r : last;  // (rows past the end are not used)
+                gr[r] = load_pack_nt<C>(row_in<T>(a.gate, p, t) + p.channel);
+                xr[r] = load_pack_nt<C>(row_in<T>(a.in, p, t) + p.channel);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) A.v[c] = 1.0f, H.v[c] = 0.0f;
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-            const uint64_t t = first + r < last ? first + r : last;  // (rows past the end are not used)
-            gr[r] = load_pack<C>(gp + t * a.gate.row);
-            xr[r] = load_pack<C>(xp + t * a.in.row);
-        }
-    }
-    Chan<C> ga[kRows], gb[kRows], A, H;
+            const bool in = first + r < p.len;
 #pragma unroll
-    for (int c = 0; c < C; ++c) A.v[c] = 1.0f, H.v[c] = 0.0f;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-        const bool in = first + r < p.len;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float al, share;
-            G::eval(gr[r][c], al, share);
-            ga[r].v[c] = in ? al : 1.0f;
-            gb[r].v[c] = in ? (G::kShare ? share * xr[r][c] : xr[r][c]) : 0.0f;
-            H.v[c] = ga[r].v[c] * H.v[c] + gb[r].v[c];
-            A.v[c] *= ga[r].v[c];
+            for (int c = 0; c < C; ++c) {
+                float al, share;
+                G::eval(gr[r][c], al, share);
+                ga[r].v[c] = in ? al : 1.0f;
+                gb[r].v[c] = in ? (G::kShare ? share * xr[r][c] : xr[r][c]) : 0.0f;
+                H.v[c] = ga[r].v[c] * H.v[c] + gb[r].v[c];
+                A.v[c] *= ga[r].v[c];
+            }
         }
     }
     s_A[wave][lane] = A;
     s_H[wave][lane] = H;
     __syncthreads();
     if (wave == 0) {
-        const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
-        const uint32_t group = blockIdx.x % a.groups;
-        uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.tile) * tile_words + (uint64_t)group * kWave * C + lane * C;
-        const bool more = ((uint64_t)p.tile + 1) * kTileRows < p.len;  // a tile follows
-        Chan<C> tA = A, tH = H;
+        const bool publish = more && blockIdx.x != a.ctl.withhold;
+        if (publish) {
 #pragma unroll
-        for (int w = 1; w < W; ++w)
+            for (int w = 1; w < W; ++w)
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                tH.v[c] = s_A[w][lane].v[c] * tH.v[c] + s_H[w][lane].v[c];
-                tA.v[c] *= s_A[w][lane].v[c];
-            }
-        const bool publish = blockIdx.x != a.ctl.withhold;
+                for (int c = 0; c < C; ++c) {
+                    H.v[c] = s_A[w][lane].v[c] * H.v[c] + s_H[w][lane].v[c];
+                    A.v[c] *= s_A[w][lane].v[c];
+                }
+            if (p.walk > 0) publish_map<C>(words, A, H);
+        }
         Chan<C> h;
-        if (p.tile == 0) {
+        if (p.walk == 0) {
 #pragma unroll
             for (int c = 0; c < C; ++c) h.v[c] = a.initial ? a.initial[state_at + c] : 0.0f;
         } else {
-            if (more && publish) {
-#pragma unroll
-                for (int c = 0; c < C; ++c) st_relaxed(words + c, word_map(tA.v[c], tH.v[c]));
-            }
-            h = look_back<C>(words, -(int64_t)tile_words, p.tile, a.ctl);
+            h = look_back<C>(words, tile_words, p.walk, a.ctl);
         }
-        Chan<C> after;
-#pragma unroll
-        for (int c = 0; c < C; ++c) after.v[c] = tA.v[c] * h.v[c] + tH.v[c];
-        if (more && publish) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) st_relaxed(words + c, word_state(after.v[c]));
-        }
+        s_carry[lane] = h;
+        if (publish) publish_state<C>(words, A, H, h);
         if (p.active) {
             if (a.checkpoints && p.len)
                 store_chan(a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels + p.channel, h);
             if (a.final_state && !p.len) store_chan(a.final_state + state_at, h);
         }
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const Chan<C> wA = s_A[w][lane], wH = s_H[w][lane];
-            s_H[w][lane] = h;
-#pragma unroll
-            for (int c = 0; c < C; ++c) h.v[c] = wA.v[c] * h.v[c] + wH.v[c];
-        }
     }
     __syncthreads();
-    Chan<C> h = s_H[wave][lane];
-    T *yp = row_out<T>(a.out, p);
+    Chan<C> h = s_carry[lane];
+    for (uint32_t w = 0; w < wave; ++w)
+#pragma unroll
+        for (int c = 0; c < C; ++c) h.v[c] = s_A[w][lane].v[c] * h.v[c] + s_H[w][lane].v[c];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
 #pragma unroll
         for (int c = 0; c < C; ++c) h.v[c] = ga[r].v[c] * h.v[c] + gb[r].v[c];
-        if (first + r < p.len && p.active) store_pack<C>(yp + (uint64_t)(first + r) * a.out.row, h.v);
+        if (first + r < p.len && p.active) store_pack<C>(row_out<T>(a.out, p, first + r) + p.channel, h.v);
     }
     // (rows past the end left h as it was)
     if (a.final_state && p.active && p.len && first <= last && last - first < kRows)
         store_chan(a.final_state + state_at, h);
+}
+
+// Makes the compiler forget where a value came from: what is computed from it
+// before and after is computed twice instead of held in registers.
+template <class T, int N>
+__device__ __forceinline__ void forget(Pack<T, N> &x)
+{
+    if constexpr (sizeof(T) * N == 2) {
+        uint16_t b = __builtin_bit_cast(uint16_t, x.v);
+        asm volatile("" : "+v"(b));
+        x.v = __builtin_bit_cast(decltype(x.v), b);
+    } else if constexpr (sizeof(T) * N == 4) {
+        uint32_t b = __builtin_bit_cast(uint32_t, x.v);
+        asm volatile("" : "+v"(b));
+        x.v = __builtin_bit_cast(decltype(x.v), b);
+    } else {
+        static_assert(sizeof(T) * N == 8, "2, 4 or 8 bytes");
+        uint64_t b = __builtin_bit_cast(uint64_t, x.v);
+        asm volatile("" : "+v"(b));
+        x.v = __builtin_bit_cast(decltype(x.v), b);
+    }
 }
 
 // The same tiles from the last to the first.  h before the tile is the forward
@@ -305,10 +336,10 @@ __global__ __launch_bounds__(W *kWave) void rec_forward_kernel(RecArgs a)
 template <class T, class G, int C, int W>
 __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
 {
-    __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_E[W][kWave];
+    __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_E[W][kWave], s_carry[kWave];
     Place p;
     if (!find_place<C>(a, true, p)) return;
-    const uint32_t wave = threadIdx.x / kWave, lane = lane_id();
+    const uint32_t wave = wave_id(), lane = lane_id();
     const uint64_t state_at = (uint64_t)p.seq * a.channels + p.channel;
     if (p.len == 0) {  // nothing lies between the final and the initial state
         if (wave == 0 && a.grad_initial && p.active) {
@@ -320,15 +351,16 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     }
     const uint32_t first = p.tile * kTileRows + wave * kRows;
     const uint32_t last = p.len - 1;
-    const T *gp = row_in<T>(a.gate, p), *xp = row_in<T>(a.in, p), *dyp = row_in<T>(a.grad_out, p);
+    const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
+    uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.walk) * tile_words + (uint64_t)p.group * kWave * C + lane * C;
 
     Pack<T, C> gr[kRows], xr[kRows], dyr[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const uint64_t t = first + r < last ? first + r : last;  // (rows past the end are not used)
-        gr[r] = load_pack<C>(gp + t * a.gate.row);
-        xr[r] = load_pack<C>(xp + t * a.in.row);
-        dyr[r] = load_pack<C>(dyp + t * a.grad_out.row);
+        gr[r] = load_pack_nt<C>(row_in<T>(a.gate, p, t) + p.channel);
+        xr[r] = load_pack_nt<C>(row_in<T>(a.in, p, t) + p.channel);
+        dyr[r] = load_pack_nt<C>(row_in<T>(a.grad_out, p, t) + p.channel);
     }
     // the wave's rows as one map, forward (A, H) and backward (A, E)
     Chan<C> A, H, E;
@@ -353,64 +385,47 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     s_E[wave][lane] = E;
     __syncthreads();
     if (wave == 0) {
-        const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
-        const uint32_t group = blockIdx.x % a.groups;
-        const uint32_t tiles = (p.len + kTileRows - 1) / kTileRows;
-        uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.tile) * tile_words + (uint64_t)group * kWave * C + lane * C;
         const bool publish = p.tile > 0 && blockIdx.x != a.ctl.withhold;
-        Chan<C> tA, tE;
+        if (publish) {
+            A = s_A[W - 1][lane], E = s_E[W - 1][lane];
 #pragma unroll
-        for (int c = 0; c < C; ++c) tA.v[c] = 1.0f, tE.v[c] = 0.0f;
+            for (int w = W - 2; w >= 0; --w)
 #pragma unroll
-        for (int w = W - 1; w >= 0; --w)
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                tE.v[c] = s_A[w][lane].v[c] * tE.v[c] + s_E[w][lane].v[c];
-                tA.v[c] *= s_A[w][lane].v[c];
-            }
+                for (int c = 0; c < C; ++c) {
+                    E.v[c] = s_A[w][lane].v[c] * E.v[c] + s_E[w][lane].v[c];
+                    A.v[c] *= s_A[w][lane].v[c];
+                }
+            if (p.walk > 0) publish_map<C>(words, A, E);
+        }
         Chan<C> e;
-        if (p.tile + 1 == tiles) {
+        if (p.walk == 0) {
 #pragma unroll
             for (int c = 0; c < C; ++c) e.v[c] = a.grad_final ? a.grad_final[state_at + c] : 0.0f;
         } else {
-            if (publish) {
-#pragma unroll
-                for (int c = 0; c < C; ++c) st_relaxed(words + c, word_map(tA.v[c], tE.v[c]));
-            }
-            e = look_back<C>(words, (int64_t)tile_words, tiles - 1 - p.tile, a.ctl);
+            e = look_back<C>(words, tile_words, p.walk, a.ctl);
         }
-        Chan<C> before;
-#pragma unroll
-        for (int c = 0; c < C; ++c) before.v[c] = tA.v[c] * e.v[c] + tE.v[c];
-        if (publish) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) st_relaxed(words + c, word_state(before.v[c]));
-        }
-        if (p.tile == 0 && a.grad_initial && p.active) store_chan(a.grad_initial + state_at, before);
-#pragma unroll
-        for (int w = W - 1; w >= 0; --w) {
-            const Chan<C> wA = s_A[w][lane], wE = s_E[w][lane];
-            s_E[w][lane] = e;
-#pragma unroll
-            for (int c = 0; c < C; ++c) e.v[c] = wA.v[c] * e.v[c] + wE.v[c];
-        }
+        s_carry[lane] = e;
+        if (publish) publish_state<C>(words, A, E, e);
+    }
+    Chan<C> h, before[kRows];
+    {
         const float *saved = a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels + p.channel;
-        Chan<C> h;
 #pragma unroll
         for (int c = 0; c < C; ++c) h.v[c] = saved[c];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const Chan<C> wA = s_A[w][lane], wH = s_H[w][lane];
-            s_H[w][lane] = h;
-#pragma unroll
-            for (int c = 0; c < C; ++c) h.v[c] = wA.v[c] * h.v[c] + wH.v[c];
-        }
     }
     __syncthreads();
-    Chan<C> h = s_H[wave][lane], e = s_E[wave][lane], before[kRows];
+    Chan<C> e = s_carry[lane];
+    for (uint32_t w = W - 1; w > wave; --w)
+#pragma unroll
+        for (int c = 0; c < C; ++c) e.v[c] = s_A[w][lane].v[c] * e.v[c] + s_E[w][lane].v[c];
+    for (uint32_t w = 0; w < wave; ++w)
+#pragma unroll
+        for (int c = 0; c < C; ++c) h.v[c] = s_A[w][lane].v[c] * h.v[c] + s_H[w][lane].v[c];
+    // (the gates are evaluated three times: kept, they would take half of the register file's waves)
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         before[r] = h;
+        forget(gr[r]);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             float al, share;
@@ -418,9 +433,9 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
             h.v[c] = al * h.v[c] + (G::kShare ? share * xr[r][c] : xr[r][c]);
         }
     }
-    T *dgp = row_out<T>(a.grad_gate, p), *dxp = row_out<T>(a.grad_in, p);
 #pragma unroll
     for (int r = kRows - 1; r >= 0; --r) {
+        forget(gr[r]);
         if (first + r < p.len) {
             float dg[C], dx[C];
 #pragma unroll
@@ -433,11 +448,12 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
                 e.v[c] = al * dh;
             }
             if (p.active) {
-                store_pack<C>(dgp + (uint64_t)(first + r) * a.grad_gate.row, dg);
-                store_pack<C>(dxp + (uint64_t)(first + r) * a.grad_in.row, dx);
+                store_pack<C>(row_out<T>(a.grad_gate, p, first + r) + p.channel, dg);
+                store_pack<C>(row_out<T>(a.grad_in, p, first + r) + p.channel, dx);
             }
         }
     }
+    if (p.tile == 0 && wave == 0 && a.grad_initial && p.active) store_chan(a.grad_initial + state_at, e);
 }
 
 // One token for each of some sequences: h = a h + b on the states of a pool, at
@@ -494,14 +510,14 @@ int gate_dispatch(lcpp_gate g, F f)
 
 // Channels of a lane: two, so that a wave's row is 256 or 512 bytes; one where
 // 64 lanes cover the channels.
-uint32_t rec_lane_channels(uint64_t channels) { return channels <= kWave ? 1 : 2; }
+uint32_t rec_lane_channels(uint64_t channels, size_t size) { return channels <= kWave || size == 4 ? 1 : 2; }
 struct RecShape {
     uint64_t tiles, groups, words;
 };
-bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, RecShape *r)
+bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t size, RecShape *r)
 {
     if (sequences > 0xFFFFFFFFull || max_length > 0x7FFFFFFFull || channels > kMaxCols) return false;
-    const uint64_t lanes = kWave * rec_lane_channels(channels);
+    const uint64_t lanes = kWave * rec_lane_channels(channels, size);
     r->groups = ceil_div(channels, lanes);
     r->tiles = std::max<uint64_t>(ceil_div(max_length, kTileRows), 1);
     // workgroups are numbered in 32 bits, and a launch has less than 2^32 threads
@@ -540,7 +556,7 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
     if (!e) return LCPP_ERR_UNSUPPORTED_DTYPE;
     if (g != LCPP_GATE_DECAY && g != LCPP_GATE_LOG && g != LCPP_GATE_SIGMOID) return LCPP_ERR_INVALID_ARG;
     RecShape r;
-    if (!rec_shape(sequences, max_length, channels, &r) || (!a.begin) != (!a.end)) return LCPP_ERR_INVALID_ARG;
+    if (!rec_shape(sequences, max_length, channels, e, &r) || (!a.begin) != (!a.end)) return LCPP_ERR_INVALID_ARG;
     if (sequences == 0 || channels == 0) return LCPP_OK;
     if (a.begin && (!elem_ok(a.begin, 4) || !elem_ok(a.end, 4))) return LCPP_ERR_INVALID_ARG;
     auto optional = [](const void *p) { return !p || elem_ok(p, 4); };
@@ -576,9 +592,12 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
     }
     return float_dispatch(t, [&](auto x) -> int {
         using T = decltype(x);
-        return gate_dispatch(g, [&](auto gate) {
+        return gate_dispatch(g, [&](auto gate) -> int {
             using G = decltype(gate);
-            return rec_lane_channels(channels) == 1 ? rec_launch<T, G, 1>(forward, a, s) : rec_launch<T, G, 2>(forward, a, s);
+            if constexpr (sizeof(T) == 2) {
+                if (rec_lane_channels(channels, sizeof(T)) == 2) return rec_launch<T, G, 2>(forward, a, s);
+            }
+            return rec_launch<T, G, 1>(forward, a, s);
         });
     });
 }
@@ -591,8 +610,10 @@ using namespace lcpp;
 extern "C" int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes)
 {
     RecShape r;
-    if (!bytes || !rec_shape(sequences, max_length, channels, &r)) return LCPP_ERR_INVALID_ARG;
+    if (!bytes || !rec_shape(sequences, max_length, channels, 2, &r)) return LCPP_ERR_INVALID_ARG;
     *bytes = rec_temp_bytes(r);
+    if (!rec_shape(sequences, max_length, channels, 4, &r)) return LCPP_ERR_INVALID_ARG;
+    *bytes = std::max<size_t>(*bytes, rec_temp_bytes(r));  // for every type
     return LCPP_OK;
 }
 

@@ -42,6 +42,14 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T *p)
     r.v = *reinterpret_cast<const typename Pack<T, N>::vec_u *>(p);
     return r;
 }
+// The same for data that is read once (streaming policy).
+template <int N, class T>
+__device__ __forceinline__ Pack<T, N> load_pack_nt(const T *p)
+{
+    Pack<T, N> r;
+    r.v = __builtin_nontemporal_load(reinterpret_cast<const typename Pack<T, N>::vec_u *>(p));
+    return r;
+}
 // The first `valid` of N elements, 0 in the others' place.
 template <int N, class T>
 __device__ __forceinline__ Pack<T, N> load_pack_part(const T *p, int valid)
