@@ -53,7 +53,9 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(DropoutArgs a)
 #pragma unroll
             for (int i = 0; i < kOctet; ++i) x[i] += r[i];
         }
-        store_octet(static_cast<T *>(a.out) + row * a.out_stride, col, a.cols, x);
+        T *out = static_cast<T *>(a.out) + row * a.out_stride;
+        if (col + kOctet <= a.cols) store_pack_nt<kOctet>(out + col, x);
+        else store_octet(out, col, a.cols, x);
         row += a.step_rows;
         octet += a.step_octets;
         if (octet >= a.row_octets) {

@@ -16,10 +16,58 @@
 namespace lcpp {
 namespace {
 
-// Sums of one or two values over the NT threads of a row's group; every thread
-// of the group gets them.  A group of several waves meets in LDS, and all groups
-// of the workgroup meet at the same barrier; `slot` alternates between the calls
-// of one row, so that one barrier a call is enough.
+// A barrier for what waves exchange in LDS.  __syncthreads() would also wait for
+// the global loads in flight, which here are those of the next rows.
+__device__ __forceinline__ void group_barrier()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A row's columns: eight at a time (an octet) in the lanes of its group of
+// threads, K octets a thread, and the last `rem` < 8 columns one to a thread, so
+// that no octet is partly valid.
+template <int NT, int K>
+struct Columns {
+    uint32_t t, full, rem, cols;
+    __device__ __forceinline__ Columns(uint32_t n) : t(threadIdx.x % NT), full(n & ~7u), rem(n & 7u), cols(n) {}
+    __device__ __forceinline__ uint32_t col(int k) const { return (t + k * NT) * kOctet; }
+    __device__ __forceinline__ bool has(int k) const { return col(k) < full; }
+    __device__ __forceinline__ bool has_tail() const { return t < rem; }
+    __device__ __forceinline__ uint32_t tail() const { return full + t; }
+};
+
+// A thread's part of a row as it lies in memory.
+template <class T, int K>
+struct RowPart {
+    Octet<T> o[K];
+    T tail;
+    template <int NT>
+    __device__ __forceinline__ void load(const T *row, const Columns<NT, K> &c)
+    {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (c.has(k)) o[k] = load_pack<kOctet>(row + c.col(k));
+        if (c.has_tail()) tail = row[c.tail()];
+    }
+    // a vector of weights, or one value everywhere
+    template <int NT>
+    __device__ __forceinline__ void load_or(const T *p, const Columns<NT, K> &c, float value)
+    {
+        tail = (T)value;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) o[k].v[i] = (T)value;
+        if (p) load(p, c);
+    }
+};
+
+// Sums of V values over the NT threads of a row's group; every thread of the
+// group gets them.  A group of several waves meets in LDS, all groups of the
+// workgroup at the same barrier; `slot` alternates from row to row, so one
+// barrier a row is enough.
 template <int NT, int WAVES, int V>
 __device__ __forceinline__ void group_sum(float (&x)[V], float (*lds)[WAVES][2], int slot)
 {
@@ -32,7 +80,7 @@ __device__ __forceinline__ void group_sum(float (&x)[V], float (*lds)[WAVES][2],
 #pragma unroll
             for (int v = 0; v < V; ++v) lds[slot][wave][v] = x[v];
         }
-        __syncthreads();
+        group_barrier();
         const uint32_t first = wave / GW * GW;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -42,6 +90,49 @@ __device__ __forceinline__ void group_sum(float (&x)[V], float (*lds)[WAVES][2],
             x[v] = s;
         }
     }
+}
+
+// Mean and mean square deviation of a row.  A wave takes its columns' mean and
+// the squares around it; the waves' pairs meet in LDS at one barrier and combine:
+// the squares around the common mean are those around the wave's own plus n
+// times the square of the means' distance.  So a row far from 0 loses nothing.
+// `count`: columns of the wave; the lambda gives f(x, valid) for each of them.
+template <int NT, int WAVES, class F>
+__device__ __forceinline__ void group_moments(F each, float count, float (*lds)[WAVES][2], const float *counts, int slot,
+                                              float cols, float &mean, float &var)
+{
+    float sum = 0.0f;
+    each([&](float x) { sum += x; });
+    const float inv = count > 0.0f ? 1.0f / count : 0.0f;
+    mean = wave_reduce_dpp(sum, SumOp()) * inv;
+    float sq = 0.0f;
+    each([&](float x) {
+        const float d = x - mean;
+        sq += d * d;
+    });
+    sq = wave_reduce_dpp(sq, SumOp());
+    if constexpr (NT > kWave) {
+        constexpr int GW = NT / kWave;
+        const uint32_t wave = threadIdx.x / kWave, first = wave / GW * GW;
+        if (lane_id() == 0) lds[slot][wave][0] = mean, lds[slot][wave][1] = sq;
+        group_barrier();
+        float m[GW], n[GW], total = 0.0f;
+        sq = 0.0f;
+#pragma unroll
+        for (int w = 0; w < GW; ++w) {
+            m[w] = lds[slot][first + w][0];
+            n[w] = counts[w];
+            sq += lds[slot][first + w][1];
+            total += n[w] * m[w];
+        }
+        mean = total / cols;
+#pragma unroll
+        for (int w = 0; w < GW; ++w) {
+            const float d = m[w] - mean;
+            sq += n[w] * (d * d);
+        }
+    }
+    var = sq / cols;
 }
 
 struct NormArgs {
@@ -54,10 +145,137 @@ struct NormArgs {
     DropArgs drop;
 };
 
+// One element's dropout, for the last columns of a row.
+__device__ __forceinline__ float drop_one(float x, uint32_t row, uint32_t col, uint64_t offset, const DropArgs &d)
+{
+    float v[kOctet] = {x, x, x, x, x, x, x, x};
+    drop_octet(v, row, col / kOctet, offset, d);
+    float r = v[0];
+#pragma unroll
+    for (int i = 1; i < kOctet; ++i) r = (int)(col % kOctet) == i ? v[i] : r;
+    return r;
+}
+
+// Rows that the registers of NT threads hold, K octets each; THREADS / NT rows at
+// a time, each workgroup several one after the other, the next ones on their way
+// while these are worked on, and the weights in registers too (AHEAD: where the
+// registers hold that).
+template <class T, class W, int NT, int K, int THREADS, bool ADD, bool AHEAD>
+__global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
+{
+    constexpr int WAVES = THREADS / kWave, RG = THREADS / NT, GW = NT / kWave;
+    __shared__ float lds[2][WAVES][2];
+    const Columns<NT, K> c(a.cols);
+    const uint32_t group = threadIdx.x / NT;
+    const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
+    // columns of each wave of a group (the same for every group)
+    float counts[GW];
+#pragma unroll
+    for (int w = 0; w < GW; ++w) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const uint32_t from = (w * kWave + k * NT) * kOctet;
+            n += from < c.full ? (c.full - from < kWave * kOctet ? c.full - from : kWave * kOctet) : 0;
+        }
+        counts[w] = (float)(n + (w == 0 ? c.rem : 0));
+    }
+    const uint32_t wave = threadIdx.x / kWave;
+    float count = counts[0];
+#pragma unroll
+    for (int w = 1; w < GW; ++w) count = wave % GW == (uint32_t)w ? counts[w] : count;
+
+    RowPart<W, K> w, b;
+    if constexpr (AHEAD) {
+        w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
+        b.load_or(static_cast<const W *>(a.bias), c, 0.0f);
+    }
+    const T *in = static_cast<const T *>(a.in), *residual = static_cast<const T *>(a.residual);
+    RowPart<T, K> next, next_r;
+    auto load = [&](uint64_t row) {
+        if (row >= a.rows) return;
+        next.load(in + row * a.in_stride, c);
+        if constexpr (ADD) next_r.load(residual + row * a.residual_stride, c);
+    };
+    uint64_t row = (uint64_t)blockIdx.x * RG + group;
+    if constexpr (AHEAD) load(row);
+    // (the workgroup's groups make the same number of rounds: they share barriers)
+    const uint64_t stride = (uint64_t)gridDim.x * RG;
+    int slot = 0;
+    for (uint64_t base = (uint64_t)blockIdx.x * RG; base < a.rows; base += stride, row += stride, slot ^= 1) {
+        if constexpr (!AHEAD) load(row);
+        RowPart<T, K> x = next, r = next_r;
+        const bool live = row < a.rows;
+        if constexpr (AHEAD) load(row + stride);
+        if constexpr (ADD) {
+            // s in the place of x, rounded as it is stored
+            if (live) {
+                T *sum = static_cast<T *>(a.sum) + row * a.sum_stride;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (!c.has(k)) continue;
+                    float v[kOctet];
+#pragma unroll
+                    for (int i = 0; i < kOctet; ++i) v[i] = x.o[k][i];
+                    if (a.drop.cut) drop_octet(v, (uint32_t)row, c.col(k) / kOctet, offset, a.drop);
+#pragma unroll
+                    for (int i = 0; i < kOctet; ++i) {
+                        v[i] += r.o[k][i];
+                        x.o[k].v[i] = (T)v[i];
+                    }
+                    store_pack<kOctet>(sum + c.col(k), v);
+                }
+                if (c.has_tail()) {
+                    float v = (float)x.tail;
+                    if (a.drop.cut) v = drop_one(v, (uint32_t)row, c.tail(), offset, a.drop);
+                    x.tail = (T)(v + (float)r.tail);
+                    sum[c.tail()] = x.tail;
+                }
+            }
+        }
+        float mean, var;
+        group_moments<NT, WAVES>(
+            [&](auto f) {
+                if (!live) return;
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (c.has(k))
+#pragma unroll
+                        for (int i = 0; i < kOctet; ++i) f(x.o[k][i]);
+                if (c.has_tail()) f((float)x.tail);
+            },
+            count, lds, counts, slot, (float)a.cols, mean, var);
+        const float rstd = 1.0f / sqrtf(var + a.eps);
+        if (!live) continue;
+        if constexpr (!AHEAD) {
+            w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
+            b.load_or(static_cast<const W *>(a.bias), c, 0.0f);
+        }
+        T *out = static_cast<T *>(a.out) + row * a.out_stride;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (!c.has(k)) continue;
+            float y[kOctet];
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) y[i] = (x.o[k][i] - mean) * rstd * w.o[k][i] + b.o[k][i];
+            store_pack_nt<kOctet>(out + c.col(k), y);
+        }
+        if (c.has_tail()) out[c.tail()] = (T)(((float)x.tail - mean) * rstd * (float)w.tail + (float)b.tail);
+        if (c.t == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+    }
+}
+
+// ---- longer rows
+constexpr int kLongThreads = 1024;
+constexpr int kLongWaves = kLongThreads / kWave;
+
 // s of one octet: the input, or residual + dropout(input) rounded to the rows'
 // type, which is also stored.
 template <class T, bool ADD>
-__device__ __forceinline__ Octet<T> norm_input(const NormArgs &a, uint64_t offset, uint32_t row, uint32_t col)
+__device__ __forceinline__ Octet<T> norm_input(const NormArgs &a, uint64_t offset, uint64_t row, uint32_t col)
 {
     Octet<T> x = load_octet(static_cast<const T *>(a.in) + row * a.in_stride, col, a.cols);
     if constexpr (ADD) {
@@ -65,7 +283,7 @@ __device__ __forceinline__ Octet<T> norm_input(const NormArgs &a, uint64_t offse
         float v[kOctet];
 #pragma unroll
         for (int i = 0; i < kOctet; ++i) v[i] = x[i];
-        if (a.drop.cut) drop_octet(v, row, col / kOctet, offset, a.drop);
+        if (a.drop.cut) drop_octet(v, (uint32_t)row, col / kOctet, offset, a.drop);
 #pragma unroll
         for (int i = 0; i < kOctet; ++i) {
             v[i] += r[i];
@@ -75,88 +293,24 @@ __device__ __forceinline__ Octet<T> norm_input(const NormArgs &a, uint64_t offse
     }
     return x;
 }
-
-template <class T, class W>
-__device__ __forceinline__ void norm_output(const NormArgs &a, uint32_t row, uint32_t col, const Octet<T> &x, float mean,
-                                            float rstd)
+template <class W>
+__device__ __forceinline__ void norm_weight(const void *weight, uint32_t col, uint32_t cols, float value, float (&w)[kOctet])
 {
-    float y[kOctet];
+    if (weight) {
+        const Octet<W> o = load_octet(static_cast<const W *>(weight), col, cols);
 #pragma unroll
-    for (int i = 0; i < kOctet; ++i) y[i] = (x[i] - mean) * rstd;
-    if (a.weight) {
-        const Octet<W> w = load_octet(static_cast<const W *>(a.weight), col, a.cols);
+        for (int i = 0; i < kOctet; ++i) w[i] = o[i];
+    } else {
 #pragma unroll
-        for (int i = 0; i < kOctet; ++i) y[i] *= w[i];
-    }
-    if (a.bias) {
-        const Octet<W> b = load_octet(static_cast<const W *>(a.bias), col, a.cols);
-#pragma unroll
-        for (int i = 0; i < kOctet; ++i) y[i] += b[i];
-    }
-    store_octet(static_cast<T *>(a.out) + row * a.out_stride, col, a.cols, y);
-}
-
-// Rows whose octets fit the registers of NT threads, K each: read once, the mean
-// first and then the squares around it, so a row far from 0 loses nothing.
-template <class T, class W, int NT, int K, int THREADS, bool ADD>
-__global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
-{
-    constexpr int WAVES = THREADS / kWave;
-    __shared__ float lds[2][WAVES][2];
-    constexpr int RG = THREADS / NT;
-    const uint32_t t = threadIdx.x % NT;
-    const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
-    // (the workgroup's groups make the same number of rounds: they share barriers)
-    for (uint64_t base = (uint64_t)blockIdx.x * RG; base < a.rows; base += (uint64_t)gridDim.x * RG) {
-        const uint64_t row64 = base + threadIdx.x / NT;
-        const bool live = row64 < a.rows;
-        const uint32_t row = (uint32_t)row64;
-        Octet<T> x[K];
-        float sum[1] = {0.0f};
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const uint32_t col = (t + k * NT) * kOctet;
-            if (live && col < a.cols) {
-                x[k] = norm_input<T, ADD>(a, offset, row, col);
-#pragma unroll
-                for (int i = 0; i < kOctet; ++i) sum[0] += x[k][i];
-            }
-        }
-        group_sum<NT, WAVES>(sum, lds, 0);
-        const float mean = sum[0] / (float)a.cols;
-        float sq[1] = {0.0f};
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const uint32_t col = (t + k * NT) * kOctet;
-            if (live && col < a.cols) {
-#pragma unroll
-                for (int i = 0; i < kOctet; ++i) {
-                    const float d = x[k][i] - mean;
-                    if (col + i < a.cols) sq[0] += d * d;
-                }
-            }
-        }
-        group_sum<NT, WAVES>(sq, lds, 1);
-        const float rstd = 1.0f / sqrtf(sq[0] / (float)a.cols + a.eps);
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const uint32_t col = (t + k * NT) * kOctet;
-            if (live && col < a.cols) norm_output<T, W>(a, row, col, x[k], mean, rstd);
-        }
-        if (live && t == 0) {
-            if (a.mean) a.mean[row] = mean;
-            if (a.rstd) a.rstd[row] = rstd;
-        }
+        for (int i = 0; i < kOctet; ++i) w[i] = value;
     }
 }
 
-// Longer rows: a workgroup reads its row three times (from the caches).
-constexpr int kLongThreads = 1024;
+// A workgroup reads its row three times (from the caches).
 template <class T, class W, bool ADD>
 __global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(NormArgs a)
 {
-    constexpr int WAVES = kLongThreads / kWave;
-    __shared__ float lds[2][WAVES][2];
+    __shared__ float lds[2][kLongWaves][2];
     const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *s = ADD ? static_cast<const T *>(a.sum) + row * a.sum_stride
@@ -167,7 +321,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(NormArg
 #pragma unroll
             for (int i = 0; i < kOctet; ++i) sum[0] += x[i];
         }
-        group_sum<kLongThreads, WAVES>(sum, lds, 0);
+        group_sum<kLongThreads, kLongWaves>(sum, lds, 0);
         const float mean = sum[0] / (float)a.cols;
         float sq[1] = {0.0f};
         // (each thread reads back the sums that it stored itself)
@@ -179,10 +333,17 @@ __global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(NormArg
                 if (col + i < a.cols) sq[0] += d * d;
             }
         }
-        group_sum<kLongThreads, WAVES>(sq, lds, 1);
+        group_sum<kLongThreads, kLongWaves>(sq, lds, 1);
         const float rstd = 1.0f / sqrtf(sq[0] / (float)a.cols + a.eps);
-        for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet)
-            norm_output<T, W>(a, row, col, load_octet(s, col, a.cols), mean, rstd);
+        for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
+            const Octet<T> x = load_octet(s, col, a.cols);
+            float w[kOctet], b[kOctet];
+            norm_weight<W>(a.weight, col, a.cols, 1.0f, w);
+            norm_weight<W>(a.bias, col, a.cols, 0.0f, b);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) w[i] = (x[i] - mean) * rstd * w[i] + b[i];
+            store_octet(static_cast<T *>(a.out) + row * a.out_stride, col, a.cols, w);
+        }
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[row] = mean;
             if (a.rstd) a.rstd[row] = rstd;
@@ -202,112 +363,116 @@ struct NormGradArgs {
     DropArgs drop;
 };
 
-// One octet's dy w (v), u, and its shares of dw and db.
-template <class T, class W>
-__device__ __forceinline__ void norm_grad_terms(const Octet<T> &dy, const Octet<T> &s, const float (&w)[kOctet],
-                                                float mean, float rstd, float (&v)[kOctet], float (&u)[kOctet])
-{
-#pragma unroll
-    for (int i = 0; i < kOctet; ++i) {
-        u[i] = (s[i] - mean) * rstd;
-        v[i] = dy[i] * w[i];
-    }
-}
-template <class W>
-__device__ __forceinline__ void norm_weight(const void *weight, uint32_t col, uint32_t cols, float (&w)[kOctet])
-{
-    if (weight) {
-        const Octet<W> o = load_octet(static_cast<const W *>(weight), col, cols);
-#pragma unroll
-        for (int i = 0; i < kOctet; ++i) w[i] = o[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < kOctet; ++i) w[i] = 1.0f;
-    }
-}
-// ds of an octet from the row's sums, and what is stored of it.
-template <class T, bool ADD>
-__device__ __forceinline__ void norm_grad_output(const NormGradArgs &a, uint64_t offset, uint32_t row, uint32_t col,
-                                                 const float (&v)[kOctet], const float (&u)[kOctet], float mean_v,
-                                                 float mean_vu, float rstd)
-{
-    float d[kOctet];
-#pragma unroll
-    for (int i = 0; i < kOctet; ++i) d[i] = rstd * (v[i] - mean_v - u[i] * mean_vu);
-    if constexpr (ADD) {
-        if (a.grad_sum) {
-            const Octet<T> g = load_octet(static_cast<const T *>(a.grad_sum) + row * a.gs_stride, col, a.cols);
-#pragma unroll
-            for (int i = 0; i < kOctet; ++i) d[i] += g[i];
-        }
-    }
-    if (a.grad_in) store_octet(static_cast<T *>(a.grad_in) + row * a.gi_stride, col, a.cols, d);
-    if constexpr (ADD) {
-        if (a.grad_branch) {
-            if (a.drop.cut) drop_octet(d, row, col / kOctet, offset, a.drop);
-            store_octet(static_cast<T *>(a.grad_branch) + row * a.gb_stride, col, a.cols, d);
-        }
-    }
-}
-
 // THREADS / NT rows at a time; a thread keeps the same columns for all of its
 // workgroup's rows, so dw and db are sums in its registers, one partial sum per
-// workgroup at the end.
-template <class T, class W, int NT, int K, int THREADS, bool ADD>
+// workgroup at the end.  The next rows are on their way while these are worked on.
+template <class T, class W, int NT, int K, int THREADS, bool ADD, bool AHEAD>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
 {
     constexpr int WAVES = THREADS / kWave, RG = THREADS / NT;
     __shared__ float lds[2][WAVES][2];
-    __shared__ float fold[RG > 1 ? NT * K * kOctet : 1];
-    const uint32_t t = threadIdx.x % NT, group = threadIdx.x / NT;
+    __shared__ float fold[RG > 1 ? NT * K * kOctet : 1], fold_tail[RG > 1 ? kOctet : 1];
+    const Columns<NT, K> c(a.cols);
+    const uint32_t group = threadIdx.x / NT;
     const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
     const float inv = 1.0f / (float)a.cols;
-    float dw[K][kOctet] = {}, db[K][kOctet] = {};
-    int slot = 0;
+    float dw[K][kOctet] = {}, db[K][kOctet] = {}, dw_tail = 0.0f, db_tail = 0.0f;
     if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
-    // (the workgroup's groups make the same number of rounds: they share barriers)
-    for (uint64_t base = (uint64_t)blockIdx.x * RG; base < a.rows; base += (uint64_t)gridDim.x * RG, slot ^= 1) {
-        const uint64_t row64 = base + group;
-        const bool live = row64 < a.rows;
-        const uint32_t row = live ? (uint32_t)row64 : a.rows - 1;
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        Octet<T> dy[K], s[K];
-        float sums[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const uint32_t col = (t + k * NT) * kOctet;
-            if (live && col < a.cols) {
-                dy[k] = load_octet(static_cast<const T *>(a.grad_out) + row * a.go_stride, col, a.cols);
-                s[k] = load_octet(static_cast<const T *>(a.in) + row * a.in_stride, col, a.cols);
-            }
+    RowPart<W, K> w;
+    if constexpr (AHEAD) w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
+    const T *grad_out = static_cast<const T *>(a.grad_out), *in = static_cast<const T *>(a.in);
+    const T *grad_sum = static_cast<const T *>(a.grad_sum);
+    RowPart<T, K> next_dy, next_s, next_g;
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    auto load = [&](uint64_t row) {
+        if (row >= a.rows) return;
+        next_dy.load(grad_out + row * a.go_stride, c);
+        next_s.load(in + row * a.in_stride, c);
+        if constexpr (ADD && AHEAD) {
+            if (grad_sum) next_g.load(grad_sum + row * a.gs_stride, c);
         }
+        next_mean = a.mean[row];
+        next_rstd = a.rstd[row];
+    };
+    uint64_t row = (uint64_t)blockIdx.x * RG + group;
+    if constexpr (AHEAD) load(row);
+    // (the workgroup's groups make the same number of rounds: they share barriers)
+    const uint64_t stride = (uint64_t)gridDim.x * RG;
+    int slot = 0;
+    for (uint64_t base = (uint64_t)blockIdx.x * RG; base < a.rows; base += stride, row += stride, slot ^= 1) {
+        if constexpr (!AHEAD) load(row);
+        RowPart<T, K> dy = next_dy, s = next_s, g = next_g;
+        const float mean = next_mean, rstd = next_rstd;
+        const bool live = row < a.rows;
+        if constexpr (AHEAD) load(row + stride);
+        else w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
+        float sums[2] = {0.0f, 0.0f};
+        if (live) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const uint32_t col = (t + k * NT) * kOctet;
-            if (live && col < a.cols) {
-                float w[kOctet], v[kOctet], u[kOctet];
-                norm_weight<W>(a.weight, col, a.cols, w);
-                norm_grad_terms<T, W>(dy[k], s[k], w, mean, rstd, v, u);
+            for (int k = 0; k < K; ++k) {
+                if (!c.has(k)) continue;
 #pragma unroll
                 for (int i = 0; i < kOctet; ++i) {
-                    // (past the row's end dy and v are 0, u is not)
-                    sums[0] += v[i];
-                    sums[1] += v[i] * u[i];
-                    dw[k][i] += dy[k][i] * u[i];
-                    db[k][i] += dy[k][i];
+                    const float u = (s.o[k][i] - mean) * rstd, v = dy.o[k][i] * w.o[k][i];
+                    sums[0] += v;
+                    sums[1] += v * u;
+                    dw[k][i] += dy.o[k][i] * u;
+                    db[k][i] += dy.o[k][i];
                 }
+            }
+            if (c.has_tail()) {
+                const float u = ((float)s.tail - mean) * rstd, v = (float)dy.tail * (float)w.tail;
+                sums[0] += v;
+                sums[1] += v * u;
+                dw_tail += (float)dy.tail * u;
+                db_tail += (float)dy.tail;
             }
         }
         group_sum<NT, WAVES>(sums, lds, slot);
+        if (!live) continue;
+        if constexpr (!AHEAD) {
+            w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
+            if constexpr (ADD) {
+                if (grad_sum) g.load(grad_sum + row * a.gs_stride, c);
+            }
+        }
         const float mean_v = sums[0] * inv, mean_vu = sums[1] * inv;
+        T *gi = static_cast<T *>(a.grad_in) + row * a.gi_stride, *gb = static_cast<T *>(a.grad_branch) + row * a.gb_stride;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const uint32_t col = (t + k * NT) * kOctet;
-            if (live && col < a.cols) {
-                float w[kOctet], v[kOctet], u[kOctet];
-                norm_weight<W>(a.weight, col, a.cols, w);
-                norm_grad_terms<T, W>(dy[k], s[k], w, mean, rstd, v, u);
-                norm_grad_output<T, ADD>(a, offset, row, col, v, u, mean_v, mean_vu, rstd);
+            if (!c.has(k)) continue;
+            float d[kOctet];
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) {
+                const float u = (s.o[k][i] - mean) * rstd, v = dy.o[k][i] * w.o[k][i];
+                d[i] = rstd * (v - mean_v - u * mean_vu);
+            }
+            if constexpr (ADD) {
+                if (grad_sum) {
+#pragma unroll
+                    for (int i = 0; i < kOctet; ++i) d[i] += g.o[k][i];
+                }
+            }
+            if (a.grad_in) store_pack_nt<kOctet>(gi + c.col(k), d);
+            if constexpr (ADD) {
+                if (a.grad_branch) {
+                    if (a.drop.cut) drop_octet(d, (uint32_t)row, c.col(k) / kOctet, offset, a.drop);
+                    store_pack_nt<kOctet>(gb + c.col(k), d);
+                }
+            }
+        }
+        if (c.has_tail()) {
+            const float u = ((float)s.tail - mean) * rstd, v = (float)dy.tail * (float)w.tail;
+            float d = rstd * (v - mean_v - u * mean_vu);
+            if constexpr (ADD) {
+                if (grad_sum) d += (float)g.tail;
+            }
+            if (a.grad_in) gi[c.tail()] = (T)d;
+            if constexpr (ADD) {
+                if (a.grad_branch) {
+                    if (a.drop.cut) d = drop_one(d, (uint32_t)row, c.tail(), offset, a.drop);
+                    gb[c.tail()] = (T)d;
+                }
             }
         }
     }
@@ -316,6 +481,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
 #pragma unroll
     for (int half = 0; half < 2; ++half, part += a.cols) {
         float(&x)[K][kOctet] = half ? db : dw;
+        float &tail = half ? db_tail : dw_tail;
         if constexpr (RG > 1) {
             // the groups add to the columns' sums one after the other, in a fixed order
             for (uint32_t g = 0; g < RG; ++g) {
@@ -324,20 +490,24 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
                     for (int k = 0; k < K; ++k)
 #pragma unroll
                         for (int i = 0; i < kOctet; ++i) {
-                            float &f = fold[(i * K + k) * NT + t];
+                            float &f = fold[(i * K + k) * NT + c.t];
                             f = g ? f + x[k][i] : x[k][i];
                             x[k][i] = f;
                         }
+                    if (c.has_tail()) {
+                        float &f = fold_tail[c.t];
+                        f = g ? f + tail : tail;
+                        tail = f;
+                    }
                 }
                 __syncthreads();
             }
         }
         if (group == RG - 1) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const uint32_t col = (t + k * NT) * kOctet;
-                if (col < a.cols) store_octet(part, col, a.cols, x[k]);
-            }
+            for (int k = 0; k < K; ++k)
+                if (c.has(k)) store_pack<kOctet>(part + c.col(k), x[k]);
+            if (c.has_tail()) part[c.tail()] = tail;
         }
     }
 }
@@ -346,8 +516,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
 template <class T, class W, bool ADD>
 __global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(NormGradArgs a)
 {
-    constexpr int WAVES = kLongThreads / kWave;
-    __shared__ float lds[2][WAVES][2];
+    __shared__ float lds[2][kLongWaves][2];
     const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
     const float inv = 1.0f / (float)a.cols;
     if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
@@ -357,21 +526,46 @@ __global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(NormGr
         const T *dy = static_cast<const T *>(a.grad_out) + row * a.go_stride;
         const T *s = static_cast<const T *>(a.in) + row * a.in_stride;
         float sums[2] = {0.0f, 0.0f};
-        float w[kOctet], v[kOctet], u[kOctet];
+        // v and u of an octet (past the row's end dy and so v are 0)
+        auto terms = [&](uint32_t col, float(&v)[kOctet], float(&u)[kOctet]) {
+            const Octet<T> d = load_octet(dy, col, a.cols), x = load_octet(s, col, a.cols);
+            float w[kOctet];
+            norm_weight<W>(a.weight, col, a.cols, 1.0f, w);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) {
+                u[i] = (x[i] - mean) * rstd;
+                v[i] = d[i] * w[i];
+            }
+        };
         for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
-            norm_weight<W>(a.weight, col, a.cols, w);
-            norm_grad_terms<T, W>(load_octet(dy, col, a.cols), load_octet(s, col, a.cols), w, mean, rstd, v, u);
+            float v[kOctet], u[kOctet];
+            terms(col, v, u);
 #pragma unroll
             for (int i = 0; i < kOctet; ++i) {
                 sums[0] += v[i];
                 sums[1] += v[i] * u[i];
             }
         }
-        group_sum<kLongThreads, WAVES>(sums, lds, slot);
+        group_sum<kLongThreads, kLongWaves>(sums, lds, slot);
         for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
-            norm_weight<W>(a.weight, col, a.cols, w);
-            norm_grad_terms<T, W>(load_octet(dy, col, a.cols), load_octet(s, col, a.cols), w, mean, rstd, v, u);
-            norm_grad_output<T, ADD>(a, offset, row, col, v, u, sums[0] * inv, sums[1] * inv, rstd);
+            float v[kOctet], u[kOctet], d[kOctet];
+            terms(col, v, u);
+#pragma unroll
+            for (int i = 0; i < kOctet; ++i) d[i] = rstd * (v[i] - sums[0] * inv - u[i] * (sums[1] * inv));
+            if constexpr (ADD) {
+                if (a.grad_sum) {
+                    const Octet<T> g = load_octet(static_cast<const T *>(a.grad_sum) + row * a.gs_stride, col, a.cols);
+#pragma unroll
+                    for (int i = 0; i < kOctet; ++i) d[i] += g[i];
+                }
+            }
+            if (a.grad_in) store_octet(static_cast<T *>(a.grad_in) + row * a.gi_stride, col, a.cols, d);
+            if constexpr (ADD) {
+                if (a.grad_branch) {
+                    if (a.drop.cut) drop_octet(d, (uint32_t)row, col / kOctet, offset, a.drop);
+                    store_octet(static_cast<T *>(a.grad_branch) + row * a.gb_stride, col, a.cols, d);
+                }
+            }
         }
     }
 }
@@ -414,7 +608,7 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void norm_fold_kernel(const floa
     float sum = 0.0f;
     if (col < cols) {
         const float *p = partial + (uint64_t)blockIdx.y * cols + col;
-#pragma unroll 4
+#pragma unroll 16
         for (uint32_t i = wave; i < parts; i += kFoldWaves) sum += p[(uint64_t)i * 2 * cols];
     }
     lds[wave][lane] = sum;
@@ -429,33 +623,36 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void norm_fold_kernel(const floa
 // ---------------------------------------------------------------- launches
 // (a launch has less than 2^32 threads: with more rows, workgroups take several)
 constexpr uint64_t kMaxGroups = 1u << 20;
+// Threads of a workgroup whose rows take nt each: as many rows as fit `atleast`.
+constexpr int norm_threads(int nt, int atleast) { return nt >= atleast ? nt : atleast / nt * nt; }
+// Workgroups that the device holds at once, which all get the same number of rows
+// (with one too many per CU the last ones run alone: 16384 x 4096 bfloat16 with
+// four workgroups per CU where three are resident 64 us, with three ...).
+template <class Kernel>
+uint64_t resident_groups(DeviceCache &cache, Kernel kernel, int threads)
+{
+    return (uint64_t)device_cus() * device_cached(cache, [&] {
+               int n = 0;
+               const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0);
+               return e == hipSuccess && n > 0 ? n : 1;
+           });
+}
 
 // NT threads with K octets each for a row of `octets`: the smallest group of
 // waves that holds it.  f(NT, K) as integral constants; false if the row is longer.
 template <class F>
-bool norm_forward_shape(uint32_t octets, F f)
+bool norm_shape(uint32_t octets, F f)
 {
     using std::integral_constant;
     if (octets <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (octets <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    else if (octets <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    else if (octets <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    else if (octets <= 1024) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-    else if (octets <= 2048) f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
-    else if (octets <= 4096) f(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
-    else return false;
-    return true;
-}
-template <class F>
-bool norm_backward_shape(uint32_t octets, F f)
-{
-    using std::integral_constant;
-    if (octets <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (octets <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    else if (octets <= 256) f(integral_constant<int, 128>{}, integral_constant<int, 2>{});
-    else if (octets <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    else if (octets <= 1024) f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
-    else if (octets <= 2048) f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    else if (octets <= 192) f(integral_constant<int, 192>{}, integral_constant<int, 1>{});
+    else if (octets <= 256) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    else if (octets <= 384) f(integral_constant<int, 384>{}, integral_constant<int, 1>{});
+    else if (octets <= 512) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+    else if (octets <= 768) f(integral_constant<int, 768>{}, integral_constant<int, 1>{});
+    else if (octets <= 1024) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+    else if (octets <= 2048) f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
     else return false;
     return true;
 }
@@ -463,15 +660,20 @@ bool norm_backward_shape(uint32_t octets, F f)
 template <class T, class W, bool ADD>
 int norm_forward_launch(const NormArgs &a, hipStream_t s)
 {
-    const uint32_t octets = (uint32_t)ceil_div(a.cols, kOctet);
+    const uint32_t octets = a.cols / kOctet;
     const char *name = ADD ? "layer_norm_add_forward" : "layer_norm_forward";
-    const bool fits = norm_forward_shape(octets, [&](auto nt, auto k) {
+    const bool fits = norm_shape(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
-        constexpr int THREADS = NT > 256 ? NT : 256;
-        const uint32_t grid = (uint32_t)std::min<uint64_t>(ceil_div(a.rows, THREADS / NT), kMaxGroups);
-        LCPP_LAUNCH(name, s, norm_forward_kernel<T, W, NT, K, THREADS, ADD><<<grid, THREADS, 0, s>>>(a));
+        constexpr int THREADS = norm_threads(NT, 256);
+        static DeviceCache cache;
+        const uint64_t most = resident_groups(cache, norm_forward_kernel<T, W, NT, K, THREADS, ADD, K <= 2>, THREADS);
+        const uint32_t grid = (uint32_t)std::min<uint64_t>(ceil_div(a.rows, THREADS / NT), most);
+        LCPP_LAUNCH(name, s, norm_forward_kernel<T, W, NT, K, THREADS, ADD, K <= 2><<<grid, THREADS, 0, s>>>(a));
     });
-    if (!fits) LCPP_LAUNCH(name, s, norm_forward_long_kernel<T, W, ADD><<<(uint32_t)std::min<uint64_t>(a.rows, kMaxGroups), kLongThreads, 0, s>>>(a));
+    if (!fits)
+        LCPP_LAUNCH(name, s,
+                    norm_forward_long_kernel<T, W, ADD>
+                    <<<(uint32_t)std::min<uint64_t>(a.rows, kMaxGroups), kLongThreads, 0, s>>>(a));
     LCPP_CHECK_LAUNCH();
     return LCPP_OK;
 }
@@ -487,19 +689,22 @@ uint64_t norm_backward_temp(uint64_t rows, uint64_t cols)
 template <class T, class W, bool ADD>
 int norm_backward_launch(const NormGradArgs &a, W *grad_weight, W *grad_bias, hipStream_t s)
 {
-    const uint32_t octets = (uint32_t)ceil_div(a.cols, kOctet);
+    const uint32_t octets = a.cols / kOctet;
     const char *name = ADD ? "layer_norm_add_backward" : "layer_norm_backward";
     uint32_t parts = 0;
-    const bool fits = norm_backward_shape(octets, [&](auto nt, auto k) {
+    const bool fits = norm_shape(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
-        constexpr int THREADS = NT > 512 ? NT : 512;
-        parts = (uint32_t)std::min<uint64_t>(ceil_div(a.rows, THREADS / NT), kMaxParts);
-        LCPP_LAUNCH(name, s, norm_backward_kernel<T, W, NT, K, THREADS, ADD><<<parts, THREADS, 0, s>>>(a));
+        constexpr int THREADS = norm_threads(NT, 512);
+        constexpr bool kAhead = K <= 2 && (NT < 1024 || sizeof(T) == 2 || !ADD);
+        static DeviceCache cache;
+        const uint64_t most = resident_groups(cache, norm_backward_kernel<T, W, NT, K, THREADS, ADD, kAhead>, THREADS);
+        parts = (uint32_t)std::min(ceil_div(a.rows, THREADS / NT), std::min(most, kMaxParts));
+        LCPP_LAUNCH(name, s, norm_backward_kernel<T, W, NT, K, THREADS, ADD, kAhead><<<parts, THREADS, 0, s>>>(a));
     });
     if (!fits) {
         if (a.partial) {
             parts = (uint32_t)std::min<uint64_t>(norm_parts(a.rows), 128);
-            const dim3 grid((uint32_t)ceil_div(octets, kColThreads), parts);
+            const dim3 grid((uint32_t)ceil_div(a.cols, kColThreads * kOctet), parts);
             LCPP_LAUNCH("layer_norm_backward_cols", s, norm_backward_cols_kernel<T><<<grid, kColThreads, 0, s>>>(a));
         }
         LCPP_LAUNCH(name, s, norm_backward_long_kernel<T, W, ADD><<<(uint32_t)std::min<uint64_t>(a.rows, kMaxGroups), kLongThreads, 0, s>>>(a));

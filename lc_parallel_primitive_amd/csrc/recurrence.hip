@@ -303,7 +303,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
     for (int r = 0; r < kRows; ++r) {
 #pragma unroll
         for (int c = 0; c < C; ++c) h.v[c] = ga[r].v[c] * h.v[c] + gb[r].v[c];
-        if (first + r < p.len && p.active) store_pack<C>(row_out<T>(a.out, p, first + r) + p.channel, h.v);
+        if (first + r < p.len && p.active) store_pack_nt<C>(row_out<T>(a.out, p, first + r) + p.channel, h.v);
     }
     // (rows past the end left h as it was)
     if (a.final_state && p.active && p.len && first <= last && last - first < kRows)
@@ -448,8 +448,8 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
                 e.v[c] = al * dh;
             }
             if (p.active) {
-                store_pack<C>(row_out<T>(a.grad_gate, p, first + r) + p.channel, dg);
-                store_pack<C>(row_out<T>(a.grad_in, p, first + r) + p.channel, dx);
+                store_pack_nt<C>(row_out<T>(a.grad_gate, p, first + r) + p.channel, dg);
+                store_pack_nt<C>(row_out<T>(a.grad_in, p, first + r) + p.channel, dx);
             }
         }
     }

@@ -67,6 +67,15 @@ __device__ __forceinline__ void store_pack(T *p, const float (&x)[N])
     for (int i = 0; i < N; ++i) v[i] = (T)x[i];
     *reinterpret_cast<typename Pack<T, N>::vec_u *>(p) = v;
 }
+// The same for results that are larger than the caches or read much later.
+template <int N, class T>
+__device__ __forceinline__ void store_pack_nt(T *p, const float (&x)[N])
+{
+    typename Pack<T, N>::vec v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (T)x[i];
+    __builtin_nontemporal_store(v, reinterpret_cast<typename Pack<T, N>::vec_u *>(p));
+}
 template <int N, class T>
 __device__ __forceinline__ void store_pack_part(T *p, const float (&x)[N], int valid)
 {

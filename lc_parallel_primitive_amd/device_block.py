@@ -19,69 +19,86 @@ and may lie any distance apart.
 from __future__ import annotations
 
 import ctypes
+import functools
 
-from ._capi import LCPP_GATES, check, float_code, lib
+from ._capi import LCPP_GATES, _float_codes, check, float_code, lib
 from .device import _Module, _nbytes, _ptr, _query, _stream
 
 
+# What a call does before its launch is most of a small call's time (device.py),
+# so a tensor's shape and strides are asked for once, refusals are worded in
+# functions of their own, and the common layouts are checked first.
+
+
 def _matrix(t, what: str):
-    """(rows, columns, row stride) of a tensor whose last dimension has unit stride."""
+    """(shape, rows, columns, row stride) of a tensor whose last dimension has unit stride."""
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
-        if shape[1] > 1 and stride[1] != 1:
-            raise ValueError(f"{what}: the columns of a row must be adjacent, got strides {stride}")
-        return shape[0], shape[1], stride[0]
+        if stride[1] == 1 or shape[1] <= 1:
+            return shape, shape[0], shape[1], stride[0]
+        raise ValueError(f"{what}: the columns of a row must be adjacent, got strides {stride}")
     if len(shape) == 0 or not t.is_contiguous():
         raise ValueError(f"{what}: must be two-dimensional or contiguous, got shape {tuple(shape)}, strides {stride}")
     cols = shape[-1]
-    return t.numel() // cols if cols else 0, cols, cols
+    return shape, t.numel() // cols if cols else 0, cols, cols
 
 
-def _like(t, ref, what: str):
-    """The row stride of a tensor that must have the shape and type of `ref`."""
-    if t.shape != ref.shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(ref.shape)}")
-    if t.dtype != ref.dtype:
-        raise TypeError(f"{what}: dtype {t.dtype}, expected {ref.dtype}")
-    return _matrix(t, what)[2]
+def _unlike(t, shape, dtype, what: str):
+    if t.shape != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype}")
 
 
-def _own_rows(t, rows: int, cols: int, stride: int, what: str):
-    if rows > 1 and stride < cols:
+def _like(t, shape, dtype, what: str):
+    """The row stride of a tensor that must have this shape and type."""
+    if t.shape != shape or t.dtype != dtype:
+        _unlike(t, shape, dtype, what)
+    stride = t.stride()
+    if len(stride) == 2 and (stride[1] == 1 or shape[1] <= 1):
+        return stride[0]
+    return _matrix(t, what)[3]
+
+
+def _like_out(t, shape, dtype, what: str):
+    """The same for an output, whose rows must not overlap."""
+    stride = _like(t, shape, dtype, what)
+    if stride < shape[-1] and len(shape) == 2 and shape[0] > 1:
         raise ValueError(f"{what}: the rows of an output must not overlap")
+    return stride
 
 
-def _vector(t, n: int, what: str, dtype_of=None):
-    """A contiguous tensor of at least n values, or None."""
+def _vector(t, n: int, what: str):
+    """The address of a contiguous tensor of at least n values, or None."""
     if t is None:
         return None
     if t.numel() < n:
         raise ValueError(f"{what}: holds {t.numel()} values, need {n}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: must be contiguous")
-    if dtype_of is not None and t.dtype != dtype_of.dtype:
-        raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype_of.dtype}")
     return t.data_ptr()
 
 
 def _float_vector(t, n: int, what: str):
-    p = _vector(t, n, what)
-    if p is not None and float_code(t.dtype) != 2:
+    if t is None:
+        return None
+    if _float_codes.get(t.dtype) != 2 and float_code(t.dtype) != 2:
         raise TypeError(f"{what}: must be float32, got {t.dtype}")
-    return p
+    return _vector(t, n, what)
 
 
 def _weight_code(code: int, *weights):
     """The lcpp_dtype of the weights that are given: the activations' or float32."""
-    wt = None
+    first = None
     for w in weights:
-        if w is not None:
-            c = float_code(w.dtype)
-            if wt is not None and c != wt:
-                raise TypeError("weight, bias and their gradients must have one dtype")
-            wt = c
-    if wt is None:
+        if w is None:
+            continue
+        if first is None:
+            first = w.dtype
+        elif w.dtype != first:
+            raise TypeError("weight, bias and their gradients must have one dtype")
+    if first is None:
         return code
+    wt = float_code(first)
     if wt != code and wt != 2:
         raise TypeError("weights must have the activations' dtype or float32")
     return wt
@@ -95,10 +112,22 @@ def _counter(t, what: str):
     return t.data_ptr()
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(lib(), name)
+
+
 _U64 = (1 << 64) - 1
 
 
-class DeviceLayerNorm(_Module):
+class _BlockModule(_Module):
+    def _call(self, name: str, temp, stream, *args):
+        status = _entry(name)(*args, stream)
+        if status or self._debug:
+            self._check(status, name, temp, stream)
+
+
+class DeviceLayerNorm(_BlockModule):
     """y = (s - mean) / sqrt(var + eps) * weight + bias over the rows of s."""
 
     @staticmethod
@@ -107,45 +136,42 @@ class DeviceLayerNorm(_Module):
 
     def Forward(self, d_in, d_out, d_weight=None, d_bias=None, eps: float = 1e-5, d_mean=None, d_rstd=None, stream=None):
         """d_out = the layer norm of d_in; d_mean, d_rstd: float32 row statistics for Backward, or None."""
-        code = float_code(d_in.dtype)
-        rows, cols, si = _matrix(d_in, "d_in")
-        so = _like(d_out, d_in, "d_out")
-        _own_rows(d_out, rows, cols, so, "d_out")
-        self._check(lib().lcpp_layer_norm_forward(
-            code, _weight_code(code, d_weight, d_bias), d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
-            _vector(d_bias, cols, "d_bias"), eps, d_out.data_ptr(), so, _float_vector(d_mean, rows, "d_mean"),
-            _float_vector(d_rstd, rows, "d_rstd"), rows, cols, _stream(stream)),
-            "lcpp_layer_norm_forward", None, stream)
+        dtype = d_in.dtype
+        code = float_code(dtype)
+        shape, rows, cols, si = _matrix(d_in, "d_in")
+        so = _like_out(d_out, shape, dtype, "d_out")
+        self._call("lcpp_layer_norm_forward", None, _stream(stream), code, _weight_code(code, d_weight, d_bias),
+                   d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"), _vector(d_bias, cols, "d_bias"), eps,
+                   d_out.data_ptr(), so, _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), rows,
+                   cols)
 
     def AddForward(self, d_in, d_residual, d_sum, d_out, d_weight=None, d_bias=None, eps: float = 1e-5, d_mean=None,
                    d_rstd=None, p: float = 0.0, seed: int = 0, offset: int = 0, d_offset=None, stream=None):
         """d_sum = d_residual + dropout(d_in), d_out = the layer norm of d_sum as it is stored.  p, seed, offset,
         d_offset as DeviceDropout.Forward."""
-        code = float_code(d_in.dtype)
-        rows, cols, si = _matrix(d_in, "d_in")
-        sr, ss, so = _like(d_residual, d_in, "d_residual"), _like(d_sum, d_in, "d_sum"), _like(d_out, d_in, "d_out")
-        _own_rows(d_sum, rows, cols, ss, "d_sum")
-        _own_rows(d_out, rows, cols, so, "d_out")
-        self._check(lib().lcpp_layer_norm_add_forward(
-            code, _weight_code(code, d_weight, d_bias), d_in.data_ptr(), si, d_residual.data_ptr(), sr, p, seed & _U64,
-            offset & _U64, _counter(d_offset, "d_offset"), _vector(d_weight, cols, "d_weight"),
-            _vector(d_bias, cols, "d_bias"), eps, d_sum.data_ptr(), ss, d_out.data_ptr(), so,
-            _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), rows, cols, _stream(stream)),
-            "lcpp_layer_norm_add_forward", None, stream)
+        dtype = d_in.dtype
+        code = float_code(dtype)
+        shape, rows, cols, si = _matrix(d_in, "d_in")
+        sr = _like(d_residual, shape, dtype, "d_residual")
+        ss, so = _like_out(d_sum, shape, dtype, "d_sum"), _like_out(d_out, shape, dtype, "d_out")
+        self._call("lcpp_layer_norm_add_forward", None, _stream(stream), code, _weight_code(code, d_weight, d_bias),
+                   d_in.data_ptr(), si, d_residual.data_ptr(), sr, p, seed & _U64, offset & _U64,
+                   _counter(d_offset, "d_offset"), _vector(d_weight, cols, "d_weight"), _vector(d_bias, cols, "d_bias"), eps,
+                   d_sum.data_ptr(), ss, d_out.data_ptr(), so, _float_vector(d_mean, rows, "d_mean"),
+                   _float_vector(d_rstd, rows, "d_rstd"), rows, cols)
 
     def Backward(self, temp_storage, d_grad_out, d_in, d_weight, d_mean, d_rstd, d_grad_in, d_grad_weight=None,
                  d_grad_bias=None, stream=None):
         """The gradients of Forward's d_in, d_weight and d_bias (the latter two None if not wanted)."""
-        code = float_code(d_in.dtype)
-        rows, cols, si = _matrix(d_in, "d_in")
-        sg, so = _like(d_grad_out, d_in, "d_grad_out"), _like(d_grad_in, d_in, "d_grad_in")
-        _own_rows(d_grad_in, rows, cols, so, "d_grad_in")
-        self._check(lib().lcpp_layer_norm_backward(
-            code, _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
-            d_grad_out.data_ptr(), sg, d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
-            _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), d_grad_in.data_ptr(), so,
-            _vector(d_grad_weight, cols, "d_grad_weight"), _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols,
-            _stream(stream)), "lcpp_layer_norm_backward", temp_storage, stream)
+        dtype = d_in.dtype
+        code = float_code(dtype)
+        shape, rows, cols, si = _matrix(d_in, "d_in")
+        sg, so = _like(d_grad_out, shape, dtype, "d_grad_out"), _like_out(d_grad_in, shape, dtype, "d_grad_in")
+        self._call("lcpp_layer_norm_backward", temp_storage, _stream(stream), code,
+                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
+                   d_grad_out.data_ptr(), sg, d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
+                   _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), d_grad_in.data_ptr(), so,
+                   _vector(d_grad_weight, cols, "d_grad_weight"), _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols)
 
     def AddBackward(self, temp_storage, d_grad_out, d_grad_sum, d_sum, d_weight, d_mean, d_rstd, d_grad_residual,
                     d_grad_in, d_grad_weight=None, d_grad_bias=None, p: float = 0.0, seed: int = 0, offset: int = 0,
@@ -153,65 +179,67 @@ class DeviceLayerNorm(_Module):
         """The gradients of AddForward.  d_grad_sum: what reaches d_sum along the residual path (None: nothing).
         d_grad_residual = d_sum's whole gradient, d_grad_in = its dropout with the forward call's random bits; either
         is None if not wanted."""
-        code = float_code(d_sum.dtype)
-        rows, cols, ss = _matrix(d_sum, "d_sum")
-        sg = _like(d_grad_out, d_sum, "d_grad_out")
-        sx, sr, si = (0 if t is None else _like(t, d_sum, nm) for t, nm in (
-            (d_grad_sum, "d_grad_sum"), (d_grad_residual, "d_grad_residual"), (d_grad_in, "d_grad_in")))
-        if d_grad_residual is not None:
-            _own_rows(d_grad_residual, rows, cols, sr, "d_grad_residual")
-        if d_grad_in is not None:
-            _own_rows(d_grad_in, rows, cols, si, "d_grad_in")
-        self._check(lib().lcpp_layer_norm_add_backward(
-            code, _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
-            d_grad_out.data_ptr(), sg, _ptr(d_grad_sum), sx, d_sum.data_ptr(), ss, _vector(d_weight, cols, "d_weight"),
-            _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), p, seed & _U64, offset & _U64,
-            _counter(d_offset, "d_offset"), _ptr(d_grad_residual), sr, _ptr(d_grad_in), si,
-            _vector(d_grad_weight, cols, "d_grad_weight"), _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols,
-            _stream(stream)), "lcpp_layer_norm_add_backward", temp_storage, stream)
+        dtype = d_sum.dtype
+        code = float_code(dtype)
+        shape, rows, cols, ss = _matrix(d_sum, "d_sum")
+        sg = _like(d_grad_out, shape, dtype, "d_grad_out")
+        sx = 0 if d_grad_sum is None else _like(d_grad_sum, shape, dtype, "d_grad_sum")
+        sr = 0 if d_grad_residual is None else _like_out(d_grad_residual, shape, dtype, "d_grad_residual")
+        si = 0 if d_grad_in is None else _like_out(d_grad_in, shape, dtype, "d_grad_in")
+        self._call("lcpp_layer_norm_add_backward", temp_storage, _stream(stream), code,
+                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
+                   d_grad_out.data_ptr(), sg, _ptr(d_grad_sum), sx, d_sum.data_ptr(), ss,
+                   _vector(d_weight, cols, "d_weight"), _float_vector(d_mean, rows, "d_mean"),
+                   _float_vector(d_rstd, rows, "d_rstd"), p, seed & _U64, offset & _U64, _counter(d_offset, "d_offset"),
+                   _ptr(d_grad_residual), sr, _ptr(d_grad_in), si, _vector(d_grad_weight, cols, "d_grad_weight"),
+                   _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols)
 
 
-class DeviceDropout(_Module):
+class DeviceDropout(_BlockModule):
     """Dropout whose mask is computed from (seed, offset, row, column) wherever it is needed, and never stored."""
 
     def Forward(self, d_in, d_out, p: float, seed: int, offset: int = 0, d_residual=None, d_offset=None, stream=None):
         """d_out = (kept ? d_in / (1 - p) : 0) [+ d_residual].  p is met to 2^-17.  offset tells the calls of one seed
         apart (a layer's number, a step's); d_offset, a device tensor of one 64-bit integer, is added to it when the
         kernel runs, so a captured graph's replays can differ."""
-        code = float_code(d_in.dtype)
-        rows, cols, si = _matrix(d_in, "d_in")
-        so = _like(d_out, d_in, "d_out")
-        _own_rows(d_out, rows, cols, so, "d_out")
-        sr = 0 if d_residual is None else _like(d_residual, d_in, "d_residual")
-        self._check(lib().lcpp_dropout(code, d_in.data_ptr(), si, _ptr(d_residual), sr, d_out.data_ptr(), so, rows, cols, p,
-                                       seed & _U64, offset & _U64, _counter(d_offset, "d_offset"), _stream(stream)),
-                    "lcpp_dropout", None, stream)
+        dtype = d_in.dtype
+        shape, rows, cols, si = _matrix(d_in, "d_in")
+        so = _like_out(d_out, shape, dtype, "d_out")
+        sr = 0 if d_residual is None else _like(d_residual, shape, dtype, "d_residual")
+        self._call("lcpp_dropout", None, _stream(stream), float_code(dtype), d_in.data_ptr(), si, _ptr(d_residual), sr,
+                   d_out.data_ptr(), so, rows, cols, p, seed & _U64, offset & _U64, _counter(d_offset, "d_offset"))
 
     def Backward(self, d_grad_out, d_grad_in, p: float, seed: int, offset: int = 0, d_offset=None, stream=None):
         """The gradient of Forward's d_in, with the forward call's p, seed and offset (d_residual's is d_grad_out itself)."""
         self.Forward(d_grad_out, d_grad_in, p, seed, offset, None, d_offset, stream)
 
 
-def _sequence_strides(t, ref, what: str, packed: bool, output: bool = False):
-    """(row stride, sequence stride) of (sequences, rows, channels), or with offsets (rows, channels)."""
-    if t.shape != ref.shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(ref.shape)}")
-    if t.dtype != ref.dtype:
-        raise TypeError(f"{what}: dtype {t.dtype}, expected {ref.dtype}")
-    stride, shape = t.stride(), t.shape
-    if shape[-1] > 1 and stride[-1] != 1:
+def _sequence_strides(t, shape, dtype, what: str, output: bool = False):
+    """(address, row stride, sequence stride) of a tensor of shape (sequences, rows, channels), or with offsets (rows,
+    channels)."""
+    if t.shape != shape or t.dtype != dtype:
+        _unlike(t, shape, dtype, what)
+    stride = t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{what}: the channels of a row must be adjacent, got strides {stride}")
-    if output:
+    if output and not (stride[-2] >= shape[-1] and (len(shape) == 2 or stride[0] >= stride[1] * shape[1])):
         # no two rows may share memory: in the order of their strides, each dimension steps over the one below it
         span = shape[-1]
         for n, st in sorted(((n, st) for n, st in zip(shape[:-1], stride[:-1]) if n > 1), key=lambda d: d[1]):
             if st < span:
                 raise ValueError(f"{what}: the rows of an output must not overlap, got strides {stride}")
             span = st * n
-    return (stride[0], 0) if packed else (stride[1], stride[0])
+    return (t.data_ptr(), stride[0], 0) if len(shape) == 2 else (t.data_ptr(), stride[1], stride[0])
 
 
-class DeviceGatedRecurrence(_Module):
+@functools.lru_cache(maxsize=1024)
+def _checkpoint_rows(max_length: int) -> int:
+    out = ctypes.c_uint64()
+    check(lib().lcpp_recurrence_checkpoint_rows(max_length, ctypes.byref(out)), "lcpp_recurrence_checkpoint_rows")
+    return out.value
+
+
+class DeviceGatedRecurrence(_BlockModule):
     """h_t = a_t h_{t-1} + b_t per channel, with a and b from a gate g and an input x:
 
         "decay"    a = g, b = x
@@ -229,92 +257,87 @@ class DeviceGatedRecurrence(_Module):
     @staticmethod
     def GetCheckpointRows(max_length: int) -> int:
         """d_checkpoints has shape (sequences, this, channels), float32."""
-        out = ctypes.c_uint64()
-        check(lib().lcpp_recurrence_checkpoint_rows(max_length, ctypes.byref(out)), "lcpp_recurrence_checkpoint_rows")
-        return out.value
+        return _checkpoint_rows(max_length)
 
-    def _sizes(self, d_gate, d_in, gate, d_begin_offsets, d_end_offsets, max_length):
-        if gate not in LCPP_GATES:
+    @staticmethod
+    def _gate(gate):
+        code = LCPP_GATES.get(gate)
+        if code is None:
             raise ValueError(f"unsupported gate {gate!r}: one of {', '.join(LCPP_GATES)}")
-        packed = d_begin_offsets is not None
-        if packed != (d_end_offsets is not None):
+        return code
+
+    @staticmethod
+    def _sizes(shape, begin, end, max_length):
+        """The last arguments of the C calls: sequences, max_length, channels, begin, end, rows."""
+        if (begin is None) != (end is None):
             raise ValueError("begin and end offsets go together")
-        if d_in.dim() != (2 if packed else 3):
-            raise ValueError("d_in: shape (sequences, length, channels), or with offsets (rows, channels)")
-        if packed:
-            if d_begin_offsets.element_size() != 4 or d_end_offsets.element_size() != 4:
-                raise TypeError("offsets must be 32-bit")
-            if max_length is None:
-                raise ValueError("offsets need max_length")
-            sequences, (rows, channels) = d_begin_offsets.numel(), d_in.shape
-            if d_end_offsets.numel() != sequences or not (d_begin_offsets.is_contiguous() and d_end_offsets.is_contiguous()):
-                raise ValueError("begin and end offsets must be contiguous and of one length")
-        else:
+        if begin is None:
+            if len(shape) != 3:
+                raise ValueError("d_in: shape (sequences, length, channels), or with offsets (rows, channels)")
             if max_length is not None:
                 raise ValueError("max_length goes with offsets")
-            sequences, max_length, channels = d_in.shape
-            rows = 0
-        return packed, (sequences, max_length, channels, _ptr(d_begin_offsets), _ptr(d_end_offsets), rows)
+            return (*shape, None, None, 0)
+        if len(shape) != 2:
+            raise ValueError("d_in: shape (sequences, length, channels), or with offsets (rows, channels)")
+        if begin.element_size() != 4 or end.element_size() != 4 or begin.is_floating_point() or end.is_floating_point():
+            raise TypeError("offsets must be 32-bit integers")
+        if max_length is None:
+            raise ValueError("offsets need max_length")
+        if begin.numel() != end.numel() or not (begin.is_contiguous() and end.is_contiguous()):
+            raise ValueError("begin and end offsets must be contiguous and of one length")
+        return begin.numel(), max_length, shape[1], begin.data_ptr(), end.data_ptr(), shape[0]
 
     def Forward(self, temp_storage, d_gate, d_in, d_out, gate: str, d_initial=None, d_final=None, d_checkpoints=None,
                 d_begin_offsets=None, d_end_offsets=None, max_length=None, stream=None):
         """d_out = h for every row.  d_initial: the states before the first rows (None: 0); d_final: those after the
         last; d_checkpoints: what Backward needs."""
-        code = float_code(d_in.dtype)
-        packed, sizes = self._sizes(d_gate, d_in, gate, d_begin_offsets, d_end_offsets, max_length)
+        shape, dtype, kind = d_in.shape, d_in.dtype, self._gate(gate)
+        sizes = self._sizes(shape, d_begin_offsets, d_end_offsets, max_length)
         states = sizes[0] * sizes[2]
-        g = _sequence_strides(d_gate, d_in, "d_gate", packed)
-        x = _sequence_strides(d_in, d_in, "d_in", packed)
-        y = _sequence_strides(d_out, d_in, "d_out", packed, True)
         saved = None
         if d_checkpoints is not None:
-            saved = _float_vector(d_checkpoints, states * self.GetCheckpointRows(sizes[1]), "d_checkpoints")
-        self._check(lib().lcpp_recurrence_forward(
-            code, LCPP_GATES[gate], _ptr(temp_storage), _nbytes(temp_storage), d_gate.data_ptr(), *g, d_in.data_ptr(), *x,
-            d_out.data_ptr(), *y, _float_vector(d_initial, states, "d_initial"), _float_vector(d_final, states, "d_final"),
-            saved, *sizes, _stream(stream)), "lcpp_recurrence_forward", temp_storage, stream)
+            saved = _float_vector(d_checkpoints, states * _checkpoint_rows(sizes[1]), "d_checkpoints")
+        self._call("lcpp_recurrence_forward", temp_storage, _stream(stream), float_code(dtype), kind, _ptr(temp_storage),
+                   _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+                   *_sequence_strides(d_in, shape, dtype, "d_in"), *_sequence_strides(d_out, shape, dtype, "d_out", True),
+                   _float_vector(d_initial, states, "d_initial"), _float_vector(d_final, states, "d_final"), saved, *sizes)
 
     def Backward(self, temp_storage, d_gate, d_in, d_checkpoints, d_grad_out, d_grad_gate, d_grad_in, gate: str,
                  d_grad_final=None, d_grad_initial=None, d_begin_offsets=None, d_end_offsets=None, max_length=None,
                  stream=None):
         """The gradients of Forward's d_gate, d_in and d_initial from those of d_out and d_final (None: 0)."""
-        code = float_code(d_in.dtype)
-        packed, sizes = self._sizes(d_gate, d_in, gate, d_begin_offsets, d_end_offsets, max_length)
+        shape, dtype, kind = d_in.shape, d_in.dtype, self._gate(gate)
+        sizes = self._sizes(shape, d_begin_offsets, d_end_offsets, max_length)
         states = sizes[0] * sizes[2]
-        g = _sequence_strides(d_gate, d_in, "d_gate", packed)
-        x = _sequence_strides(d_in, d_in, "d_in", packed)
-        dy = _sequence_strides(d_grad_out, d_in, "d_grad_out", packed)
-        dg = _sequence_strides(d_grad_gate, d_in, "d_grad_gate", packed, True)
-        dx = _sequence_strides(d_grad_in, d_in, "d_grad_in", packed, True)
-        self._check(lib().lcpp_recurrence_backward(
-            code, LCPP_GATES[gate], _ptr(temp_storage), _nbytes(temp_storage), d_gate.data_ptr(), *g, d_in.data_ptr(), *x,
-            _float_vector(d_checkpoints, states * self.GetCheckpointRows(sizes[1]), "d_checkpoints"), d_grad_out.data_ptr(),
-            *dy, d_grad_gate.data_ptr(), *dg, d_grad_in.data_ptr(), *dx,
-            _float_vector(d_grad_final, states, "d_grad_final"), _float_vector(d_grad_initial, states, "d_grad_initial"),
-            *sizes, _stream(stream)), "lcpp_recurrence_backward", temp_storage, stream)
+        self._call("lcpp_recurrence_backward", temp_storage, _stream(stream), float_code(dtype), kind, _ptr(temp_storage),
+                   _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+                   *_sequence_strides(d_in, shape, dtype, "d_in"),
+                   _float_vector(d_checkpoints, states * _checkpoint_rows(sizes[1]), "d_checkpoints"),
+                   *_sequence_strides(d_grad_out, shape, dtype, "d_grad_out"),
+                   *_sequence_strides(d_grad_gate, shape, dtype, "d_grad_gate", True),
+                   *_sequence_strides(d_grad_in, shape, dtype, "d_grad_in", True),
+                   _float_vector(d_grad_final, states, "d_grad_final"),
+                   _float_vector(d_grad_initial, states, "d_grad_initial"), *sizes)
 
     def Step(self, d_gate, d_in, d_state_in, d_state_out, d_out, gate: str, d_slots=None, stream=None):
         """One token for each of some sequences: d_gate, d_in and d_out of shape (sequences, channels).  The states are
         float32 of shape (slots, channels); d_state_out may be d_state_in.  d_slots: int32, the row of each sequence's
         state, all different; -1 marks padding (out is 0, no state changes).  None: row s for sequence s."""
-        if gate not in LCPP_GATES:
-            raise ValueError(f"unsupported gate {gate!r}: one of {', '.join(LCPP_GATES)}")
-        code = float_code(d_in.dtype)
-        if d_in.dim() != 2:
+        kind, dtype = self._gate(gate), d_in.dtype
+        shape, rows, cols, sx = _matrix(d_in, "d_in")
+        if len(shape) != 2:
             raise ValueError("d_in: shape (sequences, channels)")
-        rows, cols, sx = _matrix(d_in, "d_in")
-        sg, so = _like(d_gate, d_in, "d_gate"), _like(d_out, d_in, "d_out")
-        _own_rows(d_out, rows, cols, so, "d_out")
-        if d_state_in.shape != d_state_out.shape or d_state_in.dim() != 2 or d_state_in.shape[1] != cols:
-            raise ValueError(f"states: shapes {tuple(d_state_in.shape)} and {tuple(d_state_out.shape)}, expected (slots, {cols})")
-        slots = d_state_in.shape[0]
+        sg, so = _like(d_gate, shape, dtype, "d_gate"), _like_out(d_out, shape, dtype, "d_out")
+        pool = d_state_in.shape
+        if len(pool) != 2 or pool[1] != cols or d_state_out.shape != pool:
+            raise ValueError(f"states: shapes {tuple(pool)} and {tuple(d_state_out.shape)}, expected (slots, {cols})")
+        slots = pool[0]
         if d_slots is not None:
             if d_slots.element_size() != 4 or d_slots.is_floating_point():
                 raise TypeError("d_slots: must be int32")
-            _vector(d_slots, rows, "d_slots")
         elif slots < rows:
             raise ValueError(f"states: {slots} rows for {rows} sequences")
-        self._check(lib().lcpp_recurrence_step(
-            code, LCPP_GATES[gate], d_gate.data_ptr(), sg, d_in.data_ptr(), sx, _float_vector(d_state_in, 0, "d_state_in"),
-            _float_vector(d_state_out, 0, "d_state_out"), _ptr(d_slots), slots, d_out.data_ptr(), so, rows, cols,
-            _stream(stream)), "lcpp_recurrence_step", None, stream)
+        self._call("lcpp_recurrence_step", None, _stream(stream), float_code(dtype), kind, d_gate.data_ptr(), sg,
+                   d_in.data_ptr(), sx, _float_vector(d_state_in, 0, "d_state_in"),
+                   _float_vector(d_state_out, 0, "d_state_out"), _vector(d_slots, rows, "d_slots"), slots, d_out.data_ptr(),
+                   so, rows, cols)
