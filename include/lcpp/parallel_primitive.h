@@ -550,6 +550,176 @@ class DeviceSegmentReduce : public LuisaModule {
     }
 };
 
+/* ---- layer norm, dropout, gated linear recurrence (no counterpart in the reference; see lcpp_amd.h) */
+
+/* Activations: float, or the 16 bits of a bfloat16 or IEEE half value. */
+struct bfloat16 {
+    uint16_t bits;
+};
+struct float16 {
+    uint16_t bits;
+};
+template <class T>
+constexpr lcpp_dtype activation_dtype_of()
+{
+    using U = std::remove_cv_t<T>;
+    if constexpr (std::is_same_v<U, float>) return LCPP_FLOAT32;
+    else if constexpr (std::is_same_v<U, bfloat16>) return LCPP_BFLOAT16;
+    else if constexpr (std::is_same_v<U, float16>) return LCPP_FLOAT16;
+    else static_assert(sizeof(U) == 0, "activations are float, bfloat16 or float16");
+}
+
+/* Rows of a device matrix, `stride` elements apart; of a batch of sequences, `sequence_stride` apart. */
+template <class T>
+struct RowsView {
+    T *ptr = nullptr;
+    size_t stride = 0;
+    size_t sequence_stride = 0;
+    [[nodiscard]] T *data() const noexcept { return ptr; }
+};
+
+/* What makes a dropout call's mask. */
+struct DropoutState {
+    double p = 0.0;
+    uint64_t seed = 0, offset = 0;
+    const uint64_t *d_offset = nullptr; /* device counter added to offset, or null */
+};
+
+class DeviceLayerNorm : public LuisaModule {
+  public:
+    template <class T>
+    static size_t GetBackwardTempStorageBytes(size_t rows, size_t cols)
+    {
+        size_t b = 0;
+        lcpp_layer_norm_backward_temp_bytes(activation_dtype_of<T>(), rows, cols, &b);
+        return b;
+    }
+    /* d_weight, d_bias, d_mean, d_rstd may be null */
+    template <class T, class W>
+    void Forward(CommandList &cmdlist, RowsView<T> d_in, RowsView<T> d_out, const W *d_weight, const W *d_bias, float eps,
+                 float *d_mean, float *d_rstd, size_t rows, size_t cols)
+    {
+        check(lcpp_layer_norm_forward(activation_dtype_of<T>(), activation_dtype_of<W>(), d_in.data(), d_in.stride, d_weight,
+                                      d_bias, eps, d_out.data(), d_out.stride, d_mean, d_rstd, rows, cols, cmdlist.stream),
+              "DeviceLayerNorm::Forward", cmdlist.stream);
+    }
+    template <class T, class W>
+    void AddForward(CommandList &cmdlist, RowsView<T> d_in, RowsView<T> d_residual, const DropoutState &drop,
+                    RowsView<T> d_sum, RowsView<T> d_out, const W *d_weight, const W *d_bias, float eps, float *d_mean,
+                    float *d_rstd, size_t rows, size_t cols)
+    {
+        check(lcpp_layer_norm_add_forward(activation_dtype_of<T>(), activation_dtype_of<W>(), d_in.data(), d_in.stride,
+                                          d_residual.data(), d_residual.stride, drop.p, drop.seed, drop.offset, drop.d_offset,
+                                          d_weight, d_bias, eps, d_sum.data(), d_sum.stride, d_out.data(), d_out.stride,
+                                          d_mean, d_rstd, rows, cols, cmdlist.stream),
+              "DeviceLayerNorm::AddForward", cmdlist.stream);
+    }
+    template <class T, class W>
+    void Backward(CommandList &cmdlist, BufferView<uint> temp_storage, RowsView<T> d_grad_out, RowsView<T> d_in,
+                  const W *d_weight, const float *d_mean, const float *d_rstd, RowsView<T> d_grad_in, W *d_grad_weight,
+                  W *d_grad_bias, size_t rows, size_t cols)
+    {
+        check(lcpp_layer_norm_backward(activation_dtype_of<T>(), activation_dtype_of<W>(), temp_storage.data(),
+                                       temp_storage.size_bytes(), d_grad_out.data(), d_grad_out.stride, d_in.data(),
+                                       d_in.stride, d_weight, d_mean, d_rstd, d_grad_in.data(), d_grad_in.stride,
+                                       d_grad_weight, d_grad_bias, rows, cols, cmdlist.stream),
+              "DeviceLayerNorm::Backward", cmdlist.stream, temp_storage);
+    }
+    template <class T, class W>
+    void AddBackward(CommandList &cmdlist, BufferView<uint> temp_storage, RowsView<T> d_grad_out, RowsView<T> d_grad_sum,
+                     RowsView<T> d_sum, const W *d_weight, const float *d_mean, const float *d_rstd, const DropoutState &drop,
+                     RowsView<T> d_grad_residual, RowsView<T> d_grad_in, W *d_grad_weight, W *d_grad_bias, size_t rows,
+                     size_t cols)
+    {
+        check(lcpp_layer_norm_add_backward(activation_dtype_of<T>(), activation_dtype_of<W>(), temp_storage.data(),
+                                           temp_storage.size_bytes(), d_grad_out.data(), d_grad_out.stride,
+                                           d_grad_sum.data(), d_grad_sum.stride, d_sum.data(), d_sum.stride, d_weight, d_mean,
+                                           d_rstd, drop.p, drop.seed, drop.offset, drop.d_offset, d_grad_residual.data(),
+                                           d_grad_residual.stride, d_grad_in.data(), d_grad_in.stride, d_grad_weight,
+                                           d_grad_bias, rows, cols, cmdlist.stream),
+              "DeviceLayerNorm::AddBackward", cmdlist.stream, temp_storage);
+    }
+};
+
+class DeviceDropout : public LuisaModule {
+  public:
+    /* d_residual: a view of null for none; the backward pass is Backward with the same state */
+    template <class T>
+    void Forward(CommandList &cmdlist, RowsView<T> d_in, RowsView<T> d_out, const DropoutState &drop, size_t rows, size_t cols,
+                 RowsView<T> d_residual = {})
+    {
+        check(lcpp_dropout(activation_dtype_of<T>(), d_in.data(), d_in.stride, d_residual.data(), d_residual.stride,
+                           d_out.data(), d_out.stride, rows, cols, drop.p, drop.seed, drop.offset, drop.d_offset,
+                           cmdlist.stream),
+              "DeviceDropout::Forward", cmdlist.stream);
+    }
+    template <class T>
+    void Backward(CommandList &cmdlist, RowsView<T> d_grad_out, RowsView<T> d_grad_in, const DropoutState &drop, size_t rows,
+                  size_t cols)
+    {
+        Forward<T>(cmdlist, d_grad_out, d_grad_in, drop, rows, cols);
+    }
+};
+
+/* Where the sequences of a recurrence call lie: `count` of `length` rows each, or with offsets rows
+ * d_begin[s] .. d_end[s] of `rows` rows, none longer than `length`. */
+struct Sequences {
+    size_t count = 0, length = 0, channels = 0;
+    const uint32_t *d_begin = nullptr, *d_end = nullptr;
+    size_t rows = 0;
+};
+
+class DeviceGatedRecurrence : public LuisaModule {
+  public:
+    static size_t GetTempStorageBytes(size_t sequences, size_t max_length, size_t channels)
+    {
+        size_t b = 0;
+        lcpp_recurrence_temp_bytes(sequences, max_length, channels, &b);
+        return b;
+    }
+    static size_t GetCheckpointRows(size_t max_length)
+    {
+        uint64_t r = 0;
+        lcpp_recurrence_checkpoint_rows(max_length, &r);
+        return r;
+    }
+    template <class T>
+    void Forward(CommandList &cmdlist, BufferView<uint> temp_storage, lcpp_gate gate, RowsView<T> d_gate, RowsView<T> d_in,
+                 RowsView<T> d_out, const float *d_initial, float *d_final, float *d_checkpoints, const Sequences &seq)
+    {
+        check(lcpp_recurrence_forward(activation_dtype_of<T>(), gate, temp_storage.data(), temp_storage.size_bytes(),
+                                      d_gate.data(), d_gate.stride, d_gate.sequence_stride, d_in.data(), d_in.stride,
+                                      d_in.sequence_stride, d_out.data(), d_out.stride, d_out.sequence_stride, d_initial,
+                                      d_final, d_checkpoints, seq.count, seq.length, seq.channels, seq.d_begin, seq.d_end,
+                                      seq.rows, cmdlist.stream),
+              "DeviceGatedRecurrence::Forward", cmdlist.stream, temp_storage);
+    }
+    template <class T>
+    void Backward(CommandList &cmdlist, BufferView<uint> temp_storage, lcpp_gate gate, RowsView<T> d_gate, RowsView<T> d_in,
+                  const float *d_checkpoints, RowsView<T> d_grad_out, RowsView<T> d_grad_gate, RowsView<T> d_grad_in,
+                  const float *d_grad_final, float *d_grad_initial, const Sequences &seq)
+    {
+        check(lcpp_recurrence_backward(activation_dtype_of<T>(), gate, temp_storage.data(), temp_storage.size_bytes(),
+                                       d_gate.data(), d_gate.stride, d_gate.sequence_stride, d_in.data(), d_in.stride,
+                                       d_in.sequence_stride, d_checkpoints, d_grad_out.data(), d_grad_out.stride,
+                                       d_grad_out.sequence_stride, d_grad_gate.data(), d_grad_gate.stride,
+                                       d_grad_gate.sequence_stride, d_grad_in.data(), d_grad_in.stride,
+                                       d_grad_in.sequence_stride, d_grad_final, d_grad_initial, seq.count, seq.length,
+                                       seq.channels, seq.d_begin, seq.d_end, seq.rows, cmdlist.stream),
+              "DeviceGatedRecurrence::Backward", cmdlist.stream, temp_storage);
+    }
+    /* d_slots null: sequence s has the state of row s */
+    template <class T>
+    void Step(CommandList &cmdlist, lcpp_gate gate, RowsView<T> d_gate, RowsView<T> d_in, const float *d_state_in,
+              float *d_state_out, const int32_t *d_slots, size_t num_slots, RowsView<T> d_out, size_t sequences, size_t channels)
+    {
+        check(lcpp_recurrence_step(activation_dtype_of<T>(), gate, d_gate.data(), d_gate.stride, d_in.data(), d_in.stride,
+                                   d_state_in, d_state_out, d_slots, num_slots, d_out.data(), d_out.stride, sequences, channels,
+                                   cmdlist.stream),
+              "DeviceGatedRecurrence::Step", cmdlist.stream);
+    }
+};
+
 }  // namespace luisa::parallel_primitive
 
 #endif /* LCPP_PARALLEL_PRIMITIVE_H */
