@@ -64,6 +64,24 @@ struct RowPart {
     }
 };
 
+// Sum over a row's threads within a wave: all 64 lanes, or the 16 or 32 of a
+// narrow row, whose wave works on several rows.
+template <int NT>
+__device__ __forceinline__ float lanes_sum(float x)
+{
+    if constexpr (NT >= kWave) {
+        return wave_reduce_dpp(x, SumOp());
+    } else {
+        static_assert(NT == 16 || NT == 32, "rows of a wave");
+        x += dpp_perm<kDppQuadXor1>(x);
+        x += dpp_perm<kDppQuadXor2>(x);
+        x += dpp_perm<kDppRowHalfMirror>(x);
+        x += dpp_perm<kDppRowMirror>(x);
+        if constexpr (NT == 32) x += shfl_xor(x, 16);
+        return x;
+    }
+}
+
 // Sums of V values over the NT threads of a row's group; every thread of the
 // group gets them.  A group of several waves meets in LDS, all groups of the
 // workgroup at the same barrier; `slot` alternates from row to row, so one
@@ -72,7 +90,7 @@ template <int NT, int WAVES, int V>
 __device__ __forceinline__ void group_sum(float (&x)[V], float (*lds)[WAVES][2], int slot)
 {
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = wave_reduce_dpp(x[v], SumOp());
+    for (int v = 0; v < V; ++v) x[v] = lanes_sum<NT>(x[v]);
     if constexpr (NT > kWave) {
         constexpr int GW = NT / kWave;
         const uint32_t wave = threadIdx.x / kWave;
@@ -104,13 +122,13 @@ __device__ __forceinline__ void group_moments(F each, float count, float (*lds)[
     float sum = 0.0f;
     each([&](float x) { sum += x; });
     const float inv = count > 0.0f ? 1.0f / count : 0.0f;
-    mean = wave_reduce_dpp(sum, SumOp()) * inv;
+    mean = lanes_sum<NT>(sum) * inv;
     float sq = 0.0f;
     each([&](float x) {
         const float d = x - mean;
         sq += d * d;
     });
-    sq = wave_reduce_dpp(sq, SumOp());
+    sq = lanes_sum<NT>(sq);
     if constexpr (NT > kWave) {
         constexpr int GW = NT / kWave;
         const uint32_t wave = threadIdx.x / kWave, first = wave / GW * GW;
@@ -133,6 +151,17 @@ __device__ __forceinline__ void group_moments(F each, float count, float (*lds)[
         }
     }
     var = sq / cols;
+}
+
+// One octet of a vector of weights, or one value everywhere.
+template <class W>
+__device__ __forceinline__ Octet<W> octet_or(const void *p, uint32_t col, float value)
+{
+    if (p) return load_pack<kOctet>(static_cast<const W *>(p) + col);
+    Octet<W> o;
+#pragma unroll
+    for (int i = 0; i < kOctet; ++i) o.v[i] = (W)value;
+    return o;
 }
 
 struct NormArgs {
@@ -161,9 +190,10 @@ __device__ __forceinline__ float drop_one(float x, uint32_t row, uint32_t col, u
 // while these are worked on, and the weights in registers too (AHEAD: where the
 // registers hold that).
 template <class T, class W, int NT, int K, int THREADS, bool ADD, bool AHEAD>
-__global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ? 1 : ADD && sizeof(T) == 4 ? 2 : 4))) void norm_forward_kernel(NormArgs a)
 {
-    constexpr int WAVES = THREADS / kWave, RG = THREADS / NT, GW = NT / kWave;
+    constexpr int WAVES = THREADS / kWave, RG = THREADS / NT, GW = NT > kWave ? NT / kWave : 1;
+    constexpr uint32_t kLaneCols = (NT < kWave ? NT : kWave) * kOctet;
     __shared__ float lds[2][WAVES][2];
     const Columns<NT, K> c(a.cols);
     const uint32_t group = threadIdx.x / NT;
@@ -176,7 +206,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const uint32_t from = (w * kWave + k * NT) * kOctet;
-            n += from < c.full ? (c.full - from < kWave * kOctet ? c.full - from : kWave * kOctet) : 0;
+            n += from < c.full ? (c.full - from < kLaneCols ? c.full - from : kLaneCols) : 0;
         }
         counts[w] = (float)(n + (w == 0 ? c.rem : 0));
     }
@@ -195,7 +225,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
     auto load = [&](uint64_t row) {
         if (row >= a.rows) return;
         next.load(in + row * a.in_stride, c);
-        if constexpr (ADD) next_r.load(residual + row * a.residual_stride, c);
+        if constexpr (ADD && AHEAD) next_r.load(residual + row * a.residual_stride, c);
     };
     uint64_t row = (uint64_t)blockIdx.x * RG + group;
     if constexpr (AHEAD) load(row);
@@ -215,6 +245,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
                 for (int k = 0; k < K; ++k) {
                     if (!c.has(k)) continue;
                     float v[kOctet];
+                    if constexpr (!AHEAD) r.o[k] = load_pack<kOctet>(residual + row * a.residual_stride + c.col(k));
 #pragma unroll
                     for (int i = 0; i < kOctet; ++i) v[i] = x.o[k][i];
                     if (a.drop.cut) drop_octet(v, (uint32_t)row, c.col(k) / kOctet, offset, a.drop);
@@ -227,6 +258,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
                 }
                 if (c.has_tail()) {
                     float v = (float)x.tail;
+                    if constexpr (!AHEAD) r.tail = residual[row * a.residual_stride + c.tail()];
                     if (a.drop.cut) v = drop_one(v, (uint32_t)row, c.tail(), offset, a.drop);
                     x.tail = (T)(v + (float)r.tail);
                     sum[c.tail()] = x.tail;
@@ -247,18 +279,24 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs a)
             count, lds, counts, slot, (float)a.cols, mean, var);
         const float rstd = 1.0f / sqrtf(var + a.eps);
         if (!live) continue;
-        if constexpr (!AHEAD) {
-            w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
-            b.load_or(static_cast<const W *>(a.bias), c, 0.0f);
-        }
         T *out = static_cast<T *>(a.out) + row * a.out_stride;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!c.has(k)) continue;
+            if constexpr (!AHEAD) {
+                w.o[k] = octet_or<W>(a.weight, c.col(k), 1.0f);
+                b.o[k] = octet_or<W>(a.bias, c.col(k), 0.0f);
+            }
             float y[kOctet];
 #pragma unroll
             for (int i = 0; i < kOctet; ++i) y[i] = (x.o[k][i] - mean) * rstd * w.o[k][i] + b.o[k][i];
             store_pack_nt<kOctet>(out + c.col(k), y);
+        }
+        if constexpr (!AHEAD) {
+            if (c.has_tail()) {
+                w.tail = a.weight ? static_cast<const W *>(a.weight)[c.tail()] : (W)1.0f;
+                b.tail = a.bias ? static_cast<const W *>(a.bias)[c.tail()] : (W)0.0f;
+            }
         }
         if (c.has_tail()) out[c.tail()] = (T)(((float)x.tail - mean) * rstd * (float)w.tail + (float)b.tail);
         if (c.t == 0) {
@@ -366,12 +404,14 @@ struct NormGradArgs {
 // THREADS / NT rows at a time; a thread keeps the same columns for all of its
 // workgroup's rows, so dw and db are sums in its registers, one partial sum per
 // workgroup at the end.  The next rows are on their way while these are worked on.
-template <class T, class W, int NT, int K, int THREADS, bool ADD, bool AHEAD>
+template <class T, class W, int NT, int K, int THREADS, bool ADD, bool AHEAD, bool ACC>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
 {
     constexpr int WAVES = THREADS / kWave, RG = THREADS / NT;
     __shared__ float lds[2][WAVES][2];
-    __shared__ float fold[RG > 1 ? NT * K * kOctet : 1], fold_tail[RG > 1 ? kOctet : 1];
+    // (a wave with several rows adds their sums up first)
+    constexpr int FOLD = NT < kWave ? WAVES : RG;
+    __shared__ float fold[FOLD > 1 ? NT * K * kOctet : 1], fold_tail[FOLD > 1 ? kOctet : 1];
     const Columns<NT, K> c(a.cols);
     const uint32_t group = threadIdx.x / NT;
     const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
@@ -405,22 +445,25 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
         const float mean = next_mean, rstd = next_rstd;
         const bool live = row < a.rows;
         if constexpr (AHEAD) load(row + stride);
-        else w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
         float sums[2] = {0.0f, 0.0f};
         if (live) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (!c.has(k)) continue;
+                if constexpr (!AHEAD) w.o[k] = octet_or<W>(a.weight, c.col(k), 1.0f);
 #pragma unroll
                 for (int i = 0; i < kOctet; ++i) {
                     const float u = (s.o[k][i] - mean) * rstd, v = dy.o[k][i] * w.o[k][i];
                     sums[0] += v;
                     sums[1] += v * u;
-                    dw[k][i] += dy.o[k][i] * u;
-                    db[k][i] += dy.o[k][i];
+                    if constexpr (ACC) {
+                        dw[k][i] += dy.o[k][i] * u;
+                        db[k][i] += dy.o[k][i];
+                    }
                 }
             }
             if (c.has_tail()) {
+                if constexpr (!AHEAD) w.tail = a.weight ? static_cast<const W *>(a.weight)[c.tail()] : (W)1.0f;
                 const float u = ((float)s.tail - mean) * rstd, v = (float)dy.tail * (float)w.tail;
                 sums[0] += v;
                 sums[1] += v * u;
@@ -430,18 +473,18 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
         }
         group_sum<NT, WAVES>(sums, lds, slot);
         if (!live) continue;
-        if constexpr (!AHEAD) {
-            w.load_or(static_cast<const W *>(a.weight), c, 1.0f);
-            if constexpr (ADD) {
-                if (grad_sum) g.load(grad_sum + row * a.gs_stride, c);
-            }
-        }
         const float mean_v = sums[0] * inv, mean_vu = sums[1] * inv;
         T *gi = static_cast<T *>(a.grad_in) + row * a.gi_stride, *gb = static_cast<T *>(a.grad_branch) + row * a.gb_stride;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!c.has(k)) continue;
             float d[kOctet];
+            if constexpr (!AHEAD) {
+                w.o[k] = octet_or<W>(a.weight, c.col(k), 1.0f);
+                if constexpr (ADD) {
+                    if (grad_sum) g.o[k] = load_pack<kOctet>(grad_sum + row * a.gs_stride + c.col(k));
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kOctet; ++i) {
                 const float u = (s.o[k][i] - mean) * rstd, v = dy.o[k][i] * w.o[k][i];
@@ -465,6 +508,9 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
             const float u = ((float)s.tail - mean) * rstd, v = (float)dy.tail * (float)w.tail;
             float d = rstd * (v - mean_v - u * mean_vu);
             if constexpr (ADD) {
+                if constexpr (!AHEAD) {
+                    if (grad_sum) g.tail = grad_sum[row * a.gs_stride + c.tail()];
+                }
                 if (grad_sum) d += (float)g.tail;
             }
             if (a.grad_in) gi[c.tail()] = (T)d;
@@ -476,16 +522,31 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
             }
         }
     }
-    if (!a.partial) return;
+    if (!ACC || !a.partial) return;
     float *part = a.partial + (uint64_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
     for (int half = 0; half < 2; ++half, part += a.cols) {
         float(&x)[K][kOctet] = half ? db : dw;
         float &tail = half ? db_tail : dw_tail;
-        if constexpr (RG > 1) {
+        uint32_t turn = group;
+        bool writes = group == RG - 1;
+        if constexpr (NT < kWave) {
+#pragma unroll
+            for (int step = NT; step < kWave; step *= 2) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < kOctet; ++i) x[k][i] += shfl_xor(x[k][i], step);
+                tail += shfl_xor(tail, step);
+            }
+            const bool first = lane_id() < NT;
+            turn = first ? threadIdx.x / kWave : WAVES;
+            writes = first && turn == WAVES - 1;
+        }
+        if constexpr (FOLD > 1) {
             // the groups add to the columns' sums one after the other, in a fixed order
-            for (uint32_t g = 0; g < RG; ++g) {
-                if (group == g) {
+            for (uint32_t g = 0; g < FOLD; ++g) {
+                if (turn == g) {
 #pragma unroll
                     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -503,7 +564,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormGradArgs a)
                 __syncthreads();
             }
         }
-        if (group == RG - 1) {
+        if (writes) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
                 if (c.has(k)) store_pack<kOctet>(part + c.col(k), x[k]);
@@ -570,8 +631,9 @@ __global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(NormGr
     }
 }
 // Longer rows, dw and db: a workgroup takes 2048 columns of every gridDim.y-th
-// row.  It runs before ds is written, which may go where dy or s lies.
+// row.
 constexpr int kColThreads = 256;
+constexpr uint32_t kColGroups = 1024;  // workgroups that these partial sums are split over
 template <class T>
 __global__ __launch_bounds__(kColThreads) void norm_backward_cols_kernel(NormGradArgs a)
 {
@@ -639,22 +701,29 @@ uint64_t resident_groups(DeviceCache &cache, Kernel kernel, int threads)
 }
 
 // NT threads with K octets each for a row of `octets`: the smallest group of
-// waves that holds it.  f(NT, K) as integral constants; false if the row is longer.
+// waves that holds it.  f(NT, K) as integral constants; false if the row is longer
+// or f has no kernel of that shape.
+template <int NT, int K, class F>
+bool norm_shape_of(F f)
+{
+    return f(std::integral_constant<int, NT>{}, std::integral_constant<int, K>{});
+}
 template <class F>
 bool norm_shape(uint32_t octets, F f)
 {
-    using std::integral_constant;
-    if (octets <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (octets <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    else if (octets <= 192) f(integral_constant<int, 192>{}, integral_constant<int, 1>{});
-    else if (octets <= 256) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-    else if (octets <= 384) f(integral_constant<int, 384>{}, integral_constant<int, 1>{});
-    else if (octets <= 512) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
-    else if (octets <= 768) f(integral_constant<int, 768>{}, integral_constant<int, 1>{});
-    else if (octets <= 1024) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-    else if (octets <= 2048) f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-    else return false;
-    return true;
+    if (octets <= 16) return norm_shape_of<16, 1>(f);
+    if (octets <= 32) return norm_shape_of<32, 1>(f);
+    if (octets <= 64) return norm_shape_of<64, 1>(f);
+    if (octets <= 128) return norm_shape_of<64, 2>(f);
+    if (octets <= 192) return norm_shape_of<192, 1>(f);
+    if (octets <= 256) return norm_shape_of<256, 1>(f);
+    if (octets <= 384) return norm_shape_of<384, 1>(f);
+    if (octets <= 512) return norm_shape_of<512, 1>(f);
+    if (octets <= 768) return norm_shape_of<768, 1>(f);
+    if (octets <= 1024) return norm_shape_of<1024, 1>(f);
+    if (octets <= 2048) return norm_shape_of<512, 4>(f);
+    if (octets <= 4096) return norm_shape_of<1024, 4>(f);
+    return false;
 }
 
 template <class T, class W, bool ADD>
@@ -665,10 +734,16 @@ int norm_forward_launch(const NormArgs &a, hipStream_t s)
     const bool fits = norm_shape(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
         constexpr int THREADS = norm_threads(NT, 256);
-        static DeviceCache cache;
-        const uint64_t most = resident_groups(cache, norm_forward_kernel<T, W, NT, K, THREADS, ADD, K <= 2>, THREADS);
-        const uint32_t grid = (uint32_t)std::min<uint64_t>(ceil_div(a.rows, THREADS / NT), most);
-        LCPP_LAUNCH(name, s, norm_forward_kernel<T, W, NT, K, THREADS, ADD, K <= 2><<<grid, THREADS, 0, s>>>(a));
+        if constexpr (ADD && NT * K > 2048) {
+            return false;  // (the registers do not hold it: it would spill)
+        } else {
+            const auto kernel = norm_forward_kernel<T, W, NT, K, THREADS, ADD, K <= 2>;
+            static DeviceCache cache;
+            const uint32_t grid =
+                (uint32_t)std::min(ceil_div(a.rows, THREADS / NT), resident_groups(cache, kernel, THREADS));
+            LCPP_LAUNCH(name, s, kernel<<<grid, THREADS, 0, s>>>(a));
+            return true;
+        }
     });
     if (!fits)
         LCPP_LAUNCH(name, s,
@@ -692,22 +767,36 @@ int norm_backward_launch(const NormGradArgs &a, W *grad_weight, W *grad_bias, hi
     const uint32_t octets = a.cols / kOctet;
     const char *name = ADD ? "layer_norm_add_backward" : "layer_norm_backward";
     uint32_t parts = 0;
+    // rows whose columns' sums do not fit the registers: these are summed first (ds may go where dy or s lies)
+    auto columns = [&] {
+        if (!a.partial) return;
+        const uint32_t blocks = (uint32_t)ceil_div(a.cols, kColThreads * kOctet);
+        parts = (uint32_t)std::min<uint64_t>(ceil_div(a.rows, 8), std::min(std::max(kColGroups / blocks, 8u), (uint32_t)kMaxParts));
+        LCPP_LAUNCH("layer_norm_backward_cols", s,
+                    norm_backward_cols_kernel<T><<<dim3(blocks, parts), kColThreads, 0, s>>>(a));
+    };
     const bool fits = norm_shape(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
         constexpr int THREADS = norm_threads(NT, 512);
-        constexpr bool kAhead = K <= 2 && (NT < 1024 || sizeof(T) == 2 || !ADD);
-        static DeviceCache cache;
-        const uint64_t most = resident_groups(cache, norm_backward_kernel<T, W, NT, K, THREADS, ADD, kAhead>, THREADS);
-        parts = (uint32_t)std::min(ceil_div(a.rows, THREADS / NT), std::min(most, kMaxParts));
-        LCPP_LAUNCH(name, s, norm_backward_kernel<T, W, NT, K, THREADS, ADD, kAhead><<<parts, THREADS, 0, s>>>(a));
+        constexpr bool kAcc = NT * K <= 2048;
+        constexpr bool kAhead = K < 4 ? NT < 1024 || sizeof(T) == 2 || !ADD : kAcc && sizeof(T) == 2 && !ADD;
+        if constexpr (ADD && !kAcc) {
+            return false;  // (the registers do not hold it: it would spill)
+        } else {
+            const auto kernel = norm_backward_kernel<T, W, NT, K, THREADS, ADD, kAhead, kAcc>;
+            static DeviceCache cache;
+            uint32_t grid = (uint32_t)std::min(ceil_div(a.rows, THREADS / NT), resident_groups(cache, kernel, THREADS));
+            if (kAcc) parts = grid = std::min<uint32_t>(grid, kMaxParts);
+            else columns();
+            LCPP_LAUNCH(name, s, kernel<<<grid, THREADS, 0, s>>>(a));
+            return true;
+        }
     });
     if (!fits) {
-        if (a.partial) {
-            parts = (uint32_t)std::min<uint64_t>(norm_parts(a.rows), 128);
-            const dim3 grid((uint32_t)ceil_div(a.cols, kColThreads * kOctet), parts);
-            LCPP_LAUNCH("layer_norm_backward_cols", s, norm_backward_cols_kernel<T><<<grid, kColThreads, 0, s>>>(a));
-        }
-        LCPP_LAUNCH(name, s, norm_backward_long_kernel<T, W, ADD><<<(uint32_t)std::min<uint64_t>(a.rows, kMaxGroups), kLongThreads, 0, s>>>(a));
+        columns();
+        LCPP_LAUNCH(name, s,
+                    norm_backward_long_kernel<T, W, ADD>
+                    <<<(uint32_t)std::min<uint64_t>(a.rows, kMaxGroups), kLongThreads, 0, s>>>(a));
     }
     if (a.partial)
         LCPP_LAUNCH("layer_norm_fold", s,

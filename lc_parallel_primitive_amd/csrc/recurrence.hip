@@ -54,6 +54,7 @@ struct RecArgs {
     const uint32_t *begin, *end;           // null: sequence s begins at its stride, with max_length rows
     uint64_t rows;                         // with begin and end: rows of the tensors
     uint32_t sequences, tiles, groups, channels, max_length;
+    uint32_t run, turns;                   // chains of a run (0: no runs); workgroups of a tile of time
     uint64_t *words;                       // [sequence][tile of the walk][group][lane's channels]
     WaitCtl ctl;
 };
@@ -92,26 +93,38 @@ struct GateSigmoid {
 // as long as there are C channels.
 struct Place {
     uint32_t seq, tile, len, channel, group;
-    uint32_t walk;  // tiles of the sequence before this one in the walk
+    uint32_t walk;    // tiles of the sequence before this one in the walk
+    uint32_t number;  // of the tile among all, for the test hook
     bool active;
     uint64_t row;  // of the tensors' rows that the sequence begins at (with offsets)
 };
 // Workgroups are numbered tile by tile, so a tile waits only on workgroups
 // dispatched before its own; `reverse` counts tiles from the sequence's end.
-// Within a tile of time the chains (a sequence's group of channels) are dealt so
-// that each XCD, which gets every eighth workgroup, has neighbours: where rows do
-// not begin at a line of memory, neighbouring groups share lines, and their parts
-// meet in one L2 (8 x 4096 x 2049 bfloat16, forward and backward: 145 + 263 us
-// dealt in turn, 117 + 214 dealt in runs; of 2048 channels 92 + 151 and 87 + 145).
+//
+// Within a tile of time the chains (a sequence's groups of channels, one behind
+// the other) are cut into runs, and each of the eight XCDs, which get the
+// workgroups in turn, works on whole runs: where rows do not begin at a line of
+// memory, neighbouring groups share lines, and their parts meet in one L2.  The
+// runs go to another XCD at every tile.  Measured (us, forward + backward): 8 x
+// 4096 x 2049 bfloat16 145 + 263 with runs of one chain, 102 + 162 with an eighth
+// of all; 1 x 65536 x 2048 forward 186 with the runs on one XCD at all tiles, 163
+// in turn.  Sequences of different lengths have short runs, or the last one at
+// work would leave XCDs idle (24 packed x 1536 channels: 142 with an eighth of
+// all chains, 108 with runs of 4).  Numbers past the last chain are left at once.
+constexpr uint32_t kXcds = 8;
 template <int C>
 __device__ __forceinline__ bool find_place(const RecArgs &a, bool reverse, Place &p)
 {
-    constexpr uint32_t kXcds = 8;
-    const uint32_t chains = a.groups * a.sequences, k = blockIdx.x / chains;
-    const uint32_t turn = blockIdx.x - k * chains, xcd = turn % kXcds, rest = chains % kXcds;
-    const uint32_t chain = xcd * (chains / kXcds) + (xcd < rest ? xcd : rest) + turn / kXcds;
+    const uint32_t k = blockIdx.x / a.turns, turn = blockIdx.x - k * a.turns;
+    uint32_t chain = turn;
+    if (a.run) {
+        const uint32_t y = turn / kXcds;
+        chain = (y / a.run * kXcds + (turn + k) % kXcds) * a.run + y % a.run;
+    }
     p.seq = chain / a.groups;
     p.group = chain - p.seq * a.groups;
+    if (p.seq >= a.sequences) return false;
+    p.number = (k * a.sequences + p.seq) * a.groups + p.group;
     p.row = 0;
     p.len = a.max_length;
     if (a.begin) {
@@ -224,10 +237,10 @@ __device__ __forceinline__ void publish_state(uint64_t *words, const Chan<C> &A,
 }
 
 // Rows that begin at a line of memory (STREAM) are read and written with the
-// streaming policy: 8 x 4096 x 2048 bfloat16 87 + 145 us, without it 95 + 152.
-// Where neighbouring groups share lines these are better kept in the L2: of 2049
-// channels 117 + 214 us with the policy, 103 + 164 without it (for the forward
-// pass's loads it is the same, and better with fewer channels).
+// streaming policy: 8 x 4096 x 2048 bfloat16 87 + 145 us, without it 95 + 152; 4 x
+// 512 x 1024 10.5 + 15.0 and 10.8 + 15.5.  Where neighbouring groups share lines
+// these are better kept in the L2: of 2049 channels 117 + 214 us with the policy,
+// 102 + 162 without it.
 template <bool STREAM, int N, class T>
 __device__ __forceinline__ Pack<T, N> load_rows_of(const T *p)
 {
@@ -292,7 +305,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
     s_H[wave][lane] = H;
     __syncthreads();
     if (wave == 0) {
-        const bool publish = more && blockIdx.x != a.ctl.withhold;
+        const bool publish = more && p.number != a.ctl.withhold;
         if (publish) {
 #pragma unroll
             for (int w = 1; w < W; ++w)
@@ -409,7 +422,7 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     s_E[wave][lane] = E;
     __syncthreads();
     if (wave == 0) {
-        const bool publish = p.tile > 0 && blockIdx.x != a.ctl.withhold;
+        const bool publish = p.tile > 0 && p.number != a.ctl.withhold;
         if (publish) {
             A = s_A[W - 1][lane], E = s_E[W - 1][lane];
 #pragma unroll
@@ -536,9 +549,16 @@ int gate_dispatch(lcpp_gate g, F f)
 // 64 lanes cover the channels.
 uint32_t rec_lane_channels(uint64_t channels, size_t size) { return channels <= kWave || size == 4 ? 1 : 2; }
 struct RecShape {
-    uint64_t tiles, groups, words;
+    uint64_t tiles, groups, words, run, turns;
 };
-bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t size, RecShape *r)
+void rec_dealing(uint64_t sequences, bool offsets, RecShape *r)
+{
+    const uint64_t chains = sequences * r->groups;
+    r->run = chains < kXcds ? 0 : ceil_div(chains, kXcds);
+    if (offsets) r->run = std::min<uint64_t>(r->run, 4);
+    r->turns = r->run ? align_up(ceil_div(chains, r->run), kXcds) * r->run : chains;
+}
+bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t size, bool offsets, RecShape *r)
 {
     if (sequences > 0xFFFFFFFFull || max_length > 0x7FFFFFFFull || channels > kMaxCols) return false;
     const uint64_t lanes = kWave * rec_lane_channels(channels, size);
@@ -546,7 +566,9 @@ bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, size_
     r->tiles = std::max<uint64_t>(ceil_div(max_length, kTileRows), 1);
     // workgroups are numbered in 32 bits, and a launch has less than 2^32 threads
     const uint64_t most = 0xFFFFFFFFull / (kWaves * kWave);
-    if (r->groups && (r->tiles > most / r->groups || sequences > most / (r->groups * r->tiles))) return false;
+    if (r->groups && sequences > most / r->groups) return false;
+    rec_dealing(sequences, offsets, r);
+    if (r->turns && r->tiles > most / r->turns) return false;
     r->words = r->tiles > 1 ? sequences * r->tiles * r->groups * lanes : 0;
     return true;
 }
@@ -558,7 +580,7 @@ uint64_t rec_temp_bytes(const RecShape &r)
 template <class T, class G, int C, int W, bool STREAM>
 int rec_launch_waves(bool forward, const RecArgs &a, hipStream_t s)
 {
-    const uint32_t grid = a.sequences * a.tiles * a.groups;
+    const uint32_t grid = a.tiles * a.turns;
     if (forward) LCPP_LAUNCH("recurrence_forward", s, rec_forward_kernel<T, G, C, W, STREAM><<<grid, W * kWave, 0, s>>>(a));
     else LCPP_LAUNCH("recurrence_backward", s, rec_backward_kernel<T, G, C, W, STREAM><<<grid, W * kWave, 0, s>>>(a));
     LCPP_CHECK_LAUNCH();
@@ -589,7 +611,7 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
     if (!e) return LCPP_ERR_UNSUPPORTED_DTYPE;
     if (g != LCPP_GATE_DECAY && g != LCPP_GATE_LOG && g != LCPP_GATE_SIGMOID) return LCPP_ERR_INVALID_ARG;
     RecShape r;
-    if (!rec_shape(sequences, max_length, channels, e, &r) || (!a.begin) != (!a.end)) return LCPP_ERR_INVALID_ARG;
+    if (!rec_shape(sequences, max_length, channels, e, a.begin != nullptr, &r) || (!a.begin) != (!a.end)) return LCPP_ERR_INVALID_ARG;
     if (sequences == 0 || channels == 0) return LCPP_OK;
     if (a.begin && (!elem_ok(a.begin, 4) || !elem_ok(a.end, 4))) return LCPP_ERR_INVALID_ARG;
     auto optional = [](const void *p) { return !p || elem_ok(p, 4); };
@@ -611,6 +633,7 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
         if (temp_bytes < rec_temp_bytes(r)) return LCPP_ERR_TEMP_TOO_SMALL;
         if (!temp || (reinterpret_cast<uintptr_t>(temp) & 255)) return LCPP_ERR_INVALID_ARG;
     }
+    a.run = (uint32_t)r.run, a.turns = (uint32_t)r.turns;
     a.sequences = (uint32_t)sequences, a.tiles = (uint32_t)r.tiles, a.groups = (uint32_t)r.groups;
     a.channels = (uint32_t)channels, a.max_length = some ? (uint32_t)max_length : 0, a.rows = rows;
     if (a.begin) a.gate.seq = a.in.seq = a.grad_out.seq = a.out.seq = a.grad_gate.seq = a.grad_in.seq = 0;
@@ -643,9 +666,9 @@ using namespace lcpp;
 extern "C" int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes)
 {
     RecShape r;
-    if (!bytes || !rec_shape(sequences, max_length, channels, 2, &r)) return LCPP_ERR_INVALID_ARG;
+    if (!bytes || !rec_shape(sequences, max_length, channels, 2, false, &r)) return LCPP_ERR_INVALID_ARG;
     *bytes = rec_temp_bytes(r);
-    if (!rec_shape(sequences, max_length, channels, 4, &r)) return LCPP_ERR_INVALID_ARG;
+    if (!rec_shape(sequences, max_length, channels, 4, false, &r)) return LCPP_ERR_INVALID_ARG;
     *bytes = std::max<size_t>(*bytes, rec_temp_bytes(r));  // for every type
     return LCPP_OK;
 }

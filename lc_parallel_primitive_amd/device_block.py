@@ -67,6 +67,17 @@ def _like_out(t, shape, dtype, what: str):
     return stride
 
 
+def _in_out(x, y, in_name: str = "d_in", out_name: str = "d_out"):
+    """(shape, dtype, lcpp_dtype, rows, columns, row strides) of an input and an output of its shape and type."""
+    shape, dtype, sx, sy = x.shape, x.dtype, x.stride(), y.stride()
+    code = _float_codes.get(dtype)
+    if code and len(sx) == 2 and sx[1] == sy[-1] == 1 and y.dtype == dtype and y.shape == shape and sy[0] >= shape[1]:
+        return shape, dtype, code, shape[0], shape[1], sx[0], sy[0]
+    code = float_code(dtype)
+    _, rows, cols, si = _matrix(x, in_name)
+    return shape, dtype, code, rows, cols, si, _like_out(y, shape, dtype, out_name)
+
+
 def _vector(t, n: int, what: str):
     """The address of a contiguous tensor of at least n values, or None."""
     if t is None:
@@ -90,15 +101,15 @@ def _weight_code(code: int, *weights):
     """The lcpp_dtype of the weights that are given: the activations' or float32."""
     first = None
     for w in weights:
-        if w is None:
-            continue
-        if first is None:
-            first = w.dtype
-        elif w.dtype != first:
-            raise TypeError("weight, bias and their gradients must have one dtype")
+        if w is not None:
+            dtype = w.dtype
+            if first is None:
+                first = dtype
+            elif dtype != first:
+                raise TypeError("weight, bias and their gradients must have one dtype")
     if first is None:
         return code
-    wt = float_code(first)
+    wt = _float_codes.get(first) or float_code(first)
     if wt != code and wt != 2:
         raise TypeError("weights must have the activations' dtype or float32")
     return wt
@@ -136,10 +147,7 @@ class DeviceLayerNorm(_BlockModule):
 
     def Forward(self, d_in, d_out, d_weight=None, d_bias=None, eps: float = 1e-5, d_mean=None, d_rstd=None, stream=None):
         """d_out = the layer norm of d_in; d_mean, d_rstd: float32 row statistics for Backward, or None."""
-        dtype = d_in.dtype
-        code = float_code(dtype)
-        shape, rows, cols, si = _matrix(d_in, "d_in")
-        so = _like_out(d_out, shape, dtype, "d_out")
+        _, _, code, rows, cols, si, so = _in_out(d_in, d_out)
         self._call("lcpp_layer_norm_forward", None, _stream(stream), code, _weight_code(code, d_weight, d_bias),
                    d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"), _vector(d_bias, cols, "d_bias"), eps,
                    d_out.data_ptr(), so, _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), rows,
@@ -163,10 +171,8 @@ class DeviceLayerNorm(_BlockModule):
     def Backward(self, temp_storage, d_grad_out, d_in, d_weight, d_mean, d_rstd, d_grad_in, d_grad_weight=None,
                  d_grad_bias=None, stream=None):
         """The gradients of Forward's d_in, d_weight and d_bias (the latter two None if not wanted)."""
-        dtype = d_in.dtype
-        code = float_code(dtype)
-        shape, rows, cols, si = _matrix(d_in, "d_in")
-        sg, so = _like(d_grad_out, shape, dtype, "d_grad_out"), _like_out(d_grad_in, shape, dtype, "d_grad_in")
+        shape, dtype, code, rows, cols, si, so = _in_out(d_in, d_grad_in, "d_in", "d_grad_in")
+        sg = _like(d_grad_out, shape, dtype, "d_grad_out")
         self._call("lcpp_layer_norm_backward", temp_storage, _stream(stream), code,
                    _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
                    d_grad_out.data_ptr(), sg, d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
@@ -202,11 +208,9 @@ class DeviceDropout(_BlockModule):
         """d_out = (kept ? d_in / (1 - p) : 0) [+ d_residual].  p is met to 2^-17.  offset tells the calls of one seed
         apart (a layer's number, a step's); d_offset, a device tensor of one 64-bit integer, is added to it when the
         kernel runs, so a captured graph's replays can differ."""
-        dtype = d_in.dtype
-        shape, rows, cols, si = _matrix(d_in, "d_in")
-        so = _like_out(d_out, shape, dtype, "d_out")
+        shape, dtype, code, rows, cols, si, so = _in_out(d_in, d_out)
         sr = 0 if d_residual is None else _like(d_residual, shape, dtype, "d_residual")
-        self._call("lcpp_dropout", None, _stream(stream), float_code(dtype), d_in.data_ptr(), si, _ptr(d_residual), sr,
+        self._call("lcpp_dropout", None, _stream(stream), code, d_in.data_ptr(), si, _ptr(d_residual), sr,
                    d_out.data_ptr(), so, rows, cols, p, seed & _U64, offset & _U64, _counter(d_offset, "d_offset"))
 
     def Backward(self, d_grad_out, d_grad_in, p: float, seed: int, offset: int = 0, d_offset=None, stream=None):
@@ -323,21 +327,21 @@ class DeviceGatedRecurrence(_BlockModule):
         """One token for each of some sequences: d_gate, d_in and d_out of shape (sequences, channels).  The states are
         float32 of shape (slots, channels); d_state_out may be d_state_in.  d_slots: int32, the row of each sequence's
         state, all different; -1 marks padding (out is 0, no state changes).  None: row s for sequence s."""
-        kind, dtype = self._gate(gate), d_in.dtype
-        shape, rows, cols, sx = _matrix(d_in, "d_in")
+        shape, dtype, code, rows, cols, sx, so = _in_out(d_in, d_out)
         if len(shape) != 2:
             raise ValueError("d_in: shape (sequences, channels)")
-        sg, so = _like(d_gate, shape, dtype, "d_gate"), _like_out(d_out, shape, dtype, "d_out")
+        sg = _like(d_gate, shape, dtype, "d_gate")
         pool = d_state_in.shape
-        if len(pool) != 2 or pool[1] != cols or d_state_out.shape != pool:
+        if len(pool) != 2 or pool[1] != cols or (d_state_out is not d_state_in and d_state_out.shape != pool):
             raise ValueError(f"states: shapes {tuple(pool)} and {tuple(d_state_out.shape)}, expected (slots, {cols})")
         slots = pool[0]
+        state = _float_vector(d_state_in, 0, "d_state_in")
         if d_slots is not None:
             if d_slots.element_size() != 4 or d_slots.is_floating_point():
                 raise TypeError("d_slots: must be int32")
         elif slots < rows:
             raise ValueError(f"states: {slots} rows for {rows} sequences")
-        self._call("lcpp_recurrence_step", None, _stream(stream), float_code(dtype), kind, d_gate.data_ptr(), sg,
-                   d_in.data_ptr(), sx, _float_vector(d_state_in, 0, "d_state_in"),
-                   _float_vector(d_state_out, 0, "d_state_out"), _vector(d_slots, rows, "d_slots"), slots, d_out.data_ptr(),
-                   so, rows, cols)
+        self._call("lcpp_recurrence_step", None, _stream(stream), code, self._gate(gate), d_gate.data_ptr(), sg,
+                   d_in.data_ptr(), sx, state,
+                   state if d_state_out is d_state_in else _float_vector(d_state_out, 0, "d_state_out"),
+                   _vector(d_slots, rows, "d_slots"), slots, d_out.data_ptr(), so, rows, cols)
