@@ -402,7 +402,7 @@ int lcpp_layer_norm_add_backward(lcpp_dtype t, lcpp_dtype wt, void *temp, size_t
  * 4x32 with 7 rounds, counter (c / 8, row, offset, offset >> 32), key (seed, seed >> 32), c the
  * column.  No mask is stored: the backward pass is the same call on the gradient, without the
  * residual.  offset_dev: a device counter added to offset when the kernel runs (a captured graph
- * can advance it between replays), or NULL.  0 <= p <= 1. */
+ * can advance it between replays; 8-byte aligned), or NULL.  0 <= p <= 1. */
 int lcpp_dropout(lcpp_dtype t, const void *in, uint64_t in_stride, const void *residual, uint64_t residual_stride,
                  void *out, uint64_t out_stride, uint64_t rows, uint64_t cols, double p, uint64_t seed,
                  uint64_t offset, const uint64_t *offset_dev, void *stream);
@@ -414,7 +414,9 @@ int lcpp_dropout(lcpp_dtype t, const void *in, uint64_t in_stride, const void *r
  * begin and cut at max_length, which sizes the launch; rows of no sequence are left alone.
  * initial (NULL: 0), final_state: the states before the first and after the last row, float32
  * [sequences][channels]; an empty sequence's final state is its initial one.  checkpoints: what
- * the backward pass needs, float32 [sequences][lcpp_recurrence_checkpoint_rows][channels], or NULL. */
+ * the backward pass needs, float32 [sequences][lcpp_recurrence_checkpoint_rows][channels], or NULL.
+ * A call covers fewer than 2^23 tiles of 128 rows and 128 channels (64 of float32), sequences of
+ * max_length each; max_length < 2^31. */
 int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes);
 int lcpp_recurrence_checkpoint_rows(uint64_t max_length, uint64_t *rows);
 int lcpp_recurrence_forward(lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, const void *gate,

@@ -87,15 +87,19 @@ struct GateSigmoid {
 };
 
 // ---------------------------------------------------------------- tiles
-// Where a workgroup's lanes work.  A lane has C channels; the last lanes of a
-// last group are moved back so that they lie inside the row, and compute and
-// store what their neighbours do (the same values).  Every access is in bounds
-// as long as there are C channels.
+// Where a workgroup's lanes work.  A lane has C channels; the last lane of an odd
+// number of channels is moved back by one so that its channels lie inside the row,
+// and computes and stores one of its neighbour's too, from the same loads: the
+// same value.  Only where that neighbour is in another workgroup (`single`: the
+// wave's one channel) is the other channel not stored, since an output over an
+// input may already have been written there.  Every access is in bounds as long
+// as there are C channels.
 struct Place {
     uint32_t seq, tile, len, channel, group;
     uint32_t walk;    // tiles of the sequence before this one in the walk
     uint32_t number;  // of the tile among all, for the test hook
-    bool active;
+    bool active;   // the lane has a channel
+    bool single;   // the first lane has one channel, the others none
     uint64_t row;  // of the tensors' rows that the sequence begins at (with offsets)
 };
 // Workgroups are numbered tile by tile, so a tile waits only on workgroups
@@ -141,6 +145,7 @@ __device__ __forceinline__ bool find_place(const RecArgs &a, bool reverse, Place
     const uint32_t c = p.group * (kWave * C) + lane_id() * C;
     p.active = c < a.channels;
     p.channel = c + C <= a.channels ? c : a.channels - C;
+    p.single = C > 1 && p.group > 0 && a.channels - p.group * (kWave * C) == 1;
     return true;
 }
 // (the wave's number as a scalar, so that row addresses are scalars too and a
@@ -152,6 +157,13 @@ __device__ __forceinline__ const T *row_in(const RowsIn &t, const Place &p, uint
     return static_cast<const T *>(t.p) + ((p.row + row) * t.row + p.seq * t.seq);
 }
 
+// A lane's address in a row: a scalar and a 32-bit offset.
+template <class T>
+__device__ __forceinline__ T *lane_at(T *row, uint32_t channel)
+{
+    using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+    return reinterpret_cast<T *>(reinterpret_cast<Byte *>(row) + (uint32_t)(channel * sizeof(T)));
+}
 template <class T>
 __device__ __forceinline__ T *row_out(const RowsOut &t, const Place &p, uint64_t row)
 {
@@ -253,11 +265,32 @@ __device__ __forceinline__ void store_rows_of(T *p, const float (&x)[N])
     if constexpr (STREAM) store_pack_nt<N>(p, x);
     else store_pack<N>(p, x);
 }
-
-template <class T, int C>
-__device__ __forceinline__ void store_chan(T *p, const Chan<C> &x)
+// A lane's channels of a row or of a state, at the row's first channel.
+template <bool STREAM, bool SINGLE, int C, class T>
+__device__ __forceinline__ void store_own(T *row, const Place &p, const float (&x)[C])
 {
-    store_pack<C>(p, x.v);
+    if constexpr (SINGLE) *lane_at(row, p.channel + C - 1) = (T)x[C - 1];
+    else store_rows_of<STREAM, C>(lane_at(row, p.channel), x);
+}
+template <int C>
+__device__ __forceinline__ void store_state(float *row, const Place &p, const Chan<C> &x)
+{
+    if (p.single) store_own<false, true>(row, p, x.v);
+    else store_own<false, false>(row, p, x.v);
+}
+// f with whether the wave has a single channel as a constant: the loops over rows
+// are made for either (a branch in them costs 5 % at 8 x 4096 x 2048).  Streamed
+// rows have no odd channel.
+template <bool STREAM, int C, class F>
+__device__ __forceinline__ void with_single(const Place &p, F f)
+{
+    if constexpr (C > 1 && !STREAM) {
+        if (p.single) {
+            f(std::true_type{});
+            return;
+        }
+    }
+    f(std::false_type{});
 }
 
 template <class T, class G, int C, int W, bool STREAM>
@@ -267,7 +300,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
     Place p;
     if (!find_place<C>(a, false, p)) return;
     const uint32_t wave = wave_id(), lane = lane_id();
-    const uint64_t state_at = (uint64_t)p.seq * a.channels + p.channel;
+    const uint64_t state_row = (uint64_t)p.seq * a.channels, state_at = state_row + p.channel;
     const uint32_t first = p.tile * kTileRows + wave * kRows;
     const uint32_t last = p.len ? p.len - 1 : 0;
     const bool more = ((uint64_t)p.tile + 1) * kTileRows < p.len;  // a tile follows
@@ -278,11 +311,14 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
     {
         Pack<T, C> gr[kRows], xr[kRows];
         if (p.len) {
+            const T *g = row_in<T>(a.gate, p, first < last ? first : last), *x = row_in<T>(a.in, p, first < last ? first : last);
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
-                const uint64_t t = first + r < last ? first + r : last;  // (rows past the end are not used)
-                gr[r] = load_rows_of<STREAM, C>(row_in<T>(a.gate, p, t) + p.channel);
-                xr[r] = load_rows_of<STREAM, C>(row_in<T>(a.in, p, t) + p.channel);
+                gr[r] = load_rows_of<STREAM, C>(lane_at(g, p.channel));
+                xr[r] = load_rows_of<STREAM, C>(lane_at(x, p.channel));
+                const bool next = first + r < last;  // (rows past the end read the last one and are not used)
+                g += next ? a.gate.row : 0;
+                x += next ? a.in.row : 0;
             }
         }
 #pragma unroll
@@ -327,8 +363,8 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
         if (publish) publish_state<C>(words, A, H, h);
         if (p.active) {
             if (a.checkpoints && p.len)
-                store_chan(a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels + p.channel, h);
-            if (a.final_state && !p.len) store_chan(a.final_state + state_at, h);
+                store_state(a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels, p, h);
+            if (a.final_state && !p.len) store_state(a.final_state + state_row, p, h);
         }
     }
     __syncthreads();
@@ -336,15 +372,18 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
     for (uint32_t w = 0; w < wave; ++w)
 #pragma unroll
         for (int c = 0; c < C; ++c) h.v[c] = s_A[w][lane].v[c] * h.v[c] + s_H[w][lane].v[c];
+    with_single<STREAM, C>(p, [&](auto single) {
+        T *y = row_out<T>(a.out, p, first);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+        for (int r = 0; r < kRows; ++r, y += a.out.row) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) h.v[c] = ga[r].v[c] * h.v[c] + gb[r].v[c];
-        if (first + r < p.len && p.active) store_rows_of<STREAM, C>(row_out<T>(a.out, p, first + r) + p.channel, h.v);
-    }
+            for (int c = 0; c < C; ++c) h.v[c] = ga[r].v[c] * h.v[c] + gb[r].v[c];
+            if (first + r < p.len && p.active) store_own<STREAM, decltype(single)::value>(y, p, h.v);
+        }
+    });
     // (rows past the end left h as it was)
     if (a.final_state && p.active && p.len && first <= last && last - first < kRows)
-        store_chan(a.final_state + state_at, h);
+        store_state(a.final_state + state_row, p, h);
 }
 
 // Makes the compiler forget where a value came from: what is computed from it
@@ -377,12 +416,13 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     Place p;
     if (!find_place<C>(a, true, p)) return;
     const uint32_t wave = wave_id(), lane = lane_id();
-    const uint64_t state_at = (uint64_t)p.seq * a.channels + p.channel;
+    const uint64_t state_row = (uint64_t)p.seq * a.channels, state_at = state_row + p.channel;
     if (p.len == 0) {  // nothing lies between the final and the initial state
         if (wave == 0 && a.grad_initial && p.active) {
+            Chan<C> v;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-                a.grad_initial[state_at + c] = a.grad_final ? a.grad_final[state_at + c] : 0.0f;
+            for (int c = 0; c < C; ++c) v.v[c] = a.grad_final ? a.grad_final[state_at + c] : 0.0f;
+            store_state(a.grad_initial + state_row, p, v);
         }
         return;
     }
@@ -392,12 +432,19 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.walk) * tile_words + (uint64_t)p.group * kWave * C + lane * C;
 
     Pack<T, C> gr[kRows], xr[kRows], dyr[kRows];
+    {
+        const uint32_t t = first < last ? first : last;
+        const T *g = row_in<T>(a.gate, p, t), *x = row_in<T>(a.in, p, t), *dy = row_in<T>(a.grad_out, p, t);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-        const uint64_t t = first + r < last ? first + r : last;  // (rows past the end are not used)
-        gr[r] = load_rows_of<STREAM, C>(row_in<T>(a.gate, p, t) + p.channel);
-        xr[r] = load_rows_of<STREAM, C>(row_in<T>(a.in, p, t) + p.channel);
-        dyr[r] = load_rows_of<STREAM, C>(row_in<T>(a.grad_out, p, t) + p.channel);
+        for (int r = 0; r < kRows; ++r) {
+            gr[r] = load_rows_of<STREAM, C>(lane_at(g, p.channel));
+            xr[r] = load_rows_of<STREAM, C>(lane_at(x, p.channel));
+            dyr[r] = load_rows_of<STREAM, C>(lane_at(dy, p.channel));
+            const bool next = first + r < last;  // (rows past the end read the last one and are not used)
+            g += next ? a.gate.row : 0;
+            x += next ? a.in.row : 0;
+            dy += next ? a.grad_out.row : 0;
+        }
     }
     // the wave's rows as one map, forward (A, H) and backward (A, E)
     Chan<C> A, H, E;
@@ -470,27 +517,30 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
             h.v[c] = al * h.v[c] + (G::kShare ? share * xr[r][c] : xr[r][c]);
         }
     }
+    with_single<STREAM, C>(p, [&](auto single) {
+        T *pg = row_out<T>(a.grad_gate, p, first + kRows - 1), *px = row_out<T>(a.grad_in, p, first + kRows - 1);
 #pragma unroll
-    for (int r = kRows - 1; r >= 0; --r) {
-        forget(gr[r]);
-        if (first + r < p.len) {
-            float dg[C], dx[C];
+        for (int r = kRows - 1; r >= 0; --r, pg -= a.grad_gate.row, px -= a.grad_in.row) {
+            forget(gr[r]);
+            if (first + r < p.len) {
+                float dg[C], dx[C];
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float al, share;
-                G::eval(gr[r][c], al, share);
-                const float dh = dyr[r][c] + e.v[c];
-                dg[c] = G::grad(dh, before[r].v[c], xr[r][c], al, share);
-                dx[c] = G::kShare ? dh * share : dh;
-                e.v[c] = al * dh;
-            }
-            if (p.active) {
-                store_rows_of<STREAM, C>(row_out<T>(a.grad_gate, p, first + r) + p.channel, dg);
-                store_rows_of<STREAM, C>(row_out<T>(a.grad_in, p, first + r) + p.channel, dx);
+                for (int c = 0; c < C; ++c) {
+                    float al, share;
+                    G::eval(gr[r][c], al, share);
+                    const float dh = dyr[r][c] + e.v[c];
+                    dg[c] = G::grad(dh, before[r].v[c], xr[r][c], al, share);
+                    dx[c] = G::kShare ? dh * share : dh;
+                    e.v[c] = al * dh;
+                }
+                if (p.active) {
+                    store_own<STREAM, decltype(single)::value>(pg, p, dg);
+                    store_own<STREAM, decltype(single)::value>(px, p, dx);
+                }
             }
         }
-    }
-    if (p.tile == 0 && wave == 0 && a.grad_initial && p.active) store_chan(a.grad_initial + state_at, e);
+    });
+    if (p.tile == 0 && wave == 0 && a.grad_initial && p.active) store_state(a.grad_initial + state_row, p, e);
 }
 
 // One token for each of some sequences: h = a h + b on the states of a pool, at
@@ -599,7 +649,7 @@ int rec_launch(bool forward, const RecArgs &a, hipStream_t s)
     auto in = [&](const RowsIn &t) { return lined(t.p, t.row, t.seq); };
     auto out = [&](const RowsOut &t) { return lined(t.p, t.row, t.seq); };
     // (sequences with offsets begin at whole rows; the tensors that a pass does not have are null)
-    if (in(a.gate) && in(a.in) && in(a.grad_out) && out(a.out) && out(a.grad_gate) && out(a.grad_in))
+    if (a.channels % C == 0 && in(a.gate) && in(a.in) && in(a.grad_out) && out(a.out) && out(a.grad_gate) && out(a.grad_in))
         return rec_launch_waves<T, G, C, kWaves, true>(forward, a, s);
     return rec_launch_waves<T, G, C, kWaves, false>(forward, a, s);
 }

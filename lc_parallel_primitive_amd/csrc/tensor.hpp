@@ -161,10 +161,10 @@ __device__ __forceinline__ void drop_octet(float (&x)[kOctet], uint32_t row, uin
     }
 }
 
-// Host: the kernel's arguments for a probability; false where p is not in [0, 1].
+// Host: the kernel's arguments for a probability; false where p is not in [0, 1] or the counter is misaligned.
 inline bool drop_args(double p, uint64_t seed, uint64_t offset, const uint64_t *offset_dev, DropArgs *d)
 {
-    if (!(p >= 0.0 && p <= 1.0)) return false;
+    if (!(p >= 0.0 && p <= 1.0) || reinterpret_cast<uintptr_t>(offset_dev) % 8) return false;
     d->cut = (uint32_t)(p * 65536.0 + 0.5);
     d->scale = d->cut < 65536u ? (float)(65536.0 / (65536.0 - (double)d->cut)) : 0.0f;
     d->seed = seed;

@@ -251,6 +251,29 @@ def test_in_place_and_repeated(lcpp):
     assert int(temp[:4].view(torch.int32)[0]) == 0  # the status word
 
 
+@pytest.mark.parametrize("channels", [129, 257, 1025, 2049])
+def test_in_place_with_an_odd_channel(lcpp, channels):
+    """The last channel's lane reads its neighbour's channel too, which another workgroup may already have written."""
+    log(f"recurrence in place, {channels} channels")
+    g = gen(channels)
+    n, t, kind = 6, 400, "log"
+    gt, x, dy = (gates(g, kind, (n, t, channels), "bfloat16"), ref.rows(g, (n, t, channels), "bfloat16"),
+                 ref.rows(g, (n, t, channels), "bfloat16"))
+    h0, dhT = torch.randn(n, channels, generator=g).cuda(), torch.randn(n, channels, generator=g).cuda()
+    y, dg, dx, hT, dh0 = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x), torch.empty_like(h0), torch.empty_like(h0)
+    m = lcpp.DeviceGatedRecurrence()
+    temp, saved = temp_for(lcpp, n, t, channels), saved_for(lcpp, n, t, channels)
+    m.Forward(temp, gt, x, y, kind, h0, hT, saved)
+    m.Backward(temp, gt, x, saved, dy, dg, dx, kind, dhT, dh0)
+    for _ in range(3):
+        over, state = x.clone(), h0.clone()
+        m.Forward(temp, gt, over, over, kind, state, state, saved)
+        assert torch.equal(over, y) and torch.equal(state, hT)
+        og, od, back = gt.clone(), dy.clone(), dhT.clone()
+        m.Backward(temp, og, x, saved, od, og, od, kind, back, back)
+        assert torch.equal(og, dg) and torch.equal(od, dx) and torch.equal(back, dh0)
+
+
 @pytest.mark.parametrize("kind", ["decay", "log", "sigmoid"])
 def test_gradient_against_differences(lcpp, kind):
     """dL along random directions, L = sum(y c) + sum(hT d).  h depends on a gate as a polynomial or exponential of it:
