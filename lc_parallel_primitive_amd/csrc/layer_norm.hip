@@ -687,9 +687,9 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void norm_fold_kernel(const floa
 constexpr uint64_t kMaxGroups = 1u << 20;
 // Threads of a workgroup whose rows take nt each: as many rows as fit `atleast`.
 constexpr int norm_threads(int nt, int atleast) { return nt >= atleast ? nt : atleast / nt * nt; }
-// Workgroups that the device holds at once, which all get the same number of rows
-// (with one too many per CU the last ones run alone: 16384 x 4096 bfloat16 with
-// four workgroups per CU where three are resident 64 us, with three ...).
+// Workgroups that the device holds at once: all get the same number of rows, give
+// or take one (one more per CU than is resident would run alone in the end: 16384
+// x 4096 bfloat16 forward 64 -> 60 us).
 template <class Kernel>
 uint64_t resident_groups(DeviceCache &cache, Kernel kernel, int threads)
 {
@@ -702,13 +702,18 @@ uint64_t resident_groups(DeviceCache &cache, Kernel kernel, int threads)
 
 // NT threads with K octets each for a row of `octets`: the smallest group of
 // waves that holds it.  f(NT, K) as integral constants; false if the row is longer
-// or f has no kernel of that shape.
+// or f has no kernel of that shape.  PER: octets of a thread in rows of several
+// waves.  Two are better for the forward pass of 2-byte types, one for 4-byte
+// types and for the backward pass, which keeps sums for each (us, one -> two:
+// forward of 16384 x 4096 bfloat16 59 -> 51, 8000 x 7000 64 -> 47, 2000 x 4096
+// float32 13 -> 15; backward of 1777 x 5001 float16 with the sum 25 -> 27, 8000 x
+// 7000 114 -> 123).
 template <int NT, int K, class F>
 bool norm_shape_of(F f)
 {
     return f(std::integral_constant<int, NT>{}, std::integral_constant<int, K>{});
 }
-template <class F>
+template <int PER, class F>
 bool norm_shape(uint32_t octets, F f)
 {
     if (octets <= 16) return norm_shape_of<16, 1>(f);
@@ -716,11 +721,11 @@ bool norm_shape(uint32_t octets, F f)
     if (octets <= 64) return norm_shape_of<64, 1>(f);
     if (octets <= 128) return norm_shape_of<64, 2>(f);
     if (octets <= 192) return norm_shape_of<192, 1>(f);
-    if (octets <= 256) return norm_shape_of<256, 1>(f);
-    if (octets <= 384) return norm_shape_of<384, 1>(f);
-    if (octets <= 512) return norm_shape_of<512, 1>(f);
-    if (octets <= 768) return norm_shape_of<768, 1>(f);
-    if (octets <= 1024) return norm_shape_of<1024, 1>(f);
+    if (octets <= 256) return norm_shape_of<256 / PER, PER>(f);
+    if (octets <= 384) return norm_shape_of<384 / PER, PER>(f);
+    if (octets <= 512) return norm_shape_of<512 / PER, PER>(f);
+    if (octets <= 768) return norm_shape_of<768 / PER, PER>(f);
+    if (octets <= 1024) return norm_shape_of<1024 / PER, PER>(f);
     if (octets <= 2048) return norm_shape_of<512, 4>(f);
     if (octets <= 4096) return norm_shape_of<1024, 4>(f);
     return false;
@@ -731,7 +736,7 @@ int norm_forward_launch(const NormArgs &a, hipStream_t s)
 {
     const uint32_t octets = a.cols / kOctet;
     const char *name = ADD ? "layer_norm_add_forward" : "layer_norm_forward";
-    const bool fits = norm_shape(octets, [&](auto nt, auto k) {
+    const bool fits = norm_shape<sizeof(T) == 2 ? 2 : 1>(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
         constexpr int THREADS = norm_threads(NT, 256);
         if constexpr (ADD && NT * K > 2048) {
@@ -775,7 +780,7 @@ int norm_backward_launch(const NormGradArgs &a, W *grad_weight, W *grad_bias, hi
         LCPP_LAUNCH("layer_norm_backward_cols", s,
                     norm_backward_cols_kernel<T><<<dim3(blocks, parts), kColThreads, 0, s>>>(a));
     };
-    const bool fits = norm_shape(octets, [&](auto nt, auto k) {
+    const bool fits = norm_shape<1>(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
         constexpr int THREADS = norm_threads(NT, 512);
         constexpr bool kAcc = NT * K <= 2048;
