@@ -25,6 +25,17 @@
 //   "decay":    dg = dh h_{t-1},                   dx = dh
 //   "log":      dg = dh h_{t-1} a,                 dx = dh
 //   "sigmoid":  dg = dh (h_{t-1} - x) a (1 - a),   dx = dh (1 - a)
+//
+// Bound by memory where there are chains enough.  bfloat16, us by kernel traces and
+// TB/s of the bytes read and written once: 8 x 4096 x 2048 forward 81 (5.0), backward
+// 141 (4.8); 1 x 65536 x 2048 forward 166-172 (4.7-4.85); a copy of as many bytes
+// runs at 5.2.  Sequences of different lengths end with few tiles at work: 24 of
+// them, 16391 rows x 1536 in all, 39 + 60 (3.9, 4.2).  A single chain is bound by the
+// look-back, 0.06 us a tile: 1 x 40000 x 64 forward 19, backward 22.
+// kRows and kWaves: a tile has to lie in registers at four waves a SIMD.  With 18
+// and 20 rows a wave the backward pass of 8 x 4096 x 2048 took 181 and 178 us
+// where 16 took 159; 8 rows a wave, sixteen waves, four channels a lane and tiles of
+// 64 rows were slower too.
 #include <algorithm>
 
 #include "lookback.hpp"
@@ -193,6 +204,9 @@ struct Chan {
 // What the tiles before this one in the walk make of the sequence's first state:
 // their maps composed up to the nearest state.  One wave calls it; `words` are
 // those of this tile's channels, `step` is the distance to the tile before it.
+// A poll reads one tile's words: as all chains advance together, the tile before
+// has its state when its map is there, and a window of 2, 4 or 8 tiles reads words
+// that are not needed (1 x 65536 x 2048: 195 us with one, 216, 240 and 270).
 template <int C>
 __device__ __forceinline__ Chan<C> look_back(const uint64_t *words, uint64_t step, uint32_t before, const WaitCtl &ctl)
 {
@@ -215,6 +229,8 @@ __device__ __forceinline__ Chan<C> look_back(const uint64_t *words, uint64_t ste
                 if (lane_id() == 0) report_timeout(ctl);
                 return H;
             }
+            // (a tile's stores take far longer than this: polled at every 64 cycles 1 x
+            // 65536 x 2048 took 190 us, at every 512 186)
             __builtin_amdgcn_s_sleep(8);
         }
         bool all = true;

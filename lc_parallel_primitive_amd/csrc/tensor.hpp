@@ -13,17 +13,6 @@ namespace lcpp {
 using bf16 = __bf16;
 using f16 = _Float16;
 
-template <class T>
-__device__ __forceinline__ float to_f32(T v)
-{
-    return (float)v;
-}
-template <class T>
-__device__ __forceinline__ T from_f32(float v)
-{
-    return (T)v;
-}
-
 // N consecutive elements as they lie in memory.  Rows may begin at any element:
 // the vector types below ask for the alignment of one element only, and global
 // memory instructions take such addresses in one access on this part.
