@@ -721,13 +721,16 @@ uint64_t resident_groups(DeviceCache &cache, Kernel kernel, int threads)
 // types and for the backward pass, which keeps sums for each (us, one -> two:
 // forward of 16384 x 4096 bfloat16 59 -> 51, 8000 x 7000 64 -> 47, 2000 x 4096
 // float32 13 -> 15; backward of 1777 x 5001 float16 with the sum 25 -> 27, 8000 x
-// 7000 114 -> 123).
+// 7000 114 -> 123).  FINE: a group for 640 octets too, for the forward pass without
+// the sum (16384 x 5120 bfloat16 78 -> 76, 8000 x 5001 48 -> 44, 3000 x 4608 18 -> 14,
+// 4000 x 5120 float32 36 -> 35); with the sum (118 -> 132 at 16384 x 5120) and
+// backward (60 -> 62 at 8000 x 5001) the larger group's waves fill the CU better.
 template <int NT, int K, class F>
 bool norm_shape_of(F f)
 {
     return f(std::integral_constant<int, NT>{}, std::integral_constant<int, K>{});
 }
-template <int PER, class F>
+template <int PER, bool FINE, class F>
 bool norm_shape(uint32_t octets, F f)
 {
     if (octets <= 16) return norm_shape_of<16, 1>(f);
@@ -738,6 +741,9 @@ bool norm_shape(uint32_t octets, F f)
     if (octets <= 256) return norm_shape_of<256 / PER, PER>(f);
     if (octets <= 384) return norm_shape_of<384 / PER, PER>(f);
     if (octets <= 512) return norm_shape_of<512 / PER, PER>(f);
+    if constexpr (FINE) {
+        if (octets <= 640) return norm_shape_of<640 / PER, PER>(f);
+    }
     if (octets <= 768) return norm_shape_of<768 / PER, PER>(f);
     if (octets <= 1024) return norm_shape_of<1024 / PER, PER>(f);
     if (octets <= 2048) return norm_shape_of<512, 4>(f);
@@ -750,7 +756,7 @@ int norm_forward_launch(const NormArgs &a, hipStream_t s)
 {
     const uint32_t octets = a.cols / kOctet;
     const char *name = ADD ? "layer_norm_add_forward" : "layer_norm_forward";
-    const bool fits = norm_shape<sizeof(T) == 2 ? 2 : 1>(octets, [&](auto nt, auto k) {
+    const bool fits = norm_shape<sizeof(T) == 2 ? 2 : 1, !ADD>(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
         constexpr int THREADS = norm_threads(NT, 256);
         if constexpr (ADD && NT * K > 2048) {
@@ -794,7 +800,7 @@ int norm_backward_launch(const NormGradArgs &a, W *grad_weight, W *grad_bias, hi
         LCPP_LAUNCH("layer_norm_backward_cols", s,
                     norm_backward_cols_kernel<T><<<dim3(blocks, parts), kColThreads, 0, s>>>(a));
     };
-    const bool fits = norm_shape<1>(octets, [&](auto nt, auto k) {
+    const bool fits = norm_shape<1, false>(octets, [&](auto nt, auto k) {
         constexpr int NT = decltype(nt)::value, K = decltype(k)::value;
         constexpr int THREADS = norm_threads(NT, 512);
         constexpr bool kAcc = NT * K <= 2048;

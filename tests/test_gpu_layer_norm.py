@@ -70,6 +70,12 @@ def test_widths(lcpp, dtype, wt, cols):
     run_case(lcpp, dtype, wt, 5, cols)
 
 
+@pytest.mark.parametrize("cols", [4103, 5119, 5120, 5127, 5128])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_edges_of_the_five_eighths_group(lcpp, dtype, cols):
+    run_case(lcpp, dtype, "float32", 9, cols, pad=1)
+
+
 @pytest.mark.parametrize("nrows", [1, 2, 3, 4, 63, 513, 2050])
 @pytest.mark.parametrize("cols", [40, 700, 1536, 5000])
 def test_rows(lcpp, nrows, cols):
