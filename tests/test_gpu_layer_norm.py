@@ -259,6 +259,22 @@ def test_strides_past_32_bits(lcpp):
     assert torch.equal(x.contiguous(), tight)
 
 
+def test_a_row_wider_than_the_launches(lcpp):
+    # more columns than one launch's workgroups take at 64 each: the gradients' sums go round
+    cols = (1 << 26) + 70
+    log(f"layer norm backward, one row of {cols}")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, dy = (torch.randn(1, cols, generator=g, device="cuda") for _ in range(2))
+    mean, rstd = torch.tensor([0.125], device="cuda"), torch.tensor([0.75], device="cuda")
+    dx, dw, db = torch.empty_like(x), torch.full((cols,), 7.0, device="cuda"), torch.full((cols,), 7.0, device="cuda")
+    lcpp.DeviceLayerNorm().Backward(temp_for(lcpp, x, 1, cols), dy, x, None, mean, rstd, dx, dw, db)
+    torch.cuda.synchronize()
+    want = dy[0].double() * ((x[0].double() - 0.125) * 0.75)
+    # three roundings of a product, each of 2^-24
+    assert bool(((dw.double() - want).abs() <= 4 * 2.0**-24 * want.abs()).all())
+    assert torch.equal(db, dy[0])
+
+
 def test_refusals(lcpp):
     m = lcpp.DeviceLayerNorm()
     x = torch.zeros(4, 32, device="cuda")
