@@ -124,47 +124,73 @@ __device__ __forceinline__ void group_sum(float (&x)[V], float (*lds)[WAVES][2],
     }
 }
 
-// Mean and mean square deviation of a row.  A wave takes its columns' mean and
-// the squares around it; the waves' pairs meet in LDS at one barrier and combine:
-// the squares around the common mean are those around the wave's own plus n
-// times the square of the means' distance.  So a row far from 0 loses nothing.
-// `count`: columns of the wave; the lambda gives f(x, valid) for each of them.
+// A product as it is rounded, fused with no later sum: every difference from a mean
+// has to be from the same mean.
+__device__ __forceinline__ float rounded(float x)
+{
+    asm("" : "+v"(x));
+    return x;
+}
+// x, or 0 in the place of infinities and NaN.
+__device__ __forceinline__ float finite_or_0(float x)
+{
+    return fabsf(x) <= std::numeric_limits<float>::max() ? x : 0.0f;
+}
+// An infinite mean has no rest, and the difference of squares is not below 0 (a NaN
+// stays one).
+__device__ __forceinline__ void norm_rest(float &rest, float &sq)
+{
+    rest = finite_or_0(rest);
+    sq = sq < 0.0f ? 0.0f : sq;
+}
+
+// Mean and mean square deviation of a row.  The mean of a first sum is off by some
+// roundings of its size, which is much where a row lies far from 0 and varies
+// little, so the second pass sums the differences from it as well as their squares:
+// the mean is `mean` + `rest`, known to roundings of the differences alone, and the
+// squares around it are those around `mean` less n rest^2.  A wave does this for
+// its columns; the waves' values meet in LDS at one barrier, one wave's in each of
+// 16 lanes, and combine as distances from the first wave's mean.  (16384 x 4096 bfloat16
+// 52.6 us, with the first sum alone and each thread adding up the waves 53.0.)
+// `count`, `lane_count`: columns of the wave, and of the wave whose values the lane
+// combines (0: none); `each` gives f(x) for each of the thread's columns.
 template <int NT, int WAVES, class F>
-__device__ __forceinline__ void group_moments(F each, float count, float (*lds)[WAVES][2], const float *counts, int slot,
-                                              float cols, float &mean, float &var)
+__device__ __forceinline__ void group_moments(F each, float count, float lane_count, float (*lds)[WAVES][3], int slot,
+                                              float cols, float inv_cols, float &mean, float &rest, float &var)
 {
     float sum = 0.0f;
     each([&](float x) { sum += x; });
     const float inv = count > 0.0f ? 1.0f / count : 0.0f;
-    mean = lanes_sum<NT>(sum) * inv;
-    float sq = 0.0f;
+    mean = rounded(lanes_sum<NT>(sum) * inv);
+    float off = 0.0f, sq = 0.0f;
     each([&](float x) {
         const float d = x - mean;
+        off += d;
         sq += d * d;
     });
-    sq = lanes_sum<NT>(sq);
+    rest = lanes_sum<NT>(off) * inv;
+    sq = lanes_sum<NT>(sq) - count * (rest * rest);
+    norm_rest(rest, sq);
     if constexpr (NT > kWave) {
-        constexpr int GW = NT / kWave;
-        const uint32_t wave = threadIdx.x / kWave, first = wave / GW * GW;
-        if (lane_id() == 0) lds[slot][wave][0] = mean, lds[slot][wave][1] = sq;
+        constexpr uint32_t GW = NT / kWave;
+        const uint32_t wave = threadIdx.x / kWave, from = lane_id() % 16;
+        if (lane_id() == 0) lds[slot][wave][0] = mean, lds[slot][wave][1] = rest, lds[slot][wave][2] = sq;
         group_barrier();
-        float m[GW], n[GW], total = 0.0f;
-        sq = 0.0f;
-#pragma unroll
-        for (int w = 0; w < GW; ++w) {
-            m[w] = lds[slot][first + w][0];
-            n[w] = counts[w];
-            sq += lds[slot][first + w][1];
-            total += n[w] * m[w];
-        }
-        mean = total / cols;
-#pragma unroll
-        for (int w = 0; w < GW; ++w) {
-            const float d = m[w] - mean;
-            sq += n[w] * (d * d);
-        }
+        const bool has = from < GW;
+        const float(*w)[3] = &lds[slot][wave / GW * GW];
+        // (the first lane's sum for all: a product that is fused with a sum's first addition
+        // is rounded differently in two lanes, and `rest` has to belong to `mean`)
+        auto waves_sum = [](float x) { return read_lane(lanes_sum<16>(x), 0); };
+        const float base = finite_or_0(w[0][0]);
+        const float d = has ? (w[has ? from : 0][0] - base) + w[has ? from : 0][1] : 0.0f;
+        const float nd = lane_count * d;
+        const float shift = rounded(waves_sum(nd) * inv_cols);
+        sq = waves_sum((has ? w[has ? from : 0][2] : 0.0f) + nd * d) - cols * (shift * shift);
+        mean = base + shift;
+        rest = (base - mean) + shift;
+        norm_rest(rest, sq);
     }
-    var = sq / cols;
+    var = sq * inv_cols;
 }
 
 // One octet of a vector of weights, or one value everywhere.
@@ -206,28 +232,26 @@ __device__ __forceinline__ float drop_one(float x, uint32_t row, uint32_t col, u
 template <class T, class W, int NT, int K, int THREADS, bool ADD, bool AHEAD>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ? 1 : ADD && sizeof(T) == 4 ? 2 : 4))) void norm_forward_kernel(NormArgs a)
 {
-    constexpr int WAVES = THREADS / kWave, RG = THREADS / NT, GW = NT > kWave ? NT / kWave : 1;
+    constexpr int WAVES = THREADS / kWave, RG = THREADS / NT;
+    constexpr uint32_t GW = NT > kWave ? NT / kWave : 1;
     constexpr uint32_t kLaneCols = (NT < kWave ? NT : kWave) * kOctet;
-    __shared__ float lds[2][WAVES][2];
+    __shared__ float lds[2][WAVES][3];
     const Columns<NT, K> c(a.cols);
     const uint32_t group = threadIdx.x / NT;
     const uint64_t offset = ADD ? drop_offset(a.drop) : 0;
-    // columns of each wave of a group (the same for every group)
-    float counts[GW];
-#pragma unroll
-    for (int w = 0; w < GW; ++w) {
-        uint32_t n = 0;
+    // columns of a wave of the group
+    auto wave_cols = [&](uint32_t w) {
+        uint32_t n = w == 0 ? c.rem : 0;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const uint32_t from = (w * kWave + k * NT) * kOctet;
             n += from < c.full ? (c.full - from < kLaneCols ? c.full - from : kLaneCols) : 0;
         }
-        counts[w] = (float)(n + (w == 0 ? c.rem : 0));
-    }
-    const uint32_t wave = threadIdx.x / kWave;
-    float count = counts[0];
-#pragma unroll
-    for (int w = 1; w < GW; ++w) count = wave % GW == (uint32_t)w ? counts[w] : count;
+        return (float)n;
+    };
+    const float inv_cols = 1.0f / (float)a.cols;
+    const float count = wave_cols(threadIdx.x / kWave % GW);
+    const float lane_count = lane_id() % 16 < GW ? wave_cols(lane_id() % 16) : 0.0f;
 
     RowPart<W, K> w, b;
     if constexpr (AHEAD) {
@@ -279,7 +303,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ?
                 }
             }
         }
-        float mean, var;
+        float mean, rest, var;
         group_moments<NT, WAVES>(
             [&](auto f) {
                 if (!live) return;
@@ -290,8 +314,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ?
                         for (int i = 0; i < kOctet; ++i) f(x.o[k][i]);
                 if (c.has_tail()) f((float)x.tail);
             },
-            count, lds, counts, slot, (float)a.cols, mean, var);
-        const float rstd = 1.0f / sqrtf(var + a.eps);
+            count, lane_count, lds, slot, (float)a.cols, inv_cols, mean, rest, var);
+        const float rstd = 1.0f / sqrtf(var + a.eps), shift = rest * rstd;
         if (!live) continue;
         T *out = static_cast<T *>(a.out) + row * a.out_stride;
 #pragma unroll
@@ -303,7 +327,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ?
             }
             float y[kOctet];
 #pragma unroll
-            for (int i = 0; i < kOctet; ++i) y[i] = (x.o[k][i] - mean) * rstd * w.o[k][i] + b.o[k][i];
+            for (int i = 0; i < kOctet; ++i) y[i] = ((x.o[k][i] - mean) * rstd - shift) * w.o[k][i] + b.o[k][i];
             store_pack_nt<kOctet>(out + c.col(k), y);
         }
         if constexpr (!AHEAD) {
@@ -312,9 +336,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ?
                 b.tail = a.bias ? static_cast<const W *>(a.bias)[c.tail()] : (W)0.0f;
             }
         }
-        if (c.has_tail()) out[c.tail()] = (T)(((float)x.tail - mean) * rstd * (float)w.tail + (float)b.tail);
+        if (c.has_tail()) out[c.tail()] = (T)((((float)x.tail - mean) * rstd - shift) * (float)w.tail + (float)b.tail);
         if (c.t == 0) {
-            if (a.mean) a.mean[row] = mean;
+            if (a.mean) a.mean[row] = mean + rest;
             if (a.rstd) a.rstd[row] = rstd;
         }
     }
@@ -375,29 +399,31 @@ __global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(NormArg
         }
         group_sum<kLongThreads, kLongWaves>(sum, lds, 0);
         const float mean = sum[0] / (float)a.cols;
-        float sq[1] = {0.0f};
+        float off[2] = {0.0f, 0.0f};  // sums of the differences and of their squares, as in group_moments
         // (each thread reads back the sums that it stored itself)
         for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
             const Octet<T> x = load_octet(s, col, a.cols);
 #pragma unroll
             for (int i = 0; i < kOctet; ++i) {
                 const float d = x[i] - mean;
-                if (col + i < a.cols) sq[0] += d * d;
+                if (col + i < a.cols) off[0] += d, off[1] += d * d;
             }
         }
-        group_sum<kLongThreads, kLongWaves>(sq, lds, 1);
-        const float rstd = 1.0f / sqrtf(sq[0] / (float)a.cols + a.eps);
+        group_sum<kLongThreads, kLongWaves>(off, lds, 1);
+        float rest = off[0] / (float)a.cols, sq = off[1] - off[0] * rest;
+        norm_rest(rest, sq);
+        const float rstd = 1.0f / sqrtf(sq / (float)a.cols + a.eps), shift = rest * rstd;
         for (uint32_t col = threadIdx.x * kOctet; col < a.cols; col += kLongThreads * kOctet) {
             const Octet<T> x = load_octet(s, col, a.cols);
             float w[kOctet], b[kOctet];
             norm_weight<W>(a.weight, col, a.cols, 1.0f, w);
             norm_weight<W>(a.bias, col, a.cols, 0.0f, b);
 #pragma unroll
-            for (int i = 0; i < kOctet; ++i) w[i] = (x[i] - mean) * rstd * w[i] + b[i];
+            for (int i = 0; i < kOctet; ++i) w[i] = ((x[i] - mean) * rstd - shift) * w[i] + b[i];
             store_octet(static_cast<T *>(a.out) + row * a.out_stride, col, a.cols, w);
         }
         if (threadIdx.x == 0) {
-            if (a.mean) a.mean[row] = mean;
+            if (a.mean) a.mean[row] = mean + rest;
             if (a.rstd) a.rstd[row] = rstd;
         }
     }
