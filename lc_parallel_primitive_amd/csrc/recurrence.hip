@@ -201,53 +201,142 @@ struct Chan {
     float v[C];
 };
 
-// What the tiles before this one in the walk make of the sequence's first state:
-// their maps composed up to the nearest state.  One wave calls it; `words` are
-// those of this tile's channels, `step` is the distance to the tile before it.
-// A poll reads one tile's words: as all chains advance together, the tile before
-// has its state when its map is there, and a window of 2, 4 or 8 tiles reads words
-// that are not needed (1 x 65536 x 2048: 195 us with one, 216, 240 and 270).
+// The state after a tile, or after a step: one rounding, the same wherever it is taken.
+__device__ __forceinline__ float advance(float A, float h, float H) { return __builtin_fmaf(A, h, H); }
+
+// The state before this tile: the walk goes back over the tiles' maps to the nearest
+// state, and then forward again from it, one map after the other.  So the state is
+// what each tile in turn makes of the one before it, whichever words the walk meets:
+// the same bits at every call.  (Maps composed on the way back would be rounded in
+// an order that depends on timing.)  The nearest map stays in registers and those
+// after it in LDS; where kBack of them come before a state the walk waits there for
+// it.  One wave calls it; `words` are those of this tile's channels, `step` is the
+// distance to the tile before it, `before` the number of tiles there.
+// The first poll reads one tile's words: as all chains advance together, the tile
+// before has its state when its map is there, and a first window of 2, 4 or 8 tiles
+// reads words that are not needed (1 x 65536 x 2048: 195 us with one, 216, 240 and
+// 270).  A walk that goes on reads kWindow at once (forward + backward, one at once ->
+// four: 1 x 100000 x 512 float32 121 + 184 -> 113 + 184, 1 x 65536 x 2048 165 + 280 -> 163 +
+// 273), and 32 KB of maps are 64 or 32 of them (1 x 40000 x 64 with 32 maps 30 + 32, with
+// 64 27 + 29.5).  Maps composed on the way back, in no fixed order, took 112 + 183, 160 +
+// 276 and 20 + 22 for these three.  More registers than these cost the backward pass of
+// two channels a workgroup per CU.
 template <int C>
-__device__ __forceinline__ Chan<C> look_back(const uint64_t *words, uint64_t step, uint32_t before, const WaitCtl &ctl)
+constexpr uint32_t kBack = 64 / C;
+constexpr uint32_t kWindow = 4;
+template <int C>
+struct Words {
+    uint64_t v[C];
+};
+template <int C>
+__device__ __forceinline__ void apply_words(const Words<C> &w, Chan<C> &h)
 {
-    Chan<C> A, H;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t up = (uint32_t)(w.v[c] >> 32);
+        const float H = __builtin_bit_cast(float, (uint32_t)w.v[c]);
+        h.v[c] = up == kWordState ? H : advance(__builtin_bit_cast(float, ~up), h.v[c], H);
+    }
+}
+// Whether a word can be taken: a state, or a map where the walk may go on; a channel
+// that has met its state takes any.
+template <int C>
+__device__ __forceinline__ bool words_ready(const Words<C> &w, const bool (&done)[C], bool maps)
+{
+    bool ready = true;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const uint32_t up = (uint32_t)(w.v[c] >> 32);
+        ready = ready && (done[c] || up == kWordState || (up != 0 && maps));
+    }
+    return ballot(!ready) == 0;
+}
+template <int C>
+__device__ __forceinline__ bool words_end(const Words<C> &w, bool (&done)[C])
+{
+    bool all = true;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        done[c] = done[c] || (uint32_t)(w.v[c] >> 32) == kWordState;
+        all = all && done[c];
+    }
+    return ballot(!all) == 0;
+}
+template <int C>
+__device__ __forceinline__ void load_words(const uint64_t *words, Words<C> &w)
+{
+#pragma unroll
+    for (int c = 0; c < C; ++c) w.v[c] = ld_relaxed(words + c);
+}
+template <int C>
+__device__ __forceinline__ Chan<C> look_back(const uint64_t *words, uint64_t step, uint32_t before,
+                                             Words<C> (*maps)[kWave], const WaitCtl &ctl)
+{
+    const uint32_t lane = lane_id();
+    Chan<C> h;
     bool done[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) A.v[c] = 1.0f, H.v[c] = 0.0f, done[c] = false;
+    for (int c = 0; c < C; ++c) h.v[c] = 0.0f, done[c] = false;
     uint32_t spins = 0;
-    for (uint32_t k = 1; k <= before;) {
-        words -= step;
-        uint64_t w[C];
-        for (;;) {
-            bool ready = true;
-#pragma unroll
-            for (int c = 0; c < C; ++c) w[c] = ld_relaxed(words + c);
-#pragma unroll
-            for (int c = 0; c < C; ++c) ready = ready && (done[c] || (uint32_t)(w[c] >> 32) != 0);
-            if (ballot(!ready) == 0) break;
-            if (++spins >= ctl.spin_limit) {
-                if (lane_id() == 0) report_timeout(ctl);
-                return H;
-            }
-            // (a tile's stores take far longer than this: polled at every 64 cycles 1 x
-            // 65536 x 2048 took 190 us, at every 512 186)
-            __builtin_amdgcn_s_sleep(8);
+    auto again = [&] {
+        if (++spins >= ctl.spin_limit) {
+            if (lane == 0) report_timeout(ctl);
+            return false;
         }
-        bool all = true;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const uint32_t up = (uint32_t)(w[c] >> 32);
-            if (!done[c]) {
-                H.v[c] += A.v[c] * __builtin_bit_cast(float, (uint32_t)w[c]);
-                A.v[c] *= __builtin_bit_cast(float, ~up);
-                done[c] = up == kWordState;
-            }
-            all = all && done[c];
-        }
-        if (ballot(!all) == 0) break;
-        ++k;
+        // (a tile's stores take far longer than this: polled at every 64 cycles 1 x
+        // 65536 x 2048 took 190 us, at every 512 186)
+        __builtin_amdgcn_s_sleep(8);
+        return true;
+    };
+    Words<C> near;
+    words -= step;
+    for (;;) {
+        load_words(words, near);
+        if (words_ready(near, done, true)) break;
+        if (!again()) return h;
     }
-    return H;
+    Words<C> far = near;
+    bool end = words_end(near, done);
+    const bool alone = end;
+    uint32_t met = 0;  // maps in LDS, the nearest first
+    while (!end) {
+        // (the first tile has a state, so there is a tile before a walk that is not at its end)
+        const uint32_t left = before - 1 - met, n = left < kWindow ? left : kWindow;
+        Words<C> w[kWindow];
+#pragma unroll
+        for (uint32_t i = 0; i < kWindow; ++i) load_words(words - (i < n ? i + 1 : n) * step, w[i]);
+        uint32_t took = 0;
+        bool go = true;
+#pragma unroll
+        for (uint32_t i = 0; i < kWindow; ++i) {
+            if (!go || i >= n) continue;
+            go = words_ready(w[i], done, met < kBack<C>);
+            if (!go) continue;
+            far = w[i];
+            end = words_end(w[i], done);
+            go = !end;
+            if (end) continue;
+            maps[met++][lane] = w[i];
+            ++took;
+        }
+        words -= took * step;
+        if (!end && !took && !again()) return h;
+    }
+    // (a channel that was done nearer ends with that state)
+    apply_words(far, h);
+    while (met) {
+        constexpr uint32_t kAtOnce = 4;
+        const uint32_t n = met < kAtOnce ? met : kAtOnce;
+        Words<C> m[kAtOnce];
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) m[i] = maps[met - 1 - (i < n ? i : n - 1)][lane];
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i)
+            if (i < n) apply_words(m[i], h);
+        met -= n;
+    }
+    if (!alone) apply_words(near, h);
+    return h;
 }
 
 // One wave publishes its tile's map, and then the state after it.
@@ -261,7 +350,7 @@ template <int C>
 __device__ __forceinline__ void publish_state(uint64_t *words, const Chan<C> &A, const Chan<C> &H, const Chan<C> &h)
 {
 #pragma unroll
-    for (int c = 0; c < C; ++c) st_relaxed(words + c, word_state(A.v[c] * h.v[c] + H.v[c]));
+    for (int c = 0; c < C; ++c) st_relaxed(words + c, word_state(advance(A.v[c], h.v[c], H.v[c])));
 }
 
 // Rows that begin at a line of memory (STREAM) are read and written with the
@@ -313,6 +402,8 @@ template <class T, class G, int C, int W, bool STREAM>
 __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) void rec_forward_kernel(RecArgs a)
 {
     __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_carry[kWave];
+    constexpr bool kWalks = W == kWaves;  // (sequences of one tile have fewer waves)
+    __shared__ Words<C> s_back[kWalks ? kBack<C> : 1][kWave];
     Place p;
     if (!find_place<C>(a, false, p)) return;
     const uint32_t wave = wave_id(), lane = lane_id();
@@ -369,11 +460,11 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
             if (p.walk > 0) publish_map<C>(words, A, H);
         }
         Chan<C> h;
-        if (p.walk == 0) {
+        if (!kWalks || p.walk == 0) {
 #pragma unroll
             for (int c = 0; c < C; ++c) h.v[c] = a.initial ? a.initial[state_at + c] : 0.0f;
         } else {
-            h = look_back<C>(words, tile_words, p.walk, a.ctl);
+            h = look_back<C>(words, tile_words, p.walk, s_back, a.ctl);
         }
         s_carry[lane] = h;
         if (publish) publish_state<C>(words, A, H, h);
@@ -429,6 +520,8 @@ template <class T, class G, int C, int W, bool STREAM>
 __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
 {
     __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_E[W][kWave], s_carry[kWave];
+    constexpr bool kWalks = W == kWaves;  // (sequences of one tile have fewer waves)
+    __shared__ Words<C> s_back[kWalks ? kBack<C> : 1][kWave];
     Place p;
     if (!find_place<C>(a, true, p)) return;
     const uint32_t wave = wave_id(), lane = lane_id();
@@ -498,11 +591,11 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
             if (p.walk > 0) publish_map<C>(words, A, E);
         }
         Chan<C> e;
-        if (p.walk == 0) {
+        if (!kWalks || p.walk == 0) {
 #pragma unroll
             for (int c = 0; c < C; ++c) e.v[c] = a.grad_final ? a.grad_final[state_at + c] : 0.0f;
         } else {
-            e = look_back<C>(words, tile_words, p.walk, a.ctl);
+            e = look_back<C>(words, tile_words, p.walk, s_back, a.ctl);
         }
         s_carry[lane] = e;
         if (publish) publish_state<C>(words, A, E, e);
