@@ -418,7 +418,8 @@ int lcpp_dropout(lcpp_dtype t, const void *in, uint64_t in_stride, const void *r
  * A call covers fewer than 2^23 tiles of 128 rows and 128 channels (64 of float32), sequences of
  * max_length each; max_length < 2^31.  Rows are composed in parallel, so products of neighbouring
  * gates are formed: gates above 1 whose products pass float32's range can give NaN where a state
- * that stays 0 would have hidden them. */
+ * that stays 0 would have hidden them.  The temp query's size serves every type whose call is
+ * within that limit; it fails where none is. */
 int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes);
 int lcpp_recurrence_checkpoint_rows(uint64_t max_length, uint64_t *rows);
 int lcpp_recurrence_forward(lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, const void *gate,

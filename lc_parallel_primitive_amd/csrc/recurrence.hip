@@ -824,11 +824,18 @@ using namespace lcpp;
 
 extern "C" int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes)
 {
-    RecShape r;
-    if (!bytes || !rec_shape(sequences, max_length, channels, 2, false, &r)) return LCPP_ERR_INVALID_ARG;
-    *bytes = rec_temp_bytes(r);
-    if (!rec_shape(sequences, max_length, channels, 4, false, &r)) return LCPP_ERR_INVALID_ARG;
-    *bytes = std::max<size_t>(*bytes, rec_temp_bytes(r));  // for every type
+    if (!bytes) return LCPP_ERR_INVALID_ARG;
+    // the larger of the types' sizes, of those whose call can be launched (2-byte types have half the workgroups)
+    bool any = false;
+    uint64_t most = 0;
+    for (size_t size : {2, 4}) {
+        RecShape r;
+        if (!rec_shape(sequences, max_length, channels, size, false, &r)) continue;
+        any = true;
+        most = std::max(most, rec_temp_bytes(r));
+    }
+    if (!any) return LCPP_ERR_INVALID_ARG;
+    *bytes = most;
     return LCPP_OK;
 }
 
