@@ -69,10 +69,10 @@ class AddNorm(torch.autograd.Function):
 class Recurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, begin, end, longest):
-        n, c = begin.numel(), x.shape[1]
+        n, (rows, c) = begin.numel(), x.shape
         y = torch.empty_like(x)
-        ctx.temp = _temp(lcpp.DeviceGatedRecurrence.GetTempStorageBytes(n, longest, c))
-        saved = torch.empty(n, lcpp.DeviceGatedRecurrence.GetCheckpointRows(longest), c, device=x.device)
+        ctx.temp = _temp(lcpp.DeviceGatedRecurrence.GetTempStorageBytes(n, longest, c, rows))
+        saved = torch.empty(lcpp.DeviceGatedRecurrence.GetPackedCheckpointRows(n, longest, rows), c, device=x.device)
         ctx.where = dict(d_begin_offsets=begin, d_end_offsets=end, max_length=longest)
         MIX.Forward(ctx.temp, gate, x, y, "sigmoid", d_checkpoints=saved, **ctx.where)
         ctx.save_for_backward(gate, x, saved)

@@ -683,6 +683,19 @@ class DeviceGatedRecurrence : public LuisaModule {
         lcpp_recurrence_checkpoint_rows(max_length, &r);
         return r;
     }
+    /* the same for sequences with offsets, which need no more than their rows do */
+    static size_t GetPackedTempStorageBytes(const Sequences &seq)
+    {
+        size_t b = 0;
+        lcpp_recurrence_packed_temp_bytes(seq.count, seq.length, seq.channels, seq.rows, &b);
+        return b;
+    }
+    static size_t GetPackedCheckpointRows(const Sequences &seq) /* of all sequences */
+    {
+        uint64_t r = 0;
+        lcpp_recurrence_packed_checkpoint_rows(seq.count, seq.length, seq.rows, &r);
+        return r;
+    }
     template <class T>
     void Forward(CommandList &cmdlist, BufferView<uint> temp_storage, lcpp_gate gate, RowsView<T> d_gate, RowsView<T> d_in,
                  RowsView<T> d_out, const float *d_initial, float *d_final, float *d_checkpoints, const Sequences &seq)

@@ -415,13 +415,19 @@ int lcpp_dropout(lcpp_dtype t, const void *in, uint64_t in_stride, const void *r
  * initial (NULL: 0), final_state: the states before the first and after the last row, float32
  * [sequences][channels]; an empty sequence's final state is its initial one.  checkpoints: what
  * the backward pass needs, float32 [sequences][lcpp_recurrence_checkpoint_rows][channels], or NULL.
- * A call covers fewer than 2^23 tiles of 128 rows and 128 channels (64 of float32), sequences of
- * max_length each; max_length < 2^31.  Rows are composed in parallel, so products of neighbouring
- * gates are formed: gates above 1 whose products pass float32's range can give NaN where a state
- * that stays 0 would have hidden them.  The temp query's size serves every type whose call is
- * within that limit; it fails where none is. */
+ * A call covers fewer than 2^23 tiles of 128 rows and 128 channels (64 of float32); max_length <
+ * 2^31.  With begin and end that are rows / 128 + sequences of them, whatever the longest sequence:
+ * the packed queries give the temp storage and the checkpoints' rows, [rows][channels], for as many
+ * (sequences of different lengths need far less than max_length each, which the other two queries
+ * are for, and which serves packed calls too).  A temp query's size serves every type whose call is
+ * within the limit; it fails where none is.  Rows are composed in parallel, so products of
+ * neighbouring gates are formed: gates above 1 whose products pass float32's range can give NaN
+ * where a state that stays 0 would have hidden them. */
 int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes);
 int lcpp_recurrence_checkpoint_rows(uint64_t max_length, uint64_t *rows);
+int lcpp_recurrence_packed_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, uint64_t rows,
+                                      size_t *bytes);
+int lcpp_recurrence_packed_checkpoint_rows(uint64_t sequences, uint64_t max_length, uint64_t rows, uint64_t *out);
 int lcpp_recurrence_forward(lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, const void *gate,
                             uint64_t gate_row, uint64_t gate_seq, const void *in, uint64_t in_row, uint64_t in_seq,
                             void *out, uint64_t out_row, uint64_t out_seq, const float *initial, float *final_state,

@@ -83,6 +83,8 @@ SIGNATURES = {
     "lcpp_dropout": (_i, [_i, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _d, _u64, _u64, _vp, _vp]),
     "lcpp_recurrence_temp_bytes": (_i, [_u64, _u64, _u64, _c_size_p]),
     "lcpp_recurrence_checkpoint_rows": (_i, [_u64, ctypes.POINTER(_u64)]),
+    "lcpp_recurrence_packed_temp_bytes": (_i, [_u64, _u64, _u64, _u64, _c_size_p]),
+    "lcpp_recurrence_packed_checkpoint_rows": (_i, [_u64, _u64, _u64, ctypes.POINTER(_u64)]),
     "lcpp_recurrence_forward": (_i, [_i, _i, _vp, ctypes.c_size_t] + [_vp, _u64, _u64] * 3 + [_vp, _vp, _vp, _u64, _u64, _u64, _vp,
                                      _vp, _u64, _vp]),
     "lcpp_recurrence_backward": (_i, [_i, _i, _vp, ctypes.c_size_t] + [_vp, _u64, _u64] * 2 + [_vp] + [_vp, _u64, _u64] * 3

@@ -56,16 +56,25 @@ struct RowsOut {
     void *p;
     uint64_t row, seq;
 };
+// One tile of a sequence that lies somewhere in the tensors' rows.
+struct alignas(32) PackedTile {
+    uint32_t seq, walk;  // walk: tiles of the sequence before this one in the walk
+    uint32_t row, len;   // of the sequence
+    uint32_t base;       // tiles of the sequences before it
+};
+constexpr uint32_t kNoSequence = 0xFFFFFFFFu;
 struct RecArgs {
     RowsIn gate, in, grad_out;
     RowsOut out, grad_gate, grad_in;
     const float *initial, *grad_final;     // [sequence][channel]
     float *final_state, *grad_initial;     // [sequence][channel]
-    float *checkpoints;                    // [sequence][tile][channel]
+    float *checkpoints;                    // [tile of all sequences][channel]
     const uint32_t *begin, *end;           // null: sequence s begins at its stride, with max_length rows
     uint64_t rows;                         // with begin and end: rows of the tensors
     uint32_t sequences, tiles, groups, channels, max_length;
     uint32_t run, turns;                   // chains of a run (0: no runs); workgroups of a tile of time
+    const PackedTile *list;                // with begin and end, sequences of several tiles: `all` tiles
+    uint32_t all;
     uint64_t *words;                       // [sequence][tile of the walk][group][lane's channels]
     WaitCtl ctl;
 };
@@ -108,11 +117,23 @@ struct GateSigmoid {
 struct Place {
     uint32_t seq, tile, len, channel, group;
     uint32_t walk;    // tiles of the sequence before this one in the walk
+    uint32_t base;    // tiles of the sequences before it, which its checkpoints come after
+    uint32_t word_base;  // the same for the look-back words
     uint32_t number;  // of the tile among all, for the test hook
     bool active;   // the lane has a channel
     bool single;   // the first lane has one channel, the others none
     uint64_t row;  // of the tensors' rows that the sequence begins at (with offsets)
 };
+// The rows of sequence s, inside the tensors' rows and no more than max_length.
+__device__ __forceinline__ void sequence_rows(const uint32_t *begin, const uint32_t *end, uint64_t rows, uint32_t max_length,
+                                              uint32_t s, uint64_t &first, uint32_t &len)
+{
+    first = begin[s];
+    const uint64_t last = end[s] < rows ? end[s] : rows;
+    const uint64_t n = last > first ? last - first : 0;
+    len = n < max_length ? (uint32_t)n : max_length;
+}
+constexpr uint32_t kXcds = 8;
 // Workgroups are numbered tile by tile, so a tile waits only on workgroups
 // dispatched before its own; `reverse` counts tiles from the sequence's end.
 //
@@ -126,33 +147,56 @@ struct Place {
 // in turn.  Sequences of different lengths have short runs, or the last one at
 // work would leave XCDs idle (24 packed x 1536 channels: 142 with an eighth of
 // all chains, 108 with runs of 4).  Numbers past the last chain are left at once.
-constexpr uint32_t kXcds = 8;
+//
+// Sequences of different lengths (offsets) have their tiles in a list, which the
+// clearing launch makes from the offsets: there are no more than rows / 128 + sequences,
+// however long the longest is.  The list is in the same order, the first tiles of
+// (up to kListSequences) sequences, then the second tiles of those that have one, and
+// so on.  Runs of four chains lie on one XCD there too, dealt out within windows of 8
+// runs: a tile of a window may wait on one that is dispatched up to 31 workgroups
+// after it, of which each XCD has four at most and room for many more.  Measured against
+// the tiles of sequences x the longest, most of them empty (forward + backward): 24 x
+// 16391 rows x 1536 bfloat16 40 + 60 -> 36 + 57, 256 x 65536 x 1024 120 + 166 -> 85 + 139, 256 x
+// 262144 x 2048 with one of 32768 2255 + 2672 -> 655 + 1092.
 template <int C>
 __device__ __forceinline__ bool find_place(const RecArgs &a, bool reverse, Place &p)
 {
-    const uint32_t k = blockIdx.x / a.turns, turn = blockIdx.x - k * a.turns;
-    uint32_t chain = turn;
-    if (a.run) {
-        const uint32_t y = turn / kXcds;
-        chain = (y / a.run * kXcds + (turn + k) % kXcds) * a.run + y % a.run;
+    uint32_t tiles;
+    if (a.list) {
+        uint32_t item = blockIdx.x;
+        if (a.run) {
+            const uint32_t window = item / (kXcds * a.run), r = item - window * (kXcds * a.run), y = r / kXcds;
+            item = (window * kXcds + (r + window + window / kXcds + window / (kXcds * kXcds)) % kXcds) * a.run + y;
+        }
+        p.number = item;
+        const uint32_t at = item / a.groups;
+        p.group = item - at * a.groups;
+        if (at >= a.all) return false;
+        const PackedTile t = a.list[at];
+        if (t.seq == kNoSequence) return false;
+        p.seq = t.seq, p.walk = t.walk, p.row = t.row, p.len = t.len;
+        p.base = t.base;
+        p.word_base = t.base - t.seq;  // (the last tile of a sequence has no words)
+        tiles = (p.len + kTileRows - 1) / kTileRows;
+    } else {
+        const uint32_t k = blockIdx.x / a.turns, turn = blockIdx.x - k * a.turns;
+        uint32_t chain = turn;
+        if (a.run) {
+            const uint32_t y = turn / kXcds;
+            chain = (y / a.run * kXcds + (turn + k) % kXcds) * a.run + y % a.run;
+        }
+        p.seq = chain / a.groups;
+        p.group = chain - p.seq * a.groups;
+        if (p.seq >= a.sequences) return false;
+        p.number = (k * a.sequences + p.seq) * a.groups + p.group;
+        p.row = 0;
+        p.len = a.max_length;
+        if (a.begin) sequence_rows(a.begin, a.end, a.rows, a.max_length, p.seq, p.row, p.len);
+        tiles = (p.len + kTileRows - 1) / kTileRows;
+        p.walk = k;
+        p.base = p.word_base = p.seq * a.tiles;
     }
-    p.seq = chain / a.groups;
-    p.group = chain - p.seq * a.groups;
-    if (p.seq >= a.sequences) return false;
-    p.number = (k * a.sequences + p.seq) * a.groups + p.group;
-    p.row = 0;
-    p.len = a.max_length;
-    if (a.begin) {
-        const uint64_t first = a.begin[p.seq];
-        const uint64_t end = a.end[p.seq] < a.rows ? a.end[p.seq] : a.rows;
-        const uint64_t n = end > first ? end - first : 0;
-        p.row = first;
-        p.len = n < a.max_length ? (uint32_t)n : a.max_length;
-    }
-    const uint32_t tiles = (p.len + kTileRows - 1) / kTileRows;
-    if (k >= tiles && !(k == 0 && tiles == 0)) return false;
-    p.walk = k;
-    p.tile = reverse && tiles ? tiles - 1 - k : k;
+    p.tile = reverse && tiles ? tiles - 1 - p.walk : p.walk;
     const uint32_t c = p.group * (kWave * C) + lane_id() * C;
     p.active = c < a.channels;
     p.channel = c + C <= a.channels ? c : a.channels - C;
@@ -412,7 +456,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
     const uint32_t last = p.len ? p.len - 1 : 0;
     const bool more = ((uint64_t)p.tile + 1) * kTileRows < p.len;  // a tile follows
     const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
-    uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.walk) * tile_words + (uint64_t)p.group * kWave * C + lane * C;
+    uint64_t *words = a.words + ((uint64_t)p.word_base + p.walk) * tile_words + (uint64_t)p.group * kWave * C + lane * C;
 
     Chan<C> ga[kRows], gb[kRows], A, H;
     {
@@ -470,7 +514,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
         if (publish) publish_state<C>(words, A, H, h);
         if (p.active) {
             if (a.checkpoints && p.len)
-                store_state(a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels, p, h);
+                store_state(a.checkpoints + ((uint64_t)p.base + p.tile) * a.channels, p, h);
             if (a.final_state && !p.len) store_state(a.final_state + state_row, p, h);
         }
     }
@@ -538,7 +582,7 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     const uint32_t first = p.tile * kTileRows + wave * kRows;
     const uint32_t last = p.len - 1;
     const uint64_t tile_words = (uint64_t)a.groups * kWave * C;
-    uint64_t *words = a.words + ((uint64_t)p.seq * a.tiles + p.walk) * tile_words + (uint64_t)p.group * kWave * C + lane * C;
+    uint64_t *words = a.words + ((uint64_t)p.word_base + p.walk) * tile_words + (uint64_t)p.group * kWave * C + lane * C;
 
     Pack<T, C> gr[kRows], xr[kRows], dyr[kRows];
     {
@@ -602,7 +646,7 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     }
     Chan<C> h, before[kRows];
     {
-        const float *saved = a.checkpoints + ((uint64_t)p.seq * a.tiles + p.tile) * a.channels + p.channel;
+        const float *saved = a.checkpoints + ((uint64_t)p.base + p.tile) * a.channels + p.channel;
 #pragma unroll
         for (int c = 0; c < C; ++c) h.v[c] = saved[c];
     }
@@ -692,6 +736,122 @@ __global__ __launch_bounds__(kStepThreads) void rec_step_kernel(StepArgs a)
     }
 }
 
+// ---------------------------------------------------------------- the list of packed tiles
+// A workgroup sorts kListSequences sequences by their tiles, c_0 >= c_1 >= ..: level k
+// of the walk (their tile k) has as many entries as sequences have more than k tiles, so
+// between c_{m+1} and c_m the levels have m + 1 each and an entry's level and sequence
+// follow from its position by one search and one division.  Levels of sequences that
+// come later in the tensors follow behind.  The sums over all sequences before these are
+// made anew by every workgroup.  The other workgroups of the launch clear the status
+// word and the look-back words.  Between events, which add some 4 us: for 24
+// sequences of 16391 rows x 1536 in all 7.0 us, for 256 of 262144 x 2048, the longest of
+// 32768, 14.6 (clearing the words of 256 sequences of that one's tiles took 220).
+constexpr int kListSequences = 256;
+struct ListArgs {
+    const uint32_t *begin, *end;
+    uint64_t rows;
+    uint32_t max_length, sequences, all, builders, slices;
+    PackedTile *list;
+    uint64_t *status, *words;
+    uint64_t count;  // words
+};
+__global__ __launch_bounds__(kListSequences) void rec_list_kernel(ListArgs a)
+{
+    constexpr uint32_t N = kListSequences;
+    __shared__ uint32_t s_tiles[N + 1], s_sorted[N + 1], s_from[N], s_row[N], s_len[N];
+    __shared__ uint64_t s_base[N + 1], s_start[N], s_wave[N / kWave], s_after[N + 1];
+    const uint32_t t = threadIdx.x, wave = t / kWave;
+    if (blockIdx.x >= a.builders) {
+        const uint64_t at = (uint64_t)(blockIdx.x - a.builders) * N + t, stride = (uint64_t)(gridDim.x - a.builders) * N;
+        if (at < kStatusBytes / 8) a.status[at] = 0;
+        for (uint64_t i = at; i < a.count; i += stride) a.words[i] = 0;
+        return;
+    }
+    const uint32_t block = blockIdx.x / a.slices, slice = blockIdx.x - block * a.slices, first = block * N;
+    const uint32_t n = a.sequences - first < N ? a.sequences - first : N;
+    auto tiles_of = [&](uint32_t seq, uint64_t &row, uint32_t &len) {
+        sequence_rows(a.begin, a.end, a.rows, a.max_length, seq, row, len);
+        return len ? (len + kTileRows - 1) / kTileRows : 1u;  // (an empty one's tile passes the state on)
+    };
+    uint64_t sum = 0;
+    for (uint32_t i = t; i < first; i += N) {
+        uint64_t row;
+        uint32_t len;
+        sum += tiles_of(i, row, len);
+    }
+    uint64_t row = 0;
+    uint32_t len = 0;
+    const uint32_t own = t < n ? tiles_of(first + t, row, len) : 0;
+    s_tiles[t] = own, s_row[t] = (uint32_t)row, s_len[t] = len;
+    // the sum over all sequences before these, and the sums over these up to each
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) sum += shfl_xor(sum, m);
+    uint64_t scan = own;
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+        const uint64_t up = shfl_up(scan, m);
+        scan += lane_id() >= (uint32_t)m ? up : 0;
+    }
+    if (lane_id() == kWave - 1) s_wave[wave] = sum, s_after[wave] = scan;
+    __syncthreads();
+    uint64_t before = 0, base = 0;
+    for (uint32_t w = 0; w < N / kWave; ++w) {
+        base += s_wave[w];
+        before += w < wave ? s_after[w] : 0;
+    }
+    s_base[t] = base + before + scan - own;
+    // place in the order of falling numbers of tiles
+    uint32_t place = 0;
+#pragma unroll 16
+    for (uint32_t j = 0; j < n; ++j) place += s_tiles[j] > own || (s_tiles[j] == own && j < t) ? 1 : 0;
+    __syncthreads();
+    if (t < n) s_sorted[place] = own, s_from[place] = t;
+    else s_sorted[t] = 0, s_from[t] = 0;
+    if (t == 0) s_sorted[N] = 0;
+    __syncthreads();
+    // s_after[m]: the sum of sorted numbers from m on
+    uint64_t rest = s_sorted[N - 1 - t];
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+        const uint64_t up = shfl_up(rest, m);
+        rest += lane_id() >= (uint32_t)m ? up : 0;
+    }
+    if (lane_id() == kWave - 1) s_wave[wave] = rest;
+    __syncthreads();
+    for (uint32_t w = 0; w < wave; ++w) rest += s_wave[w];
+    s_after[N - 1 - t] = rest;
+    if (t == 0) s_after[N] = 0;
+    __syncthreads();
+    // where the levels with t + 1 entries begin
+    s_start[t] = (uint64_t)(t + 1) * s_sorted[t + 1] + s_after[t + 1];
+    __syncthreads();
+    const uint64_t mine = s_after[0];
+    const uint32_t words_end = a.all - a.sequences;
+    for (uint64_t r = (uint64_t)slice * N + t; r < mine && base + r < a.all; r += (uint64_t)a.slices * N) {
+        uint32_t lo = 0, hi = n - 1;  // the smallest m whose levels begin at r or before
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (s_start[mid] <= r) hi = mid;
+            else lo = mid + 1;
+        }
+        const uint32_t at = (uint32_t)(r - s_start[lo]), level = at / (lo + 1), from = s_from[at - level * (lo + 1)];
+        PackedTile e = {};
+        e.seq = first + from, e.walk = s_sorted[lo + 1] + level, e.row = s_row[from], e.len = s_len[from];
+        // Disjoint sequences have no more tiles than `all`.  Tiles past that are left
+        // out, the later ones of a sequence with them, so that none waits for a tile
+        // that there is not and none writes past the words.
+        const uint64_t slot = s_base[from] + e.walk;
+        const bool fits = slot < a.all && (e.walk + 1 == s_tiles[from] || slot - e.seq < words_end) &&
+                          (e.walk == 0 || slot - 1 - e.seq < words_end);
+        e.base = (uint32_t)s_base[from];
+        if (!fits) e.seq = kNoSequence;
+        a.list[base + r] = e;
+    }
+    if (first + N >= a.sequences) {
+        for (uint64_t i = base + mine + (uint64_t)slice * N + t; i < a.all; i += (uint64_t)a.slices * N) a.list[i].seq = kNoSequence;
+    }
+}
+
 // ---------------------------------------------------------------- launches
 template <class F>
 int gate_dispatch(lcpp_gate g, F f)
@@ -708,38 +868,62 @@ int gate_dispatch(lcpp_gate g, F f)
 // 64 lanes cover the channels.
 uint32_t rec_lane_channels(uint64_t channels, size_t size) { return channels <= kWave || size == 4 ? 1 : 2; }
 struct RecShape {
-    uint64_t tiles, groups, words, run, turns;
+    uint64_t max_length, tiles, groups, run, turns;
+    uint64_t all, grid, words;  // tiles of all sequences, workgroups, look-back words
+    bool list;                  // packed, of several tiles
 };
-void rec_dealing(uint64_t sequences, bool offsets, RecShape *r)
-{
-    const uint64_t chains = sequences * r->groups;
-    r->run = chains < kXcds ? 0 : ceil_div(chains, kXcds);
-    if (offsets) r->run = std::min<uint64_t>(r->run, 4);
-    r->turns = r->run ? align_up(ceil_div(chains, r->run), kXcds) * r->run : chains;
-}
-bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t size, bool offsets, RecShape *r)
+// `packed`: with offsets, of `rows` rows.
+bool rec_shape(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t size, bool packed, uint64_t rows, RecShape *r)
 {
     if (sequences > 0xFFFFFFFFull || max_length > 0x7FFFFFFFull || channels > kMaxCols) return false;
     const uint64_t lanes = kWave * rec_lane_channels(channels, size);
+    r->max_length = packed ? std::min(max_length, rows) : max_length;
     r->groups = ceil_div(channels, lanes);
-    r->tiles = std::max<uint64_t>(ceil_div(max_length, kTileRows), 1);
+    r->tiles = std::max<uint64_t>(ceil_div(r->max_length, kTileRows), 1);
+    r->list = packed && r->tiles > 1;
     // workgroups are numbered in 32 bits, and a launch has less than 2^32 threads
     const uint64_t most = 0xFFFFFFFFull / (kWaves * kWave);
     if (r->groups && sequences > most / r->groups) return false;
-    rec_dealing(sequences, offsets, r);
+    const uint64_t chains = sequences * r->groups;
+    r->run = chains < kXcds ? 0 : ceil_div(chains, kXcds);
+    if (packed) r->run = std::min<uint64_t>(r->run, 4);
+    r->all = sequences * r->tiles;
+    if (r->list) {
+        r->all = std::min(r->all, rows / kTileRows + sequences);
+        if (r->groups && r->all > most / r->groups) return false;
+        r->turns = 0;
+        r->grid = r->run ? align_up(r->all * r->groups, kXcds * r->run) : r->all * r->groups;
+        r->words = (r->all - sequences) * r->groups * lanes;
+        return r->grid <= most;
+    }
+    r->turns = r->run ? align_up(ceil_div(chains, r->run), kXcds) * r->run : chains;
     if (r->turns && r->tiles > most / r->turns) return false;
-    r->words = r->tiles > 1 ? sequences * r->tiles * r->groups * lanes : 0;
+    r->grid = r->tiles * r->turns;
+    r->words = r->tiles > 1 ? r->all * r->groups * lanes : 0;
     return true;
 }
+uint64_t rec_list_bytes(const RecShape &r) { return r.list ? align_up(r.all * sizeof(PackedTile), 256) : 0; }
 uint64_t rec_temp_bytes(const RecShape &r)
 {
-    return r.words ? kStatusBytes + align_up(r.words * sizeof(uint64_t), 256) : 0;
+    return r.tiles > 1 ? kStatusBytes + rec_list_bytes(r) + align_up(r.words * sizeof(uint64_t), 256) : 0;
+}
+// The larger of the types' sizes, of those whose call can be launched (2-byte types have
+// half the workgroups), or false.
+bool rec_most_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, bool packed, uint64_t rows, uint64_t *most)
+{
+    bool any = false;
+    for (size_t size : {2, 4}) {
+        RecShape r;
+        if (!rec_shape(sequences, max_length, channels, size, packed, rows, &r)) continue;
+        any = true;
+        *most = std::max(*most, rec_temp_bytes(r));
+    }
+    return any;
 }
 
 template <class T, class G, int C, int W, bool STREAM>
-int rec_launch_waves(bool forward, const RecArgs &a, hipStream_t s)
+int rec_launch_waves(bool forward, const RecArgs &a, uint32_t grid, hipStream_t s)
 {
-    const uint32_t grid = a.tiles * a.turns;
     if (forward) LCPP_LAUNCH("recurrence_forward", s, rec_forward_kernel<T, G, C, W, STREAM><<<grid, W * kWave, 0, s>>>(a));
     else LCPP_LAUNCH("recurrence_backward", s, rec_backward_kernel<T, G, C, W, STREAM><<<grid, W * kWave, 0, s>>>(a));
     LCPP_CHECK_LAUNCH();
@@ -747,10 +931,10 @@ int rec_launch_waves(bool forward, const RecArgs &a, hipStream_t s)
 }
 // Sequences of one tile take no more waves than have rows.
 template <class T, class G, int C>
-int rec_launch(bool forward, const RecArgs &a, hipStream_t s)
+int rec_launch(bool forward, const RecArgs &a, uint32_t grid, hipStream_t s)
 {
-    if (a.max_length <= kRows) return rec_launch_waves<T, G, C, 1, false>(forward, a, s);
-    if (a.max_length <= 4 * kRows) return rec_launch_waves<T, G, C, 4, false>(forward, a, s);
+    if (a.max_length <= kRows) return rec_launch_waves<T, G, C, 1, false>(forward, a, grid, s);
+    if (a.max_length <= 4 * kRows) return rec_launch_waves<T, G, C, 4, false>(forward, a, grid, s);
     constexpr uint64_t kLine = 128;
     auto lined = [](const void *p, uint64_t row, uint64_t seq) {
         return (reinterpret_cast<uintptr_t>(p) | row * sizeof(T) | seq * sizeof(T)) % kLine == 0;
@@ -759,8 +943,8 @@ int rec_launch(bool forward, const RecArgs &a, hipStream_t s)
     auto out = [&](const RowsOut &t) { return lined(t.p, t.row, t.seq); };
     // (sequences with offsets begin at whole rows; the tensors that a pass does not have are null)
     if (a.channels % C == 0 && in(a.gate) && in(a.in) && in(a.grad_out) && out(a.out) && out(a.grad_gate) && out(a.grad_in))
-        return rec_launch_waves<T, G, C, kWaves, true>(forward, a, s);
-    return rec_launch_waves<T, G, C, kWaves, false>(forward, a, s);
+        return rec_launch_waves<T, G, C, kWaves, true>(forward, a, grid, s);
+    return rec_launch_waves<T, G, C, kWaves, false>(forward, a, grid, s);
 }
 
 int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_bytes, RecArgs &a, uint64_t sequences,
@@ -770,7 +954,7 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
     if (!e) return LCPP_ERR_UNSUPPORTED_DTYPE;
     if (g != LCPP_GATE_DECAY && g != LCPP_GATE_LOG && g != LCPP_GATE_SIGMOID) return LCPP_ERR_INVALID_ARG;
     RecShape r;
-    if (!rec_shape(sequences, max_length, channels, e, a.begin != nullptr, &r) || (!a.begin) != (!a.end)) return LCPP_ERR_INVALID_ARG;
+    if (!rec_shape(sequences, max_length, channels, e, a.begin != nullptr, rows, &r) || (!a.begin) != (!a.end)) return LCPP_ERR_INVALID_ARG;
     if (sequences == 0 || channels == 0) return LCPP_OK;
     if (a.begin && (!elem_ok(a.begin, 4) || !elem_ok(a.end, 4))) return LCPP_ERR_INVALID_ARG;
     auto optional = [](const void *p) { return !p || elem_ok(p, 4); };
@@ -788,31 +972,41 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
         if (forward ? !out_ok(a.out) : !(elem_ok(a.grad_out.p, e) && out_ok(a.grad_gate) && out_ok(a.grad_in) && a.checkpoints))
             return LCPP_ERR_INVALID_ARG;
     }
-    if (r.words) {
-        if (temp_bytes < rec_temp_bytes(r)) return LCPP_ERR_TEMP_TOO_SMALL;
+    const uint64_t need = rec_temp_bytes(r);
+    if (need) {
+        if (temp_bytes < need) return LCPP_ERR_TEMP_TOO_SMALL;
         if (!temp || (reinterpret_cast<uintptr_t>(temp) & 255)) return LCPP_ERR_INVALID_ARG;
     }
-    a.run = (uint32_t)r.run, a.turns = (uint32_t)r.turns;
+    a.run = (uint32_t)r.run, a.turns = (uint32_t)r.turns, a.all = (uint32_t)r.all;
     a.sequences = (uint32_t)sequences, a.tiles = (uint32_t)r.tiles, a.groups = (uint32_t)r.groups;
-    a.channels = (uint32_t)channels, a.max_length = some ? (uint32_t)max_length : 0, a.rows = rows;
+    a.channels = (uint32_t)channels, a.max_length = some ? (uint32_t)r.max_length : 0, a.rows = rows;
     if (a.begin) a.gate.seq = a.in.seq = a.grad_out.seq = a.out.seq = a.grad_gate.seq = a.grad_in.seq = 0;
-    uint64_t *head = static_cast<uint64_t *>(temp);
-    if (r.words) {
-        a.words = head + kStatusBytes / 8;
-        a.ctl = wait_ctl(static_cast<uint32_t *>(temp));
-        const int rc = lb_init(head, kStatusBytes / 8 + r.words, s, "recurrence_init");
+    char *head = static_cast<char *>(temp);
+    a.ctl = wait_ctl(need ? static_cast<uint32_t *>(temp) : nullptr);  // (one tile a sequence: nothing waits)
+    if (need) a.words = reinterpret_cast<uint64_t *>(head + kStatusBytes + rec_list_bytes(r));
+    if (r.list) {
+        ListArgs l = {a.begin, a.end, rows, a.max_length, a.sequences, a.all, 0, 0, nullptr, nullptr, a.words, r.words};
+        l.list = reinterpret_cast<PackedTile *>(head + kStatusBytes), l.status = reinterpret_cast<uint64_t *>(head);
+        a.list = l.list;
+        const uint64_t blocks = ceil_div(sequences, kListSequences);
+        l.slices = (uint32_t)std::min<uint64_t>(ceil_div(r.all, blocks * kListSequences), 16);
+        l.builders = (uint32_t)blocks * l.slices;
+        const uint32_t grid = l.builders + (uint32_t)std::min<uint64_t>(ceil_div(r.words, kListSequences) + 1, 1024);
+        LCPP_LAUNCH("recurrence_init", s, rec_list_kernel<<<grid, kListSequences, 0, s>>>(l));
+        LCPP_CHECK_LAUNCH();
+    } else if (need) {
+        const int rc = lb_init(static_cast<uint64_t *>(temp), kStatusBytes / 8 + r.words, s, "recurrence_init");
         if (rc != LCPP_OK) return rc;
-    } else {
-        a.ctl = wait_ctl(nullptr);  // one tile a sequence: nothing waits
     }
+    const uint32_t grid = (uint32_t)r.grid;
     return float_dispatch(t, [&](auto x) -> int {
         using T = decltype(x);
         return gate_dispatch(g, [&](auto gate) -> int {
             using G = decltype(gate);
             if constexpr (sizeof(T) == 2) {
-                if (rec_lane_channels(channels, sizeof(T)) == 2) return rec_launch<T, G, 2>(forward, a, s);
+                if (rec_lane_channels(channels, sizeof(T)) == 2) return rec_launch<T, G, 2>(forward, a, grid, s);
             }
-            return rec_launch<T, G, 1>(forward, a, s);
+            return rec_launch<T, G, 1>(forward, a, grid, s);
         });
     });
 }
@@ -825,16 +1019,19 @@ using namespace lcpp;
 extern "C" int lcpp_recurrence_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, size_t *bytes)
 {
     if (!bytes) return LCPP_ERR_INVALID_ARG;
-    // the larger of the types' sizes, of those whose call can be launched (2-byte types have half the workgroups)
-    bool any = false;
     uint64_t most = 0;
-    for (size_t size : {2, 4}) {
-        RecShape r;
-        if (!rec_shape(sequences, max_length, channels, size, false, &r)) continue;
-        any = true;
-        most = std::max(most, rec_temp_bytes(r));
-    }
-    if (!any) return LCPP_ERR_INVALID_ARG;
+    const bool fixed = rec_most_bytes(sequences, max_length, channels, false, 0, &most);
+    const bool packed = rec_most_bytes(sequences, max_length, channels, true, ~0ull, &most);
+    if (!fixed && !packed) return LCPP_ERR_INVALID_ARG;
+    *bytes = most;
+    return LCPP_OK;
+}
+
+extern "C" int lcpp_recurrence_packed_temp_bytes(uint64_t sequences, uint64_t max_length, uint64_t channels, uint64_t rows,
+                                                 size_t *bytes)
+{
+    uint64_t most = 0;
+    if (!bytes || !rec_most_bytes(sequences, max_length, channels, true, rows, &most)) return LCPP_ERR_INVALID_ARG;
     *bytes = most;
     return LCPP_OK;
 }
@@ -843,6 +1040,14 @@ extern "C" int lcpp_recurrence_checkpoint_rows(uint64_t max_length, uint64_t *ro
 {
     if (!rows || max_length > 0x7FFFFFFFull) return LCPP_ERR_INVALID_ARG;
     *rows = std::max<uint64_t>(ceil_div(max_length, kTileRows), 1);
+    return LCPP_OK;
+}
+
+extern "C" int lcpp_recurrence_packed_checkpoint_rows(uint64_t sequences, uint64_t max_length, uint64_t rows, uint64_t *out)
+{
+    RecShape r;
+    if (!out || !rec_shape(sequences, max_length, 1, 2, true, rows, &r)) return LCPP_ERR_INVALID_ARG;
+    *out = r.all;
     return LCPP_OK;
 }
 

@@ -243,6 +243,23 @@ def _checkpoint_rows(max_length: int) -> int:
     return out.value
 
 
+@functools.lru_cache(maxsize=1024)
+def _packed_checkpoint_rows(sequences: int, max_length: int, rows: int) -> int:
+    out = ctypes.c_uint64()
+    check(lib().lcpp_recurrence_packed_checkpoint_rows(sequences, max_length, rows, ctypes.byref(out)),
+          "lcpp_recurrence_packed_checkpoint_rows")
+    return out.value
+
+
+def _checkpoints(t, sizes):
+    """The address of the checkpoints of a call of these sizes (DeviceGatedRecurrence._sizes), or None."""
+    if t is None:
+        return None
+    n, max_length, channels, begin, _, rows = sizes
+    held = n * _checkpoint_rows(max_length) if begin is None else _packed_checkpoint_rows(n, max_length, rows)
+    return _float_vector(t, held * channels, "d_checkpoints")
+
+
 class DeviceGatedRecurrence(_BlockModule):
     """h_t = a_t h_{t-1} + b_t per channel, with a and b from a gate g and an input x:
 
@@ -255,13 +272,22 @@ class DeviceGatedRecurrence(_BlockModule):
     there).  States are float32 of shape (sequences, channels)."""
 
     @staticmethod
-    def GetTempStorageBytes(sequences: int, max_length: int, channels: int) -> int:
-        return _query(lib().lcpp_recurrence_temp_bytes, sequences, max_length, channels)
+    def GetTempStorageBytes(sequences: int, max_length: int, channels: int, rows: int | None = None) -> int:
+        """For sequences of max_length each; with `rows`, for packed ones of that many rows in all, which need far less
+        where their lengths differ."""
+        if rows is None:
+            return _query(lib().lcpp_recurrence_temp_bytes, sequences, max_length, channels)
+        return _query(lib().lcpp_recurrence_packed_temp_bytes, sequences, max_length, channels, rows)
 
     @staticmethod
     def GetCheckpointRows(max_length: int) -> int:
         """d_checkpoints has shape (sequences, this, channels), float32."""
         return _checkpoint_rows(max_length)
+
+    @staticmethod
+    def GetPackedCheckpointRows(sequences: int, max_length: int, rows: int) -> int:
+        """With offsets, d_checkpoints of shape (this, channels) is enough."""
+        return _packed_checkpoint_rows(sequences, max_length, rows)
 
     @staticmethod
     def _gate(gate):
@@ -298,13 +324,11 @@ class DeviceGatedRecurrence(_BlockModule):
         shape, dtype, kind = d_in.shape, d_in.dtype, self._gate(gate)
         sizes = self._sizes(shape, d_begin_offsets, d_end_offsets, max_length)
         states = sizes[0] * sizes[2]
-        saved = None
-        if d_checkpoints is not None:
-            saved = _float_vector(d_checkpoints, states * _checkpoint_rows(sizes[1]), "d_checkpoints")
         self._call("lcpp_recurrence_forward", temp_storage, _stream(stream), float_code(dtype), kind, _ptr(temp_storage),
                    _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
                    *_sequence_strides(d_in, shape, dtype, "d_in"), *_sequence_strides(d_out, shape, dtype, "d_out", True),
-                   _float_vector(d_initial, states, "d_initial"), _float_vector(d_final, states, "d_final"), saved, *sizes)
+                   _float_vector(d_initial, states, "d_initial"), _float_vector(d_final, states, "d_final"),
+                   _checkpoints(d_checkpoints, sizes), *sizes)
 
     def Backward(self, temp_storage, d_gate, d_in, d_checkpoints, d_grad_out, d_grad_gate, d_grad_in, gate: str,
                  d_grad_final=None, d_grad_initial=None, d_begin_offsets=None, d_end_offsets=None, max_length=None,
@@ -316,7 +340,7 @@ class DeviceGatedRecurrence(_BlockModule):
         self._call("lcpp_recurrence_backward", temp_storage, _stream(stream), float_code(dtype), kind, _ptr(temp_storage),
                    _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
                    *_sequence_strides(d_in, shape, dtype, "d_in"),
-                   _float_vector(d_checkpoints, states * _checkpoint_rows(sizes[1]), "d_checkpoints"),
+                   _checkpoints(d_checkpoints, sizes),
                    *_sequence_strides(d_grad_out, shape, dtype, "d_grad_out"),
                    *_sequence_strides(d_grad_gate, shape, dtype, "d_grad_gate", True),
                    *_sequence_strides(d_grad_in, shape, dtype, "d_grad_in", True),
