@@ -705,7 +705,8 @@ class DeviceGatedRecurrence : public LuisaModule {
                                       d_in.sequence_stride, d_out.data(), d_out.stride, d_out.sequence_stride, d_initial,
                                       d_final, d_checkpoints, seq.count, seq.length, seq.channels, seq.d_begin, seq.d_end,
                                       seq.rows, cmdlist.stream),
-              "DeviceGatedRecurrence::Forward", cmdlist.stream, temp_storage);
+              "DeviceGatedRecurrence::Forward", cmdlist.stream,
+              seq.count && seq.channels ? temp_storage : BufferView<uint>{});
     }
     template <class T>
     void Backward(CommandList &cmdlist, BufferView<uint> temp_storage, lcpp_gate gate, RowsView<T> d_gate, RowsView<T> d_in,
@@ -719,7 +720,8 @@ class DeviceGatedRecurrence : public LuisaModule {
                                        d_grad_gate.sequence_stride, d_grad_in.data(), d_grad_in.stride,
                                        d_grad_in.sequence_stride, d_grad_final, d_grad_initial, seq.count, seq.length,
                                        seq.channels, seq.d_begin, seq.d_end, seq.rows, cmdlist.stream),
-              "DeviceGatedRecurrence::Backward", cmdlist.stream, temp_storage);
+              "DeviceGatedRecurrence::Backward", cmdlist.stream,
+              seq.count && seq.channels ? temp_storage : BufferView<uint>{});
     }
     /* d_slots null: sequence s has the state of row s */
     template <class T>

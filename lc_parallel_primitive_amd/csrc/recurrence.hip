@@ -77,6 +77,7 @@ struct RecArgs {
     uint32_t all;
     uint64_t *words;                       // [sequence][tile of the walk][group][lane's channels]
     WaitCtl ctl;
+    uint32_t *status;  // of temp storage that the call does not need, cleared by the kernel (may be null)
 };
 
 // ---------------------------------------------------------------- gates
@@ -448,6 +449,7 @@ __global__ __launch_bounds__(W *kWave) __attribute__((amdgpu_waves_per_eu(4))) v
     __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_carry[kWave];
     constexpr bool kWalks = W == kWaves;  // (sequences of one tile have fewer waves)
     __shared__ Words<C> s_back[kWalks ? kBack<C> : 1][kWave];
+    if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
     Place p;
     if (!find_place<C>(a, false, p)) return;
     const uint32_t wave = wave_id(), lane = lane_id();
@@ -566,6 +568,7 @@ __global__ __launch_bounds__(W *kWave) void rec_backward_kernel(RecArgs a)
     __shared__ Chan<C> s_A[W][kWave], s_H[W][kWave], s_E[W][kWave], s_carry[kWave];
     constexpr bool kWalks = W == kWaves;  // (sequences of one tile have fewer waves)
     __shared__ Words<C> s_back[kWalks ? kBack<C> : 1][kWave];
+    if (a.status && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
     Place p;
     if (!find_place<C>(a, true, p)) return;
     const uint32_t wave = wave_id(), lane = lane_id();
@@ -983,6 +986,8 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
     if (a.begin) a.gate.seq = a.in.seq = a.grad_out.seq = a.out.seq = a.grad_gate.seq = a.grad_in.seq = 0;
     char *head = static_cast<char *>(temp);
     a.ctl = wait_ctl(need ? static_cast<uint32_t *>(temp) : nullptr);  // (one tile a sequence: nothing waits)
+    if (!need && temp && temp_bytes >= kStatusBytes && !(reinterpret_cast<uintptr_t>(temp) & 255))
+        a.status = static_cast<uint32_t *>(temp);
     if (need) a.words = reinterpret_cast<uint64_t *>(head + kStatusBytes + rec_list_bytes(r));
     if (r.list) {
         ListArgs l = {a.begin, a.end, rows, a.max_length, a.sequences, a.all, 0, 0, nullptr, nullptr, a.words, r.words};

@@ -324,8 +324,9 @@ class DeviceGatedRecurrence(_BlockModule):
         shape, dtype, kind = d_in.shape, d_in.dtype, self._gate(gate)
         sizes = self._sizes(shape, d_begin_offsets, d_end_offsets, max_length)
         states = sizes[0] * sizes[2]
-        self._call("lcpp_recurrence_forward", temp_storage, _stream(stream), float_code(dtype), kind, _ptr(temp_storage),
-                   _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+        # (a call without states launches nothing and leaves the status word)
+        self._call("lcpp_recurrence_forward", temp_storage if states else None, _stream(stream), float_code(dtype), kind,
+                   _ptr(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
                    *_sequence_strides(d_in, shape, dtype, "d_in"), *_sequence_strides(d_out, shape, dtype, "d_out", True),
                    _float_vector(d_initial, states, "d_initial"), _float_vector(d_final, states, "d_final"),
                    _checkpoints(d_checkpoints, sizes), *sizes)
@@ -337,8 +338,9 @@ class DeviceGatedRecurrence(_BlockModule):
         shape, dtype, kind = d_in.shape, d_in.dtype, self._gate(gate)
         sizes = self._sizes(shape, d_begin_offsets, d_end_offsets, max_length)
         states = sizes[0] * sizes[2]
-        self._call("lcpp_recurrence_backward", temp_storage, _stream(stream), float_code(dtype), kind, _ptr(temp_storage),
-                   _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+        # (a call without states launches nothing and leaves the status word)
+        self._call("lcpp_recurrence_backward", temp_storage if states else None, _stream(stream), float_code(dtype), kind,
+                   _ptr(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
                    *_sequence_strides(d_in, shape, dtype, "d_in"),
                    _checkpoints(d_checkpoints, sizes),
                    *_sequence_strides(d_grad_out, shape, dtype, "d_grad_out"),
