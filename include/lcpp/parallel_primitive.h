@@ -623,7 +623,8 @@ class DeviceLayerNorm : public LuisaModule {
                                        temp_storage.size_bytes(), d_grad_out.data(), d_grad_out.stride, d_in.data(),
                                        d_in.stride, d_weight, d_mean, d_rstd, d_grad_in.data(), d_grad_in.stride,
                                        d_grad_weight, d_grad_bias, rows, cols, cmdlist.stream),
-              "DeviceLayerNorm::Backward", cmdlist.stream, temp_storage);
+              "DeviceLayerNorm::Backward", cmdlist.stream,
+              cols && (rows || d_grad_weight || d_grad_bias) ? temp_storage : BufferView<uint>{});
     }
     template <class T, class W>
     void AddBackward(CommandList &cmdlist, BufferView<uint> temp_storage, RowsView<T> d_grad_out, RowsView<T> d_grad_sum,
@@ -637,7 +638,8 @@ class DeviceLayerNorm : public LuisaModule {
                                            d_rstd, drop.p, drop.seed, drop.offset, drop.d_offset, d_grad_residual.data(),
                                            d_grad_residual.stride, d_grad_in.data(), d_grad_in.stride, d_grad_weight,
                                            d_grad_bias, rows, cols, cmdlist.stream),
-              "DeviceLayerNorm::AddBackward", cmdlist.stream, temp_storage);
+              "DeviceLayerNorm::AddBackward", cmdlist.stream,
+              cols && (rows || d_grad_weight || d_grad_bias) ? temp_storage : BufferView<uint>{});
     }
 };
 

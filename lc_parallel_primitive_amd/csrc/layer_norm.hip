@@ -862,8 +862,9 @@ int norm_backward_launch(const NormGradArgs &a, W *grad_weight, W *grad_bias, hi
 }
 
 template <class W>
-__global__ void norm_zero_kernel(W *x, W *y, uint32_t n)
+__global__ void norm_zero_kernel(W *x, W *y, uint32_t n, uint32_t *status)
 {
+    if (status && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
     for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
         if (x) x[i] = (W)0.0f;
         if (y) y[i] = (W)0.0f;
@@ -912,14 +913,15 @@ int norm_backward(lcpp_dtype t, lcpp_dtype wt, bool add, void *temp, size_t temp
     if (rows > kMaxRows || cols > kMaxCols) return LCPP_ERR_INVALID_ARG;
     if (cols == 0) return LCPP_OK;
     if (!norm_pointer(grad_weight, we, false) || !norm_pointer(grad_bias, we, false)) return LCPP_ERR_INVALID_ARG;
+    if (temp && temp_bytes >= kStatusBytes && !(reinterpret_cast<uintptr_t>(temp) & 255))
+        a.status = static_cast<uint32_t *>(temp);
     if (rows == 0) {  // sums over no rows
         if (!grad_weight && !grad_bias) return LCPP_OK;
-        // (the temp query is 0 for no rows: temp holds no status word)
         return norm_dispatch(t, wt, [&](auto, auto w) -> int {
             using W = decltype(w);
             LCPP_LAUNCH("layer_norm_zero", s,
                         norm_zero_kernel<W><<<(uint32_t)std::min<uint64_t>(ceil_div(cols, 256), 1024), 256, 0, s>>>(
-                            static_cast<W *>(grad_weight), static_cast<W *>(grad_bias), (uint32_t)cols));
+                            static_cast<W *>(grad_weight), static_cast<W *>(grad_bias), (uint32_t)cols, a.status));
             LCPP_CHECK_LAUNCH();
             return LCPP_OK;
         });
@@ -935,8 +937,6 @@ int norm_backward(lcpp_dtype t, lcpp_dtype wt, bool add, void *temp, size_t temp
         if (!temp || (reinterpret_cast<uintptr_t>(temp) & 255)) return LCPP_ERR_INVALID_ARG;
         a.partial = reinterpret_cast<float *>(static_cast<char *>(temp) + kStatusBytes);
     }
-    if (temp && temp_bytes >= kStatusBytes && !(reinterpret_cast<uintptr_t>(temp) & 255))
-        a.status = static_cast<uint32_t *>(temp);
     return norm_dispatch(t, wt, [&](auto x, auto w) -> int {
         using T = decltype(x);
         using W = decltype(w);

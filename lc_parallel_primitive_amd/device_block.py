@@ -173,7 +173,9 @@ class DeviceLayerNorm(_BlockModule):
         """The gradients of Forward's d_in, d_weight and d_bias (the latter two None if not wanted)."""
         shape, dtype, code, rows, cols, si, so = _in_out(d_in, d_grad_in, "d_in", "d_grad_in")
         sg = _like(d_grad_out, shape, dtype, "d_grad_out")
-        self._call("lcpp_layer_norm_backward", temp_storage, _stream(stream), code,
+        # (a call without columns, or without rows and weights' gradients, launches nothing and leaves the status word)
+        used = cols and (rows or d_grad_weight is not None or d_grad_bias is not None)
+        self._call("lcpp_layer_norm_backward", temp_storage if used else None, _stream(stream), code,
                    _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
                    d_grad_out.data_ptr(), sg, d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
                    _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), d_grad_in.data_ptr(), so,
@@ -192,7 +194,9 @@ class DeviceLayerNorm(_BlockModule):
         sx = 0 if d_grad_sum is None else _like(d_grad_sum, shape, dtype, "d_grad_sum")
         sr = 0 if d_grad_residual is None else _like_out(d_grad_residual, shape, dtype, "d_grad_residual")
         si = 0 if d_grad_in is None else _like_out(d_grad_in, shape, dtype, "d_grad_in")
-        self._call("lcpp_layer_norm_add_backward", temp_storage, _stream(stream), code,
+        # (a call without columns, or without rows and weights' gradients, launches nothing and leaves the status word)
+        used = cols and (rows or d_grad_weight is not None or d_grad_bias is not None)
+        self._call("lcpp_layer_norm_add_backward", temp_storage if used else None, _stream(stream), code,
                    _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
                    d_grad_out.data_ptr(), sg, _ptr(d_grad_sum), sx, d_sum.data_ptr(), ss,
                    _vector(d_weight, cols, "d_weight"), _float_vector(d_mean, rows, "d_mean"),

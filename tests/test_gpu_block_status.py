@@ -50,3 +50,29 @@ def test_recurrences_of_nothing(lcpp):
         saved = torch.zeros(shape[0], 3, shape[2], device="cuda")
         m.Forward(stale(), x, x, x.clone(), "sigmoid", d_checkpoints=saved)
         m.Backward(stale(), x, x, saved, x, x.clone(), x.clone(), "sigmoid")
+
+
+def test_layer_norm_gradients_over_no_rows(lcpp):
+    log("layer norm of no rows on a stale workspace")
+    m = lcpp.DeviceLayerNorm().create(debug_stream=torch.cuda.current_stream())
+    w = torch.ones(50, device="cuda")
+    x, stat = torch.empty(0, 50, device="cuda"), torch.empty(0, device="cuda")
+    for dw, db in ((w.clone(), w.clone()), (w.clone(), None), (None, w.clone())):
+        temp = stale()
+        m.Backward(temp, x, x, w, stat, stat, x.clone(), dw, db)
+        assert int(temp[:4].view(torch.int32)[0]) == 0
+        temp = stale()
+        m.AddBackward(temp, x, None, x, w, stat, stat, x.clone(), x.clone(), dw, db)
+        assert int(temp[:4].view(torch.int32)[0]) == 0
+        assert not any(bool(v.any()) for v in (dw, db) if v is not None)
+
+
+def test_layer_norm_gradients_of_nothing(lcpp):
+    log("layer norm of no columns on a stale workspace")
+    m = lcpp.DeviceLayerNorm().create(debug_stream=torch.cuda.current_stream())
+    x, stat = torch.empty(0, 50, device="cuda"), torch.empty(0, device="cuda")
+    m.Backward(stale(), x, x, None, stat, stat, x.clone())
+    m.AddBackward(stale(), x, None, x, None, stat, stat, x.clone(), x.clone())
+    x, w, stat = torch.empty(4, 0, device="cuda"), torch.empty(0, device="cuda"), torch.ones(4, device="cuda")
+    m.Backward(stale(), x, x, w, stat, stat, x.clone(), w.clone(), w.clone())
+    m.AddBackward(stale(), x, None, x, w, stat, stat, x.clone(), x.clone(), w.clone(), w.clone())
