@@ -362,7 +362,8 @@ int lcpp_segment_reduce_argmax_fixed(lcpp_dtype t, void *temp, size_t temp_bytes
  * columns; *_stride is the distance between rows in elements, of any size for
  * inputs (0 repeats a row) and at least cols for outputs.  Pointers need the
  * alignment of one element only.  Outputs may lie exactly in the place of an
- * input of the same type and stride (but `sum` not in that of `out`); other
+ * input of the same type and stride; two outputs that begin at one place are
+ * refused (but the two row gradients without dropout, which are the same), other
  * overlaps give wrong results.  rows < 2^32, cols <= 2^30.
  * ------------------------------------------------------------------- */
 /* out[r] = (in[r] - mean) * rstd * weight + bias with each row's mean and rstd = 1 / sqrt(var +

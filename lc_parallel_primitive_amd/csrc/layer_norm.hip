@@ -898,6 +898,7 @@ int norm_forward(lcpp_dtype t, lcpp_dtype wt, bool add, const NormArgs &a, uint6
     if (!(a.eps >= 0.0f)) return LCPP_ERR_INVALID_ARG;
     if (add && (!elem_ok(a.residual, e) || !elem_ok(a.sum, e) || !rows_apart(a.sum_stride, rows, cols)))
         return LCPP_ERR_INVALID_ARG;
+    if (same_place(a.mean, a.rstd) || (add && same_place(a.sum, a.out))) return LCPP_ERR_INVALID_ARG;
     return norm_dispatch(t, wt, [&](auto x, auto w) -> int {
         using T = decltype(x);
         using W = decltype(w);
@@ -937,6 +938,8 @@ int norm_backward(lcpp_dtype t, lcpp_dtype wt, bool add, void *temp, size_t temp
         if (!temp || (reinterpret_cast<uintptr_t>(temp) & 255)) return LCPP_ERR_INVALID_ARG;
         a.partial = reinterpret_cast<float *>(static_cast<char *>(temp) + kStatusBytes);
     }
+    // (without dropout the two gradients of rows are the same)
+    if (same_place(grad_weight, grad_bias) || (a.drop.cut && same_place(a.grad_in, a.grad_branch))) return LCPP_ERR_INVALID_ARG;
     return norm_dispatch(t, wt, [&](auto x, auto w) -> int {
         using T = decltype(x);
         using W = decltype(w);

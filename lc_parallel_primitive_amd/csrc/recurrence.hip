@@ -974,6 +974,7 @@ int rec_run(bool forward, lcpp_dtype t, lcpp_gate g, void *temp, size_t temp_byt
         if (!elem_ok(a.gate.p, e) || !elem_ok(a.in.p, e)) return LCPP_ERR_INVALID_ARG;
         if (forward ? !out_ok(a.out) : !(elem_ok(a.grad_out.p, e) && out_ok(a.grad_gate) && out_ok(a.grad_in) && a.checkpoints))
             return LCPP_ERR_INVALID_ARG;
+        if (!forward && same_place(a.grad_gate.p, a.grad_in.p)) return LCPP_ERR_INVALID_ARG;
     }
     const uint64_t need = rec_temp_bytes(r);
     if (need) {

@@ -190,6 +190,8 @@ int float_dispatch(lcpp_dtype t, F f)
 }
 // A pointer that is not null and aligned to one element.
 inline bool elem_ok(const void *p, size_t size) { return p && reinterpret_cast<uintptr_t>(p) % size == 0; }
+// Two outputs in one place: one of them would be lost.
+inline bool same_place(const void *p, const void *q) { return p && p == q; }
 // Rows that do not overlap, as every output's have to be.
 inline bool rows_apart(uint64_t stride, uint64_t rows, uint64_t cols) { return rows <= 1 || stride >= cols; }
 

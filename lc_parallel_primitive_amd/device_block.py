@@ -155,8 +155,8 @@ class DeviceLayerNorm(_BlockModule):
 
     def AddForward(self, d_in, d_residual, d_sum, d_out, d_weight=None, d_bias=None, eps: float = 1e-5, d_mean=None,
                    d_rstd=None, p: float = 0.0, seed: int = 0, offset: int = 0, d_offset=None, stream=None):
-        """d_sum = d_residual + dropout(d_in), d_out = the layer norm of d_sum as it is stored.  p, seed, offset,
-        d_offset as DeviceDropout.Forward."""
+        """d_sum = d_residual + dropout(d_in), d_out = the layer norm of d_sum as it is stored; d_sum may be d_residual
+        or d_in, but not d_out.  p, seed, offset, d_offset as DeviceDropout.Forward."""
         dtype = d_in.dtype
         code = float_code(dtype)
         shape, rows, cols, si = _matrix(d_in, "d_in")
