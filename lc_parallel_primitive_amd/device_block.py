@@ -10,7 +10,8 @@ Activations and their gradients are float32, bfloat16 or float16; weights are
 of the same type or float32; statistics and recurrent states are float32.
 Everything is computed in 32 bits and rounded once when it is stored.  Sizes
 are those of the tensors.  Rows need unit stride along their last dimension
-and may lie any distance apart.
+and may lie any distance apart.  A tensor that is not on the GPU is refused
+(ValueError): its address would fault there.
 
     norm, mix, drop = DeviceLayerNorm(), DeviceGatedRecurrence(), DeviceDropout()
     norm.AddForward(d_mixed, d_residual, d_residual_out, d_normed, weight, bias, 1e-5, mean, rstd, p=0.1, seed=7)
@@ -30,8 +31,14 @@ from .device import _Module, _nbytes, _ptr, _query, _stream
 # functions of their own, and the common layouts are checked first.
 
 
+def _off_gpu(t, what: str):
+    raise ValueError(f"{what}: must be on the GPU, got a tensor on {t.device}")
+
+
 def _matrix(t, what: str):
     """(shape, rows, columns, row stride) of a tensor whose last dimension has unit stride."""
+    if not t.is_cuda:
+        _off_gpu(t, what)
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
         if stride[1] == 1 or shape[1] <= 1:
@@ -53,6 +60,8 @@ def _like(t, shape, dtype, what: str):
     """The row stride of a tensor that must have this shape and type."""
     if t.shape != shape or t.dtype != dtype:
         _unlike(t, shape, dtype, what)
+    if not t.is_cuda:
+        _off_gpu(t, what)
     stride = t.stride()
     if len(stride) == 2 and (stride[1] == 1 or shape[1] <= 1):
         return stride[0]
@@ -71,7 +80,8 @@ def _in_out(x, y, in_name: str = "d_in", out_name: str = "d_out"):
     """(shape, dtype, lcpp_dtype, rows, columns, row strides) of an input and an output of its shape and type."""
     shape, dtype, sx, sy = x.shape, x.dtype, x.stride(), y.stride()
     code = _float_codes.get(dtype)
-    if code and len(sx) == 2 and sx[1] == sy[-1] == 1 and y.dtype == dtype and y.shape == shape and sy[0] >= shape[1]:
+    if (code and y.shape == shape and len(sx) == 2 and sx[1] == sy[1] == 1 and y.dtype == dtype and sy[0] >= shape[1]
+            and x.is_cuda and y.is_cuda):
         return shape, dtype, code, shape[0], shape[1], sx[0], sy[0]
     code = float_code(dtype)
     _, rows, cols, si = _matrix(x, in_name)
@@ -86,6 +96,17 @@ def _vector(t, n: int, what: str):
         raise ValueError(f"{what}: holds {t.numel()} values, need {n}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: must be contiguous")
+    if not t.is_cuda:
+        _off_gpu(t, what)
+    return t.data_ptr()
+
+
+def _temp(t):
+    """The address of the temp storage, or None."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        _off_gpu(t, "temp_storage")
     return t.data_ptr()
 
 
@@ -120,6 +141,8 @@ def _counter(t, what: str):
         return None
     if t.numel() < 1 or t.element_size() != 8:
         raise ValueError(f"{what}: must hold a 64-bit integer")
+    if not t.is_cuda:
+        _off_gpu(t, what)
     return t.data_ptr()
 
 
@@ -176,7 +199,7 @@ class DeviceLayerNorm(_BlockModule):
         # (a call without columns, or without rows and weights' gradients, launches nothing and leaves the status word)
         used = cols and (rows or d_grad_weight is not None or d_grad_bias is not None)
         self._call("lcpp_layer_norm_backward", temp_storage if used else None, _stream(stream), code,
-                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
+                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _temp(temp_storage), _nbytes(temp_storage),
                    d_grad_out.data_ptr(), sg, d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
                    _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), d_grad_in.data_ptr(), so,
                    _vector(d_grad_weight, cols, "d_grad_weight"), _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols)
@@ -197,7 +220,7 @@ class DeviceLayerNorm(_BlockModule):
         # (a call without columns, or without rows and weights' gradients, launches nothing and leaves the status word)
         used = cols and (rows or d_grad_weight is not None or d_grad_bias is not None)
         self._call("lcpp_layer_norm_add_backward", temp_storage if used else None, _stream(stream), code,
-                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _ptr(temp_storage), _nbytes(temp_storage),
+                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _temp(temp_storage), _nbytes(temp_storage),
                    d_grad_out.data_ptr(), sg, _ptr(d_grad_sum), sx, d_sum.data_ptr(), ss,
                    _vector(d_weight, cols, "d_weight"), _float_vector(d_mean, rows, "d_mean"),
                    _float_vector(d_rstd, rows, "d_rstd"), p, seed & _U64, offset & _U64, _counter(d_offset, "d_offset"),
@@ -227,6 +250,8 @@ def _sequence_strides(t, shape, dtype, what: str, output: bool = False):
     channels)."""
     if t.shape != shape or t.dtype != dtype:
         _unlike(t, shape, dtype, what)
+    if not t.is_cuda:
+        _off_gpu(t, what)
     stride = t.stride()
     if stride[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{what}: the channels of a row must be adjacent, got strides {stride}")
@@ -319,6 +344,8 @@ class DeviceGatedRecurrence(_BlockModule):
             raise ValueError("offsets need max_length")
         if begin.numel() != end.numel() or not (begin.is_contiguous() and end.is_contiguous()):
             raise ValueError("begin and end offsets must be contiguous and of one length")
+        if not (begin.is_cuda and end.is_cuda):
+            _off_gpu(end if begin.is_cuda else begin, "offsets")
         return begin.numel(), max_length, shape[1], begin.data_ptr(), end.data_ptr(), shape[0]
 
     def Forward(self, temp_storage, d_gate, d_in, d_out, gate: str, d_initial=None, d_final=None, d_checkpoints=None,
@@ -330,7 +357,7 @@ class DeviceGatedRecurrence(_BlockModule):
         states = sizes[0] * sizes[2]
         # (a call without states launches nothing and leaves the status word)
         self._call("lcpp_recurrence_forward", temp_storage if states else None, _stream(stream), float_code(dtype), kind,
-                   _ptr(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+                   _temp(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
                    *_sequence_strides(d_in, shape, dtype, "d_in"), *_sequence_strides(d_out, shape, dtype, "d_out", True),
                    _float_vector(d_initial, states, "d_initial"), _float_vector(d_final, states, "d_final"),
                    _checkpoints(d_checkpoints, sizes), *sizes)
@@ -344,7 +371,7 @@ class DeviceGatedRecurrence(_BlockModule):
         states = sizes[0] * sizes[2]
         # (a call without states launches nothing and leaves the status word)
         self._call("lcpp_recurrence_backward", temp_storage if states else None, _stream(stream), float_code(dtype), kind,
-                   _ptr(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+                   _temp(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
                    *_sequence_strides(d_in, shape, dtype, "d_in"),
                    _checkpoints(d_checkpoints, sizes),
                    *_sequence_strides(d_grad_out, shape, dtype, "d_grad_out"),
