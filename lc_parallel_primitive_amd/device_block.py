@@ -139,7 +139,7 @@ def _weight_code(code: int, *weights):
 def _counter(t, what: str):
     if t is None:
         return None
-    if t.numel() < 1 or t.element_size() != 8:
+    if t.numel() < 1 or t.element_size() != 8 or t.is_floating_point() or t.is_complex():
         raise ValueError(f"{what}: must hold a 64-bit integer")
     if not t.is_cuda:
         _off_gpu(t, what)
