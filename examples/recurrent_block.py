@@ -6,13 +6,15 @@ sequences that count in steps of their own, then decoded one token at a time.
 Each residual block is   h = h + dropout(W_o recurrence(W_g n, W_v n)),   n = layer norm(h),   and a block's
 residual sum, dropout and the next block's norm are one call.  Training packs sequences of different lengths one
 behind the other (begin and end offsets, nothing padded); decoding keeps one state per layer and sequence in a pool
-of slots and gives the same logits as the whole sequences at once."""
+of slots and gives the same logits as the whole sequences at once.  Gradients of gradients are not computed: asking
+for them is an error."""
 from __future__ import annotations
 
 import os
 import sys
 
 import torch
+from torch.autograd.function import once_differentiable
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
@@ -36,6 +38,7 @@ class Norm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, w, mean, rstd = ctx.saved_tensors
         dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
@@ -57,6 +60,7 @@ class AddNorm(torch.autograd.Function):
         return total, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dtotal, dy):
         total, w, mean, rstd = ctx.saved_tensors
         dres, dx = torch.empty_like(total), torch.empty_like(total)
@@ -79,6 +83,7 @@ class Recurrence(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         gate, x, saved = ctx.saved_tensors
         dg, dx = torch.empty_like(dy), torch.empty_like(dy)
