@@ -23,7 +23,7 @@ import ctypes
 import functools
 
 from ._capi import LCPP_GATES, _float_codes, check, float_code, lib
-from .device import _Module, _nbytes, _ptr, _query, _stream
+from .device import _Module, _ptr, _query, _stream
 
 
 # What a call does before its launch is most of a small call's time (device.py),
@@ -70,10 +70,16 @@ def _like(t, shape, dtype, what: str):
 
 def _like_out(t, shape, dtype, what: str):
     """The same for an output, whose rows must not overlap."""
-    stride = _like(t, shape, dtype, what)
-    if stride < shape[-1] and len(shape) == 2 and shape[0] > 1:
+    if t.shape != shape or t.dtype != dtype:
+        _unlike(t, shape, dtype, what)
+    if not t.is_cuda:
+        _off_gpu(t, what)
+    stride = t.stride()
+    if len(stride) != 2 or (stride[1] != 1 and shape[1] > 1):
+        return _matrix(t, what)[3]
+    if stride[0] < shape[1] and shape[0] > 1:
         raise ValueError(f"{what}: the rows of an output must not overlap")
-    return stride
+    return stride[0]
 
 
 def _in_out(x, y, in_name: str = "d_in", out_name: str = "d_out"):
@@ -92,22 +98,22 @@ def _vector(t, n: int, what: str):
     """The address of a contiguous tensor of at least n values, or None."""
     if t is None:
         return None
+    if t.numel() >= n and t.is_contiguous() and t.is_cuda:
+        return t.data_ptr()
     if t.numel() < n:
         raise ValueError(f"{what}: holds {t.numel()} values, need {n}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: must be contiguous")
-    if not t.is_cuda:
-        _off_gpu(t, what)
-    return t.data_ptr()
+    _off_gpu(t, what)
 
 
 def _temp(t):
-    """The address of the temp storage, or None."""
+    """(address, bytes) of the temp storage, or (None, 0)."""
     if t is None:
-        return None
+        return None, 0
     if not t.is_cuda:
         _off_gpu(t, "temp_storage")
-    return t.data_ptr()
+    return t.data_ptr(), t.nbytes
 
 
 def _float_vector(t, n: int, what: str):
@@ -115,22 +121,23 @@ def _float_vector(t, n: int, what: str):
         return None
     if _float_codes.get(t.dtype) != 2 and float_code(t.dtype) != 2:
         raise TypeError(f"{what}: must be float32, got {t.dtype}")
+    if t.numel() >= n and t.is_contiguous() and t.is_cuda:
+        return t.data_ptr()
     return _vector(t, n, what)
 
 
-def _weight_code(code: int, *weights):
+def _weight_code(code: int, weight, *others):
     """The lcpp_dtype of the weights that are given: the activations' or float32."""
-    first = None
-    for w in weights:
+    dtype = None if weight is None else weight.dtype
+    for w in others:
         if w is not None:
-            dtype = w.dtype
-            if first is None:
-                first = dtype
-            elif dtype != first:
+            if dtype is None:
+                dtype = w.dtype
+            elif w.dtype != dtype:
                 raise TypeError("weight, bias and their gradients must have one dtype")
-    if first is None:
+    if dtype is None:
         return code
-    wt = _float_codes.get(first) or float_code(first)
+    wt = _float_codes.get(dtype) or float_code(dtype)
     if wt != code and wt != 2:
         raise TypeError("weights must have the activations' dtype or float32")
     return wt
@@ -146,17 +153,17 @@ def _counter(t, what: str):
     return t.data_ptr()
 
 
-@functools.lru_cache(maxsize=None)
+_entries: dict = {}
+
+
 def _entry(name: str):
-    return getattr(lib(), name)
-
-
-_U64 = (1 << 64) - 1
+    f = _entries[name] = getattr(lib(), name)
+    return f
 
 
 class _BlockModule(_Module):
     def _call(self, name: str, temp, stream, *args):
-        status = _entry(name)(*args, stream)
+        status = (_entries.get(name) or _entry(name))(*args, stream)
         if status or self._debug:
             self._check(status, name, temp, stream)
 
@@ -186,7 +193,7 @@ class DeviceLayerNorm(_BlockModule):
         sr = _like(d_residual, shape, dtype, "d_residual")
         ss, so = _like_out(d_sum, shape, dtype, "d_sum"), _like_out(d_out, shape, dtype, "d_out")
         self._call("lcpp_layer_norm_add_forward", None, _stream(stream), code, _weight_code(code, d_weight, d_bias),
-                   d_in.data_ptr(), si, d_residual.data_ptr(), sr, p, seed & _U64, offset & _U64,
+                   d_in.data_ptr(), si, d_residual.data_ptr(), sr, p, seed, offset,
                    _counter(d_offset, "d_offset"), _vector(d_weight, cols, "d_weight"), _vector(d_bias, cols, "d_bias"), eps,
                    d_sum.data_ptr(), ss, d_out.data_ptr(), so, _float_vector(d_mean, rows, "d_mean"),
                    _float_vector(d_rstd, rows, "d_rstd"), rows, cols)
@@ -196,10 +203,9 @@ class DeviceLayerNorm(_BlockModule):
         """The gradients of Forward's d_in, d_weight and d_bias (the latter two None if not wanted)."""
         shape, dtype, code, rows, cols, si, so = _in_out(d_in, d_grad_in, "d_in", "d_grad_in")
         sg = _like(d_grad_out, shape, dtype, "d_grad_out")
-        # (a call without columns, or without rows and weights' gradients, launches nothing and leaves the status word)
-        used = cols and (rows or d_grad_weight is not None or d_grad_bias is not None)
-        self._call("lcpp_layer_norm_backward", temp_storage if used else None, _stream(stream), code,
-                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _temp(temp_storage), _nbytes(temp_storage),
+        # (a call of nothing may launch nothing and leave the status word)
+        self._call("lcpp_layer_norm_backward", temp_storage if rows and cols else None, _stream(stream), code,
+                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), *_temp(temp_storage),
                    d_grad_out.data_ptr(), sg, d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
                    _float_vector(d_mean, rows, "d_mean"), _float_vector(d_rstd, rows, "d_rstd"), d_grad_in.data_ptr(), so,
                    _vector(d_grad_weight, cols, "d_grad_weight"), _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols)
@@ -217,13 +223,12 @@ class DeviceLayerNorm(_BlockModule):
         sx = 0 if d_grad_sum is None else _like(d_grad_sum, shape, dtype, "d_grad_sum")
         sr = 0 if d_grad_residual is None else _like_out(d_grad_residual, shape, dtype, "d_grad_residual")
         si = 0 if d_grad_in is None else _like_out(d_grad_in, shape, dtype, "d_grad_in")
-        # (a call without columns, or without rows and weights' gradients, launches nothing and leaves the status word)
-        used = cols and (rows or d_grad_weight is not None or d_grad_bias is not None)
-        self._call("lcpp_layer_norm_add_backward", temp_storage if used else None, _stream(stream), code,
-                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), _temp(temp_storage), _nbytes(temp_storage),
+        # (a call of nothing may launch nothing and leave the status word)
+        self._call("lcpp_layer_norm_add_backward", temp_storage if rows and cols else None, _stream(stream), code,
+                   _weight_code(code, d_weight, d_grad_weight, d_grad_bias), *_temp(temp_storage),
                    d_grad_out.data_ptr(), sg, _ptr(d_grad_sum), sx, d_sum.data_ptr(), ss,
                    _vector(d_weight, cols, "d_weight"), _float_vector(d_mean, rows, "d_mean"),
-                   _float_vector(d_rstd, rows, "d_rstd"), p, seed & _U64, offset & _U64, _counter(d_offset, "d_offset"),
+                   _float_vector(d_rstd, rows, "d_rstd"), p, seed, offset, _counter(d_offset, "d_offset"),
                    _ptr(d_grad_residual), sr, _ptr(d_grad_in), si, _vector(d_grad_weight, cols, "d_grad_weight"),
                    _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols)
 
@@ -238,7 +243,7 @@ class DeviceDropout(_BlockModule):
         shape, dtype, code, rows, cols, si, so = _in_out(d_in, d_out)
         sr = 0 if d_residual is None else _like(d_residual, shape, dtype, "d_residual")
         self._call("lcpp_dropout", None, _stream(stream), code, d_in.data_ptr(), si, _ptr(d_residual), sr,
-                   d_out.data_ptr(), so, rows, cols, p, seed & _U64, offset & _U64, _counter(d_offset, "d_offset"))
+                   d_out.data_ptr(), so, rows, cols, p, seed, offset, _counter(d_offset, "d_offset"))
 
     def Backward(self, d_grad_out, d_grad_in, p: float, seed: int, offset: int = 0, d_offset=None, stream=None):
         """The gradient of Forward's d_in, with the forward call's p, seed and offset (d_residual's is d_grad_out itself)."""
@@ -250,6 +255,11 @@ def _sequence_strides(t, shape, dtype, what: str, output: bool = False):
     channels)."""
     if t.shape != shape or t.dtype != dtype:
         _unlike(t, shape, dtype, what)
+    return _strides(t, shape, what, output)
+
+
+def _strides(t, shape, what: str, output: bool = False):
+    """The same of a tensor that is known to have this shape."""
     if not t.is_cuda:
         _off_gpu(t, what)
     stride = t.stride()
@@ -357,8 +367,8 @@ class DeviceGatedRecurrence(_BlockModule):
         states = sizes[0] * sizes[2]
         # (a call without states launches nothing and leaves the status word)
         self._call("lcpp_recurrence_forward", temp_storage if states else None, _stream(stream), float_code(dtype), kind,
-                   _temp(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
-                   *_sequence_strides(d_in, shape, dtype, "d_in"), *_sequence_strides(d_out, shape, dtype, "d_out", True),
+                   *_temp(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+                   *_strides(d_in, shape, "d_in"), *_sequence_strides(d_out, shape, dtype, "d_out", True),
                    _float_vector(d_initial, states, "d_initial"), _float_vector(d_final, states, "d_final"),
                    _checkpoints(d_checkpoints, sizes), *sizes)
 
@@ -371,8 +381,8 @@ class DeviceGatedRecurrence(_BlockModule):
         states = sizes[0] * sizes[2]
         # (a call without states launches nothing and leaves the status word)
         self._call("lcpp_recurrence_backward", temp_storage if states else None, _stream(stream), float_code(dtype), kind,
-                   _temp(temp_storage), _nbytes(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
-                   *_sequence_strides(d_in, shape, dtype, "d_in"),
+                   *_temp(temp_storage), *_sequence_strides(d_gate, shape, dtype, "d_gate"),
+                   *_strides(d_in, shape, "d_in"),
                    _checkpoints(d_checkpoints, sizes),
                    *_sequence_strides(d_grad_out, shape, dtype, "d_grad_out"),
                    *_sequence_strides(d_grad_gate, shape, dtype, "d_grad_gate", True),
