@@ -358,7 +358,9 @@ int lcpp_segment_reduce_argmax_fixed(lcpp_dtype t, void *temp, size_t temp_bytes
  * t: LCPP_FLOAT32, LCPP_BFLOAT16 or LCPP_FLOAT16 for activations and their
  * gradients; statistics, states and random-bit counters are float32 / 64-bit
  * integers as declared.  Everything is computed in 32 bits and rounded once,
- * to nearest even, when it is stored.  Rows have unit stride along their
+ * to nearest even, when it is stored (so a row whose sum or squares pass float32's
+ * range is normalised to NaN).  Exponentials are the GPU's own of base 2: of exp(g)
+ * and of the smaller side of sigmoid(g) some (8 + 2 |g|) 2^-24 may be wrong.  Rows have unit stride along their
  * columns; *_stride is the distance between rows in elements, of any size for
  * inputs (0 repeats a row) and at least cols for outputs.  Pointers need the
  * alignment of one element only.  Outputs may lie exactly in the place of an

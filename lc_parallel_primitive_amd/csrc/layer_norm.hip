@@ -18,9 +18,9 @@
 // sums in the same registers, one partial sum per workgroup, and a second launch
 // adds these in a fixed order: no atomics, the same result at every call.
 //
-// Measured (us and what that makes of the bytes read and written once; TB/s):
-// 16384 x 4096 bfloat16 forward 52 (5.2), backward 69 (5.8), the partial sums 5; 16384
-// x 2048 with the sum and dropout, forward 44 (6.1), backward 60 (5.6), the partial
+// Measured (us by kernel traces and what that makes of the bytes read and written once;
+// TB/s): 16384 x 4096 bfloat16 forward 51 (5.3), backward 68 (6.0), the partial sums 5;
+// 16384 x 2048 with the sum and dropout, forward 45 (5.9), backward 60 (5.6), the partial
 // sums 5.  A copy of 512 MiB runs at 5.3; what the pass before has left in the
 // last-level cache makes up the rest.  16 x 1024 forward 3: a launch.
 #include <algorithm>
@@ -732,8 +732,8 @@ constexpr uint64_t kMaxGroups = 1u << 20;
 // Threads of a workgroup whose rows take nt each: as many rows as fit `atleast`.
 constexpr int norm_threads(int nt, int atleast) { return nt >= atleast ? nt : atleast / nt * nt; }
 // Workgroups that the device holds at once: all get the same number of rows, give
-// or take one (one more per CU than is resident would run alone in the end: 16384
-// x 4096 bfloat16 forward 64 -> 60 us).
+// or take one (one more per CU than is resident runs alone in the end: 16384 x 4096
+// bfloat16 forward 53 us, 59 with one more).
 template <class Kernel>
 uint64_t resident_groups(DeviceCache &cache, Kernel kernel, int threads)
 {
@@ -747,14 +747,15 @@ uint64_t resident_groups(DeviceCache &cache, Kernel kernel, int threads)
 // NT threads with K octets each for a row of `octets`: the smallest group of
 // waves that holds it.  f(NT, K) as integral constants; false if the row is longer
 // or f has no kernel of that shape.  PER: octets of a thread in rows of several
-// waves.  Two are better for the forward pass of 2-byte types, one for 4-byte
-// types and for the backward pass, which keeps sums for each (us, one -> two:
-// forward of 16384 x 4096 bfloat16 59 -> 51, 8000 x 7000 64 -> 47, 2000 x 4096
-// float32 13 -> 15; backward of 1777 x 5001 float16 with the sum 25 -> 27, 8000 x
-// 7000 114 -> 123).  FINE: a group for 640 octets too, for the forward pass without
-// the sum (16384 x 5120 bfloat16 78 -> 76, 8000 x 5001 48 -> 44, 3000 x 4608 18 -> 14,
-// 4000 x 5120 float32 36 -> 35); with the sum (118 -> 132 at 16384 x 5120) and
-// backward (60 -> 62 at 8000 x 5001) the larger group's waves fill the CU better.
+// waves.  Two are better for the forward pass of 2-byte types, one for 4-byte types
+// (us between events, one -> two: 16384 x 4096 bfloat16 55.6 -> 52.6, 16384 x 5120 87 -> 77,
+// 3000 x 4608 19 -> 15; 2000 x 4096 float32 15.0 -> 17.5).  The backward pass keeps sums
+// for each octet; two lose with few rows or full groups (1777 x 5001 float16 with the sum 27.2
+// -> 29.7, 8000 x 7000 bfloat16 56 -> 60) and win with many rows of 5120 columns (104 -> 89).
+// FINE: a group for 640 octets too, for the forward pass without the sum (16384 x 5120
+// bfloat16 83 -> 77, 8000 x 5001 50 -> 45, 3000 x 4608 19 -> 15); with the sum (113 -> 117 at
+// 16384 x 5120) and backward (60.5 -> 63 at 8000 x 5001, 21.0 -> 23.4 at 3000 x 4608) the larger
+// group's waves fill the CU better.
 template <int NT, int K, class F>
 bool norm_shape_of(F f)
 {

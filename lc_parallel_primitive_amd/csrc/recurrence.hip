@@ -28,14 +28,14 @@
 //
 // Bound by memory where there are chains enough.  bfloat16, us by kernel traces and
 // TB/s of the bytes read and written once: 8 x 4096 x 2048 forward 81 (5.0), backward
-// 141 (4.8); 1 x 65536 x 2048 forward 166-172 (4.7-4.85); a copy of as many bytes
-// runs at 5.2.  Sequences of different lengths end with few tiles at work: 24 of
-// them, 16391 rows x 1536 in all, 39 + 60 (3.9, 4.2).  A single chain is bound by the
-// look-back, 0.06 us a tile: 1 x 40000 x 64 forward 19, backward 22.
-// kRows and kWaves: a tile has to lie in registers at four waves a SIMD.  With 18
-// and 20 rows a wave the backward pass of 8 x 4096 x 2048 took 181 and 178 us
-// where 16 took 159; 8 rows a wave, sixteen waves, four channels a lane and tiles of
-// 64 rows were slower too.
+// 138 (4.9); 1 x 65536 x 2048 forward 163 between events (4.95), 176 in a trace; a copy of
+// as many bytes runs at 5.2.  Sequences of different lengths end with few tiles at
+// work: 24 of them, 16391 rows x 1536 in all, 35 + 59 (4.3 both).  A single chain is bound
+// by the look-back, 0.06 us a tile: 1 x 40000 x 64 forward 27, backward 29.5 between events.
+// kRows and kWaves: a tile has to lie in registers at four waves a SIMD.  An earlier
+// form's backward pass of 8 x 4096 x 2048 took 181 and 178 us with 18 and 20 rows a wave,
+// 159 with 16; 8 rows a wave, sixteen waves, four channels a lane and tiles of 64 rows
+// were slower too.
 #include <algorithm>
 
 #include "lookback.hpp"
@@ -86,6 +86,8 @@ struct GateDecay {
     __device__ static __forceinline__ void eval(float g, float &a, float &share) { a = g, share = 1.0f; }
     __device__ static __forceinline__ float grad(float dh, float before, float, float, float) { return dh * before; }
 };
+// (the native exponential: g log2(e) is rounded once, which is |g| roundings of the
+// result; where that is much the result is small)
 struct GateLog {
     static constexpr bool kShare = false;
     __device__ static __forceinline__ void eval(float g, float &a, float &share) { a = __expf(g), share = 1.0f; }
@@ -143,11 +145,12 @@ constexpr uint32_t kXcds = 8;
 // workgroups in turn, works on whole runs: where rows do not begin at a line of
 // memory, neighbouring groups share lines, and their parts meet in one L2.  The
 // runs go to another XCD at every tile.  Measured (us, forward + backward): 8 x
-// 4096 x 2049 bfloat16 145 + 263 with runs of one chain, 102 + 162 with an eighth
-// of all; 1 x 65536 x 2048 forward 186 with the runs on one XCD at all tiles, 163
-// in turn.  Sequences of different lengths have short runs, or the last one at
-// work would leave XCDs idle (24 packed x 1536 channels: 142 with an eighth of
-// all chains, 108 with runs of 4).  Numbers past the last chain are left at once.
+// 4096 x 2049 bfloat16 125 + 194 with runs of one chain, 98 + 164 with an eighth of
+// all (1 x 65536 x 2048, whose rows begin at lines, 157 + 265 and 163 + 273); the latter
+// 196 + 292 with the runs on one XCD at all tiles.  Sequences of different lengths have
+// runs of 4, or the last one at work would leave XCDs idle (24 packed, 16391 rows: runs of 1,
+// 4 and 16 of 1536 channels 36.5 + 57, 37 + 60, 38 + 60, of 1537 channels 53 + 74, 49 + 69, 47 + 69).
+// Numbers past the last chain are left at once.
 //
 // Sequences of different lengths (offsets) have their tiles in a list, which the
 // clearing launch makes from the offsets: there are no more than rows / 128 + sequences,
@@ -259,8 +262,8 @@ __device__ __forceinline__ float advance(float A, float h, float H) { return __b
 // distance to the tile before it, `before` the number of tiles there.
 // The first poll reads one tile's words: as all chains advance together, the tile
 // before has its state when its map is there, and a first window of 2, 4 or 8 tiles
-// reads words that are not needed (1 x 65536 x 2048: 195 us with one, 216, 240 and
-// 270).  A walk that goes on reads kWindow at once (forward + backward, one at once ->
+// reads words that are not needed (an earlier form at 1 x 65536 x 2048: 195 us with one,
+// 216, 240 and 270).  A walk that goes on reads kWindow at once (forward + backward, one at once ->
 // four: 1 x 100000 x 512 float32 121 + 184 -> 113 + 184, 1 x 65536 x 2048 165 + 280 -> 163 +
 // 273), and 32 KB of maps are 64 or 32 of them (1 x 40000 x 64 with 32 maps 30 + 32, with
 // 64 27 + 29.5).  Maps composed on the way back, in no fixed order, took 112 + 183, 160 +
@@ -328,8 +331,8 @@ __device__ __forceinline__ Chan<C> look_back(const uint64_t *words, uint64_t ste
             if (lane == 0) report_timeout(ctl);
             return false;
         }
-        // (a tile's stores take far longer than this: polled at every 64 cycles 1 x
-        // 65536 x 2048 took 190 us, at every 512 186)
+        // (a tile's stores take longer than this; 1 x 65536 x 2048 takes the same with polls
+        // at every 64 cycles, which only add to the traffic)
         __builtin_amdgcn_s_sleep(8);
         return true;
     };
@@ -399,10 +402,10 @@ __device__ __forceinline__ void publish_state(uint64_t *words, const Chan<C> &A,
 }
 
 // Rows that begin at a line of memory (STREAM) are read and written with the
-// streaming policy: 8 x 4096 x 2048 bfloat16 87 + 145 us, without it 95 + 152; 4 x
-// 512 x 1024 10.5 + 15.0 and 10.8 + 15.5.  Where neighbouring groups share lines
-// these are better kept in the L2: of 2049 channels 117 + 214 us with the policy,
-// 102 + 162 without it.
+// streaming policy: 8 x 4096 x 2048 bfloat16 82 + 136 us, without it 88 + 147; 4 x
+// 512 x 1024 10.4 + 15.0 and 10.6 + 15.6.  Where neighbouring groups share lines
+// these are better kept in the L2: of 2050 channels 113 + 197 us with the policy,
+// 95 + 158 without it.
 template <bool STREAM, int N, class T>
 __device__ __forceinline__ Pack<T, N> load_rows_of(const T *p)
 {
