@@ -53,8 +53,10 @@ typedef enum lcpp_dtype LCPP_ENUM_INT {
     LCPP_INT64 = 3,
     LCPP_UINT64 = 4,
     LCPP_FLOAT64 = 5,
-    LCPP_BFLOAT16 = 6, /* these two: lcpp_layer_norm_*, lcpp_dropout, lcpp_recurrence_* only */
-    LCPP_FLOAT16 = 7
+    LCPP_BFLOAT16 = 6, /* these two: the operators of a language model's blocks only */
+    LCPP_FLOAT16 = 7,
+    LCPP_FLOAT8_E4M3 = 8, /* 8-bit floating point with 3 bits of fraction (largest value 448, no infinity) and with */
+    LCPP_FLOAT8_E5M2 = 9  /* 2 (57344): where an entry point names them */
 } lcpp_dtype;
 
 /* Reduction operators and element transforms of lcpp_reduce_transform (the
@@ -78,6 +80,12 @@ typedef enum lcpp_gate LCPP_ENUM_INT {
     LCPP_GATE_LOG = 1,    /* a = exp(g), b = x */
     LCPP_GATE_SIGMOID = 2 /* a = sigmoid(g), b = (1 - a) x */
 } lcpp_gate;
+
+/* How lcpp_router_* make a row's weights of its logits. */
+typedef enum lcpp_score LCPP_ENUM_INT {
+    LCPP_SCORE_SOFTMAX = 0, /* exp(l) / sum of exp(l) */
+    LCPP_SCORE_SIGMOID = 1  /* 1 / (1 + exp(-l)) */
+} lcpp_score;
 
 typedef enum lcpp_status LCPP_ENUM_INT {
     LCPP_OK = 0,
@@ -453,6 +461,98 @@ int lcpp_recurrence_step(lcpp_dtype t, lcpp_gate g, const void *gate, uint64_t g
                          uint64_t in_stride, const float *state_in, float *state_out, const int32_t *slots,
                          uint64_t num_slots, void *out, uint64_t out_stride, uint64_t sequences, uint64_t channels,
                          void *stream);
+
+/* ---------------------------------------------------------------------
+ * RMS norm, expert router, tokens sorted by expert, experts' products (no
+ * counterpart in the reference): the sparse feed-forward half of a language
+ * model's block.  Types, strides and places of outputs as above.  A pair is a
+ * token's choice: number token * choices + choice.  tokens * choices < 2^31.
+ * ------------------------------------------------------------------- */
+/* s = in, or with a residual s = residual + in, stored at sum in type t; out[r] = s[r] * rstd *
+ * weight with rstd = 1 / sqrt(mean(s[r]^2) + eps) of s as it is stored.  weight: `cols` values of
+ * type wt (t or LCPP_FLOAT32), NULL for 1.  rstd: one value per row for the backward pass, or NULL.
+ * quant (NULL: none): out before its rounding to t, in type qt (LCPP_FLOAT8_E4M3 or _E5M2): for each
+ * row and `group` columns (32, 64, 128, 256 or 512, the last ones less; 0: the whole row)
+ * scale = max(max |out|, 2^-100) / (the type's largest value), quant = out / scale rounded to
+ * nearest even; scales[r * scale_row_stride + g * scale_group_stride].  A group with a value that is
+ * not finite has the scale NaN and values NaN.  out may be NULL where quant is not.  The square of a
+ * value passes float32's range from 2^64 on: such a row gives 0 (rstd 0).  quant may not lie over
+ * an input. */
+int lcpp_rms_norm_forward(lcpp_dtype t, lcpp_dtype wt, const void *in, uint64_t in_stride, const void *residual,
+                          uint64_t residual_stride, const void *weight, float eps, void *sum, uint64_t sum_stride,
+                          void *out, uint64_t out_stride, float *rstd, lcpp_dtype qt, void *quant,
+                          uint64_t quant_stride, float *scales, uint64_t scale_row_stride,
+                          uint64_t scale_group_stride, uint32_t group, uint64_t rows, uint64_t cols, void *stream);
+/* Partial sums of the weight's gradient: up to 512 rows of cols floats. */
+int lcpp_rms_norm_backward_temp_bytes(lcpp_dtype t, uint64_t rows, uint64_t cols, size_t *bytes);
+/* The gradients from that of `out` (quant passes it on as if it were out): in: s as it was
+ * normalised; grad_sum: what reaches s by other ways, or NULL; grad_in: the gradient of s, which
+ * is that of in and of the residual; grad_weight: `cols` values of type wt, or NULL (else temp is
+ * needed); for rows = 0 it is set to 0.  The same bits at every call. */
+int lcpp_rms_norm_backward(lcpp_dtype t, lcpp_dtype wt, void *temp, size_t temp_bytes, const void *grad_out,
+                           uint64_t grad_out_stride, const void *grad_sum, uint64_t grad_sum_stride, const void *in,
+                           uint64_t in_stride, const void *weight, const float *rstd, void *grad_in,
+                           uint64_t grad_in_stride, void *grad_weight, uint64_t rows, uint64_t cols, void *stream);
+
+/* For each row of logits [tokens][num_experts] the `choices` experts whose key, the logit plus
+ * bias[expert] (NULL: 0) rounded once to float32, is largest, in falling order, ties to the lowest
+ * index, a NaN before all others; an expert whose logit or key is -infinity is never chosen: where
+ * too few are left experts is -1 and the weight 0.  weights = scale * the logit's share (lcpp_score;
+ * the bias has no part in it); with normalize, shares of the sum over the chosen ones.  experts,
+ * weights: [tokens][choices].  num_experts <= 1024, choices <= 64 and <= num_experts.  Exponentials
+ * are the GPU's own of base 2: (8 + 2 |x|) 2^-24 of exp(x) may be wrong. */
+int lcpp_router_forward(lcpp_dtype t, lcpp_score score, int normalize, float scale, const void *logits,
+                        uint64_t logits_stride, const float *bias, int32_t *experts, float *weights, uint64_t tokens,
+                        uint64_t num_experts, uint64_t choices, void *stream);
+/* The gradient of the logits from that of the weights, for the experts that the forward call chose
+ * (others than 0 .. num_experts - 1 have none).  grad_logits may lie over logits. */
+int lcpp_router_backward(lcpp_dtype t, lcpp_score score, int normalize, float scale, const void *logits,
+                         uint64_t logits_stride, const int32_t *experts, const float *grad_weights, void *grad_logits,
+                         uint64_t grad_stride, uint64_t tokens, uint64_t num_experts, uint64_t choices, void *stream);
+
+/* The pairs in the order of their experts, stable: positions[pair] = its row there, -1 for pairs
+ * whose expert is not in 0 .. num_experts - 1; offsets[num_experts + 1]: where each expert's rows
+ * begin, and the number of all; sources[row] = the row's pair (tokens * choices values, those behind
+ * the last row left alone), or NULL.  1 <= num_experts <= 1024. */
+int lcpp_token_sort_temp_bytes(uint64_t tokens, uint64_t choices, uint64_t num_experts, size_t *bytes);
+int lcpp_token_sort(void *temp, size_t temp_bytes, const int32_t *experts, uint64_t tokens, uint64_t choices,
+                    uint64_t num_experts, int32_t *positions, int32_t *offsets, int32_t *sources, void *stream);
+/* out[positions[t][j]] = weights[t][j] * in[t] (weights NULL: a copy, of any type of 1, 2 or 4 bytes
+ * that is not LCPP_INT64, _UINT64 or _FLOAT64) for every pair whose position is in 0 .. rows - 1; other rows of
+ * out are left alone.  No two pairs may have one position.  dots (NULL: none) [tokens][choices] =
+ * the sum over columns of in[t] * other[positions[t][j]], 0 for pairs without a row; out may then be
+ * NULL.  choices <= 64. */
+int lcpp_token_spread(lcpp_dtype t, const void *in, uint64_t in_stride, const int32_t *positions,
+                      const float *weights, void *out, uint64_t out_stride, const void *other, uint64_t other_stride,
+                      float *dots, uint64_t rows, uint64_t tokens, uint64_t choices, uint64_t cols, void *stream);
+/* out[t] = residual[t] (NULL: 0) + sum over j of weights[t][j] (NULL: 1) * in[positions[t][j]], in the
+ * order of j and in 32 bits; pairs without a row count nothing.  dots (NULL: none; not with a
+ * residual) = the sum over columns of other[t] * in[positions[t][j]]. */
+int lcpp_token_sum(lcpp_dtype t, const void *in, uint64_t in_stride, uint64_t rows, const int32_t *positions,
+                   const float *weights, const void *residual, uint64_t residual_stride, void *out,
+                   uint64_t out_stride, const void *other, uint64_t other_stride, float *dots, uint64_t tokens,
+                   uint64_t choices, uint64_t cols, void *stream);
+
+/* Rows offsets[e] .. offsets[e + 1] of in times the transpose of expert e's matrix, weight + e *
+ * weight_expert_stride, of `outputs` rows of `inputs` values, weight_stride apart: out[r][o] = the sum
+ * over i of in[r][i] * weight[e][o][i], in 32 bits, rounded once to out_t, which is t.  Offsets are
+ * increasing; rows outside all of them are left alone.  t may be LCPP_FLOAT8_E4M3, with scales and out_t
+ * any of the three types: in_scales[r * in_scale_row_stride + g * in_scale_group_stride] for each
+ * row's 128 inputs and weight_scales [experts][ceil(outputs / 128)][ceil(inputs / 128)] for each 128
+ * outputs x 128 inputs multiply the values (else both are NULL). */
+int lcpp_expert_product(lcpp_dtype t, const void *in, uint64_t in_stride, const void *weight, uint64_t weight_stride,
+                        uint64_t weight_expert_stride, const int32_t *offsets, lcpp_dtype out_t, void *out,
+                        uint64_t out_stride, const float *in_scales, uint64_t in_scale_row_stride,
+                        uint64_t in_scale_group_stride, const float *weight_scales, uint64_t rows, uint64_t experts,
+                        uint64_t outputs, uint64_t inputs, void *stream);
+/* The gradients of in and of the matrices (each NULL if not wanted; the latter of type t or
+ * LCPP_FLOAT32, 0 for experts without rows) from that of out.  The same bits at every call. */
+int lcpp_expert_product_backward(lcpp_dtype t, const void *grad_out, uint64_t grad_out_stride, const void *in,
+                                 uint64_t in_stride, const void *weight, uint64_t weight_stride,
+                                 uint64_t weight_expert_stride, const int32_t *offsets, void *grad_in,
+                                 uint64_t grad_in_stride, lcpp_dtype grad_weight_t, void *grad_weight,
+                                 uint64_t grad_weight_stride, uint64_t grad_weight_expert_stride, uint64_t rows,
+                                 uint64_t experts, uint64_t outputs, uint64_t inputs, void *stream);
 
 /* ---------------------------------------------------------------------
  * Instrumentation (no counterpart in the reference).  When enabled, every

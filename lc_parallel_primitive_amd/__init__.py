@@ -25,7 +25,8 @@ from ._capi import (  # noqa: F401
     profile_enable,
     profile_read,
 )
-from .device_block import DeviceDropout, DeviceGatedRecurrence, DeviceLayerNorm  # noqa: F401
+from .device_block import DeviceDropout, DeviceGatedRecurrence, DeviceLayerNorm, DeviceRMSNorm  # noqa: F401
+from .device_expert import DeviceExpertProduct, DeviceExpertRouter, DeviceTokenSort  # noqa: F401
 from .device import DeviceRadixSort, DeviceReduce, DeviceScan, DeviceSegmentReduce  # noqa: F401
 
 __all__ = [
@@ -34,8 +35,12 @@ __all__ = [
     "DeviceRadixSort",
     "DeviceSegmentReduce",
     "DeviceLayerNorm",
+    "DeviceRMSNorm",
     "DeviceDropout",
     "DeviceGatedRecurrence",
+    "DeviceExpertRouter",
+    "DeviceExpertProduct",
+    "DeviceTokenSort",
     "LcppError",
     "lib",
     "lib_path",

@@ -9,10 +9,12 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 lib_path = os.path.join(_PKG, "liblcpp_amd.so")
 
 LCPP_INT32, LCPP_UINT32, LCPP_FLOAT32, LCPP_INT64, LCPP_UINT64, LCPP_FLOAT64 = range(6)
-LCPP_BFLOAT16, LCPP_FLOAT16 = 6, 7  # the layer norm, dropout and recurrence only
+LCPP_BFLOAT16, LCPP_FLOAT16 = 6, 7  # the operators of a language model's blocks only
+LCPP_FLOAT8_E4M3, LCPP_FLOAT8_E5M2 = 8, 9
 LCPP_OPS = {"sum": 0, "min": 1, "max": 2}
 LCPP_TRANSFORMS = {"identity": 0, "negate": 1, "abs": 2, "square": 3}
 LCPP_GATES = {"decay": 0, "log": 1, "sigmoid": 2}
+LCPP_SCORES = {"softmax": 0, "sigmoid": 1}
 LCPP_DTYPES = {
     "int32": LCPP_INT32,
     "uint32": LCPP_UINT32,
@@ -90,6 +92,21 @@ SIGNATURES = {
     "lcpp_recurrence_backward": (_i, [_i, _i, _vp, ctypes.c_size_t] + [_vp, _u64, _u64] * 2 + [_vp] + [_vp, _u64, _u64] * 3
                                  + [_vp, _vp, _u64, _u64, _u64, _vp, _vp, _u64, _vp]),
     "lcpp_recurrence_step": (_i, [_i, _i, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _u64, _u64, _vp]),
+    "lcpp_rms_norm_forward": (_i, [_i, _i, _vp, _u64, _vp, _u64, _vp, _f, _vp, _u64, _vp, _u64, _vp, _i, _vp, _u64, _vp, _u64, _u64,
+                                   ctypes.c_uint32, _u64, _u64, _vp]),
+    "lcpp_rms_norm_backward_temp_bytes": (_i, [_i, _u64, _u64, _c_size_p]),
+    "lcpp_rms_norm_backward": (_i, [_i, _i, _vp, ctypes.c_size_t, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _vp, _u64,
+                                    _u64, _vp]),
+    "lcpp_router_forward": (_i, [_i, _i, _i, _f, _vp, _u64, _vp, _vp, _vp, _u64, _u64, _u64, _vp]),
+    "lcpp_router_backward": (_i, [_i, _i, _i, _f, _vp, _u64, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _vp]),
+    "lcpp_token_sort_temp_bytes": (_i, [_u64, _u64, _u64, _c_size_p]),
+    "lcpp_token_sort": (_i, [_vp, ctypes.c_size_t, _vp, _u64, _u64, _u64, _vp, _vp, _vp, _vp]),
+    "lcpp_token_spread": (_i, [_i, _vp, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _u64, _vp]),
+    "lcpp_token_sum": (_i, [_i, _vp, _u64, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _vp]),
+    "lcpp_expert_product": (_i, [_i, _vp, _u64, _vp, _u64, _u64, _vp, _i, _vp, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64,
+                                 _vp]),
+    "lcpp_expert_product_backward": (_i, [_i, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _vp, _vp, _u64, _i, _vp, _u64, _u64, _u64, _u64,
+                                          _u64, _u64, _vp]),
     "lcpp_temp_status": (_i, [_vp, ctypes.c_size_t, _vp]),
     "lcpp_temp_status_record": (_i, [_vp, ctypes.c_size_t, _vp, _vp]),
     "lcpp_device_status_decode": (_i, [ctypes.c_uint32]),
@@ -174,6 +191,26 @@ def float_code(dtype) -> int:
         raise TypeError(f"unsupported dtype {dtype}: float32, bfloat16 or float16")
     try:
         _float_codes[dtype] = code
+    except TypeError:  # not hashable
+        pass
+    return code
+
+
+_quant_codes: dict = {}
+
+
+def quant_code(dtype) -> int:
+    """lcpp_dtype of an 8-bit floating type: float8_e4m3fn or float8_e5m2."""
+    try:
+        return _quant_codes[dtype]
+    except (KeyError, TypeError):
+        pass
+    name = str(dtype).replace("torch.", "")
+    code = {"float8_e4m3fn": LCPP_FLOAT8_E4M3, "float8_e5m2": LCPP_FLOAT8_E5M2}.get(name)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}: float8_e4m3fn or float8_e5m2")
+    try:
+        _quant_codes[dtype] = code
     except TypeError:  # not hashable
         pass
     return code

@@ -1,5 +1,5 @@
-"""The operators of a recurrent language model's residual block: layer norm,
-dropout and the gated linear recurrence, forward and backward.
+"""The operators of a recurrent language model's residual block: layer norm, RMS
+norm, dropout and the gated linear recurrence, forward and backward.
 
 The reference has none of them; they follow its manner here as the classes of
 device.py do: caller-owned outputs and temp storage, an asynchronous call on a
@@ -22,7 +22,7 @@ from __future__ import annotations
 import ctypes
 import functools
 
-from ._capi import LCPP_GATES, _float_codes, check, float_code, lib
+from ._capi import LCPP_GATES, _float_codes, check, float_code, lib, quant_code
 from .device import _Module, _ptr, _query, _stream
 
 
@@ -231,6 +231,76 @@ class DeviceLayerNorm(_BlockModule):
                    _float_vector(d_rstd, rows, "d_rstd"), p, seed, offset, _counter(d_offset, "d_offset"),
                    _ptr(d_grad_residual), sr, _ptr(d_grad_in), si, _vector(d_grad_weight, cols, "d_grad_weight"),
                    _vector(d_grad_bias, cols, "d_grad_bias"), rows, cols)
+
+
+def _scales(t, rows: int, cols: int, group: int):
+    """(address, row stride, group stride) of the scales of rows in 8 bits."""
+    groups = -(-cols // group) if group else 1 if cols else 0
+    if t is None or t.dtype is None or tuple(t.shape) != (rows, groups):
+        raise ValueError(f"d_scales: shape {None if t is None else tuple(t.shape)}, expected {(rows, groups)}")
+    if float_code(t.dtype) != 2:
+        raise TypeError(f"d_scales: must be float32, got {t.dtype}")
+    if not t.is_cuda:
+        _off_gpu(t, "d_scales")
+    return t.data_ptr(), *t.stride()
+
+
+class DeviceRMSNorm(_BlockModule):
+    """y = s / sqrt(mean(s^2) + eps) * weight over the rows of s, in the rows' type, in 8 bits with scales, or both.
+
+    In 8 bits: d_quant of type float8_e4m3fn or float8_e5m2, and float32 d_scales of shape (rows, ceil(columns /
+    group)) with any strides: for each row and `group` columns (32, 64, 128, 256 or 512; 0: the whole row) scale =
+    max(max |y|, 2^-100) / (the type's largest value), and d_quant = y / scale, of y before it is rounded to the rows'
+    type.  A group with a value that is not finite has the scale NaN and values NaN.  d_out may then be None."""
+
+    @staticmethod
+    def GetBackwardTempStorageBytes(dtype, rows: int, cols: int) -> int:
+        return _query(lib().lcpp_rms_norm_backward_temp_bytes, float_code(dtype), rows, cols)
+
+    def _forward(self, d_in, d_residual, d_sum, d_out, d_weight, eps, d_rstd, d_quant, d_scales, group, stream):
+        dtype = d_in.dtype
+        code = float_code(dtype)
+        shape, rows, cols, si = _matrix(d_in, "d_in")
+        residual, total = (None, 0), (None, 0)
+        if d_residual is not None:
+            residual = d_residual.data_ptr(), _like(d_residual, shape, dtype, "d_residual")
+            total = d_sum.data_ptr(), _like_out(d_sum, shape, dtype, "d_sum")
+        out = (None, 0) if d_out is None else (d_out.data_ptr(), _like_out(d_out, shape, dtype, "d_out"))
+        quant = 0, None, 0, None, 0, 0, 0
+        if d_quant is not None:
+            quant = (quant_code(d_quant.dtype), d_quant.data_ptr(), _like_out(d_quant, shape, d_quant.dtype, "d_quant"),
+                     *_scales(d_scales, rows, cols, group), group)
+        elif d_out is None:
+            raise ValueError("d_out or d_quant must be given")
+        self._call("lcpp_rms_norm_forward", None, _stream(stream), code, _weight_code(code, d_weight), d_in.data_ptr(), si,
+                   *residual, _vector(d_weight, cols, "d_weight"), eps, *total, *out, _float_vector(d_rstd, rows, "d_rstd"),
+                   *quant, rows, cols)
+
+    def Forward(self, d_in, d_out, d_weight=None, eps: float = 1e-6, d_rstd=None, d_quant=None, d_scales=None,
+                group: int = 128, stream=None):
+        """d_out = the RMS norm of d_in; d_rstd: float32 row statistics for Backward, or None."""
+        self._forward(d_in, None, None, d_out, d_weight, eps, d_rstd, d_quant, d_scales, group, stream)
+
+    def AddForward(self, d_in, d_residual, d_sum, d_out, d_weight=None, eps: float = 1e-6, d_rstd=None, d_quant=None,
+                   d_scales=None, group: int = 128, stream=None):
+        """d_sum = d_residual + d_in, and the RMS norm of d_sum as it is stored; d_sum may be d_residual or d_in, but
+        not d_out."""
+        self._forward(d_in, d_residual, d_sum, d_out, d_weight, eps, d_rstd, d_quant, d_scales, group, stream)
+
+    def Backward(self, temp_storage, d_grad_out, d_in, d_weight, d_rstd, d_grad_in, d_grad_weight=None, d_grad_sum=None,
+                 stream=None):
+        """The gradients of Forward's d_in (AddForward's: d_in is its d_sum, and d_grad_in the gradient of d_in and of
+        d_residual) and d_weight (None if not wanted).  d_grad_sum: what reaches d_sum along the residual path (None:
+        nothing).  The 8-bit output's gradient is taken as d_out's."""
+        shape, dtype, code, rows, cols, si, so = _in_out(d_in, d_grad_in, "d_in", "d_grad_in")
+        sg = _like(d_grad_out, shape, dtype, "d_grad_out")
+        sx = 0 if d_grad_sum is None else _like(d_grad_sum, shape, dtype, "d_grad_sum")
+        # (a call of nothing may launch nothing and leave the status word)
+        self._call("lcpp_rms_norm_backward", temp_storage if rows and cols else None, _stream(stream), code,
+                   _weight_code(code, d_weight, d_grad_weight), *_temp(temp_storage), d_grad_out.data_ptr(), sg,
+                   _ptr(d_grad_sum), sx, d_in.data_ptr(), si, _vector(d_weight, cols, "d_weight"),
+                   _float_vector(d_rstd, rows, "d_rstd"), d_grad_in.data_ptr(), so,
+                   _vector(d_grad_weight, cols, "d_grad_weight"), rows, cols)
 
 
 class DeviceDropout(_BlockModule):
