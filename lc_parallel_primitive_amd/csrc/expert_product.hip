@@ -47,7 +47,6 @@ struct ProductArgs {
 };
 
 constexpr uint32_t kChunk = 16;         // bytes
-constexpr uint32_t kStageBytes = 128;   // of c
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -59,7 +58,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kOutside = 0xFFFFFF00u;
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t voff, uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc) : "memory");
 }
 __device__ __forceinline__ u32x4 stage_rsrc(const void *p)
 {
@@ -71,63 +70,78 @@ __device__ __forceinline__ u32x4 stage_rsrc(const void *p)
     r.w = (uint32_t)kRawBufferWord3;
     return r;
 }
-// Every wave's loads to LDS have arrived, and every wave has read what it needed before.
+// Every wave's loads to LDS but the last LATER ones have arrived, and every wave has read what
+// it needed before.
+template <int LATER = 0>
 __device__ __forceinline__ void stage_barrier()
 {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // ---------------------------------------------------------------- an operand's stage
-// X elements (rows or columns of the operand) x 128 bytes of c.  ACROSS: c runs from row to
-// row, X columns in each; else X rows with c along them.
-template <class T, uint32_t X, uint32_t THREADS, bool ACROSS>
+// X elements (rows or columns of the operand) x BYTES of c.  ACROSS: c runs from row to row,
+// X columns in each; else X rows with c along them.
+template <class T, uint32_t X, uint32_t BYTES, uint32_t THREADS, bool ACROSS>
 struct Stage {
     static constexpr uint32_t kElems = kChunk / sizeof(T);         // of a chunk
-    static constexpr uint32_t kDepth = kStageBytes / sizeof(T);    // of c
-    static constexpr uint32_t kRowChunks = ACROSS ? X / kElems : kStageBytes / kChunk;
-    static constexpr uint32_t kBytes = X * kStageBytes;
+    static constexpr uint32_t kDepth = BYTES / sizeof(T);          // of c
+    static constexpr uint32_t kRowChunks = ACROSS ? X / kElems : BYTES / kChunk;
+    static constexpr uint32_t kBytes = X * BYTES;
     static constexpr uint32_t kLoads = kBytes / kChunk / THREADS;  // of a thread
     static_assert(kBytes % (kChunk * THREADS) == 0, "whole loads");
-    // where chunk c of a row is kept
-    static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return ACROSS ? (row & 3) << 2 : (row >> 1) & 7; }
+    // Chunk c of a row is kept in place c ^ swizzle(row).  Along: the 16 rows that a read touches at
+    // once fill the 256 bytes of all banks, rows of 64 bytes by fours and rows of 128 by twos.  Across:
+    // the four rows of a transposing read have 64 bytes each.
+    static __device__ __forceinline__ uint32_t swizzle(uint32_t row)
+    {
+        static_assert(BYTES == 64 || BYTES == 128, "rows of 4 or 8 chunks");
+        return ACROSS ? (row & 3) << 2 : BYTES == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+    }
 
     const T *base;     // of the tile
     uint64_t stride;   // of rows, in elements
     uint32_t valid;    // of X
     uint32_t depth;    // of c in all
-    uint32_t row[kLoads], chunk[kLoads], off[kLoads];
+    // of the thread's chunk 0; the others are kRowStep rows apart and have the same chunk, the rows' swizzles repeating
+    // after as many
+    static constexpr uint32_t kRowStep = THREADS / kRowChunks;
+    static_assert(THREADS % kRowChunks == 0 && kRowStep % (ACROSS ? 4 : 16) == 0, "the same swizzle");
+    uint32_t row, chunk;
+    uint32_t off[kLoads];
 
-    __device__ __forceinline__ Stage(const T *p, uint64_t s, uint32_t x, uint32_t c) : base(p), stride(s), valid(x), depth(c)
+    __device__ __forceinline__ void set(const T *p, uint64_t s, uint32_t x, uint32_t c)
     {
+        base = p, stride = s, valid = x, depth = c;
+        row = threadIdx.x / kRowChunks;
+        chunk = (threadIdx.x % kRowChunks) ^ swizzle(row);
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t slot = i * THREADS + threadIdx.x;
-            row[i] = slot / kRowChunks;
-            chunk[i] = (slot % kRowChunks) ^ swizzle(row[i]);
+            const uint32_t r = row + i * kRowStep;
             if constexpr (ACROSS) {
-                off[i] = chunk[i] * kElems < valid ? (uint32_t)(row[i] * stride * sizeof(T)) + chunk[i] * kChunk : kOutside;
+                off[i] = chunk * kElems < valid ? (uint32_t)(r * stride * sizeof(T)) + chunk * kChunk : kOutside;
             } else {
                 // (rows past the last one are the last one again, and are not stored)
-                const uint32_t r = row[i] < valid ? row[i] : valid - 1;
-                off[i] = (uint32_t)(r * stride * sizeof(T)) + chunk[i] * kChunk;
+                off[i] = (uint32_t)((r < valid ? r : valid - 1) * stride * sizeof(T)) + chunk * kChunk;
             }
         }
     }
-    // The stage from c = from on, all of whose chunks are aligned and whole.
+    // Load i of the stage from c = from on, all of whose chunks are aligned and whole; 0 past the end.
+    __device__ __forceinline__ u32x4 source(uint32_t from) const { return stage_rsrc(base + (ACROSS ? from * stride : from)); }
+    __device__ __forceinline__ void issue_one(uint32_t i, u32x4 rsrc, uint32_t from, uint32_t lds) const
+    {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        uint32_t v = off[i];
+        if (from + (ACROSS ? row + i * kRowStep : chunk * kElems) >= depth) v = kOutside;
+        load_to_lds(rsrc, v, lds + (i * THREADS + wave * kWave) * kChunk);
+    }
     __device__ __forceinline__ void issue(uint32_t from, uint32_t lds) const
     {
-        const u32x4 rsrc = stage_rsrc(base + (ACROSS ? from * stride : from));
-        const bool last = from + kDepth > depth;
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        const u32x4 rsrc = source(from);
 #pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            uint32_t v = off[i];
-            if (last && from + (ACROSS ? row[i] : chunk[i] * kElems) >= depth) v = kOutside;
-            load_to_lds(rsrc, v, lds + (i * THREADS + wave * kWave) * kChunk);
-        }
+        for (uint32_t i = 0; i < kLoads; ++i) issue_one(i, rsrc, from, lds);
     }
     // The same by way of registers, for any stride, size and alignment.
     struct Held {
@@ -137,9 +151,9 @@ struct Stage {
     {
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t c = from + (ACROSS ? row[i] : chunk[i] * kElems);
-            const uint32_t r = ACROSS ? 0 : row[i] < valid ? row[i] : valid - 1;
-            const uint32_t inside = ACROSS ? valid : depth, at = ACROSS ? chunk[i] * kElems : c;
+            const uint32_t line = row + i * kRowStep, c = from + (ACROSS ? line : chunk * kElems);
+            const uint32_t r = ACROSS ? 0 : line < valid ? line : valid - 1;
+            const uint32_t inside = ACROSS ? valid : depth, at = ACROSS ? chunk * kElems : c;
             const bool there = c < depth && at < inside;
             const T *p = base + (ACROSS ? c * stride + at : r * stride + c);
             typedef T vec __attribute__((ext_vector_type(kElems)));
@@ -168,7 +182,7 @@ struct Stage {
     static __device__ __forceinline__ u32x4 along(const char *lds, uint32_t x, uint32_t chunk)
     {
         const uint32_t r = x + lane_id() % 32;
-        return *reinterpret_cast<const u32x4 *>(lds + r * kStageBytes + ((chunk ^ swizzle(r)) * kChunk));
+        return *reinterpret_cast<const u32x4 *>(lds + r * BYTES + ((chunk ^ swizzle(r)) * kChunk));
     }
     static __device__ __forceinline__ uint32_t across_at(uint32_t row, uint32_t col)
     {
@@ -224,73 +238,137 @@ __device__ __forceinline__ f32x16 multiply(u32x4 l, u32x4 r, f32x16 acc, float)
 }
 
 // ---------------------------------------------------------------- tiles
-// The tile of a workgroup.  Those of one expert lie one behind the other, m fastest; each
-// XCD, which get the workgroups in turn, works on neighbouring ones, which share operands in
-// its L2.
-struct Tile {
-    uint32_t expert, m, n;  // numbers of the tile's first row and column, in tiles
-    int64_t first;          // the expert's rows
-    uint32_t count;
-};
-template <Product P>
-__device__ __forceinline__ bool find_tile(const ProductArgs &a, uint32_t tm, uint32_t tn, Tile &t)
+// The tiles of an expert lie one behind the other, kBand rows of tiles at a time, m fastest: the
+// 32 that the CUs of an XCD have at once are 8 x 4 and share operands in its L2.
+constexpr uint32_t kBand = 8;
+__device__ __forceinline__ void tile_place(uint32_t in, uint32_t mt, uint32_t nt, uint32_t &m, uint32_t &n)
 {
-    const uint32_t nt = (a.n + tn - 1) / tn;
-    constexpr uint32_t kXcds = 8;
-    const uint32_t lane = lane_id();
-    auto span = [&](uint32_t e, int64_t &first, uint32_t &count) {
-        int64_t b = a.offsets[e], z = a.offsets[e + 1];
-        b = b < 0 ? 0 : b;
-        z = z > (int64_t)a.rows ? (int64_t)a.rows : z;
-        first = b;
-        count = z > b ? (uint32_t)(z - b) : 0;
-    };
-    uint32_t all = 0, id = blockIdx.x;
-    if constexpr (P == Product::kGradMatrix) {
-        const uint32_t mt = (a.m + tm - 1) / tm, each = mt * nt;
-        const uint32_t per = (a.experts * each + kXcds - 1) / kXcds;
-        id = id % kXcds * per + id / kXcds;
-        if (blockIdx.x / kXcds >= per || id >= a.experts * each) return false;
-        t.expert = id / each;
-        const uint32_t in = id - t.expert * each;
-        t.n = in / mt;
-        t.m = in - t.n * mt;
-        span(t.expert, t.first, t.count);
-        return true;
-    }
-    for (uint32_t e = 0; e < a.experts; e += kWave) {
-        int64_t first;
-        uint32_t count = 0;
-        if (e + lane < a.experts) span(e + lane, first, count);
-        all += wave_reduce_dpp((count + tm - 1) / tm, SumOp());
-    }
-    const uint32_t per = (all * nt + kXcds - 1) / kXcds;
-    id = id % kXcds * per + id / kXcds;
-    if (blockIdx.x / kXcds >= per || id >= all * nt) return false;
-    uint32_t before = 0;
-    for (uint32_t e = 0; e < a.experts; e += kWave) {
-        int64_t first = 0;
-        uint32_t count = 0;
-        if (e + lane < a.experts) span(e + lane, first, count);
-        const uint32_t tiles = (count + tm - 1) / tm;
-        const uint32_t sum = wave_inclusive_scan(tiles, SumOp());
-        const uint64_t past = ballot((before + sum) * nt > id);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            t.expert = e + at;
-            t.first = read_lane(first, at);
-            t.count = read_lane(count, at);
-            const uint32_t mt = read_lane(tiles, at), in = id - (before + read_lane(sum, at) - mt) * nt;
-            t.n = in / mt;
-            t.m = in - t.n * mt;
-            return true;
-        }
-        before += read_lane(sum, kWave - 1);
-    }
-    return false;
+    const uint32_t band = in / (kBand * nt), from = band * kBand, high = mt - from < kBand ? mt - from : kBand;
+    in -= from * nt;
+    n = in / high;
+    m = from + in - n * high;
 }
 
-template <class T, class O>
+constexpr uint32_t kProductExperts = 1024;  // at most
+constexpr uint32_t kXcds = 8;
+struct Tile {
+    uint32_t expert, m, n;  // numbers of the tile's first row and column, in tiles
+    uint32_t first, count;  // the expert's rows
+    bool there;
+};
+// The experts with their rows, and the number of tiles before each, in LDS.  A workgroup takes
+// one tile after the other, without asking the others.  Forward and grad rows, whose tiles take
+// the same time: the XCDs, which get the workgroups in turn, have an eighth of all tiles each.
+// Grad matrix, whose tiles take as long as their expert has rows: experts with many rows come
+// first, and chunks of tiles, one for each workgroup of an XCD, go to the XCD that has least to do
+// so far, which every workgroup works out for itself (32768 rows, 16 experts of 2816 x 2048, the
+// largest with a quarter of the rows: 985 us with an eighth each in the experts' order, 484
+// with chunks dealt to and fro).  Past kChunks they are dealt to and fro.
+template <Product P, int TM, int TN, int THREADS>
+struct Tiles {
+    uint32_t start[kProductExperts + 1];
+    uint32_t first[kProductExperts], count[kProductExperts];
+    uint16_t order[kProductExperts];
+    static constexpr uint32_t kChunks = P == Product::kGradMatrix ? 512 : 1;
+    uint16_t mine[kChunks];  // the chunks of this workgroup's XCD
+    uint32_t mine_count;
+    uint32_t wave_sum[THREADS / kWave];
+    uint32_t all;
+
+    __device__ __forceinline__ void make(const ProductArgs &a)
+    {
+        const uint32_t tid = threadIdx.x, nt = (a.n + TN - 1) / TN;
+        for (uint32_t e = tid; e < a.experts; e += THREADS) {
+            int64_t b = a.offsets[e], z = a.offsets[e + 1];
+            b = b < 0 ? 0 : b;
+            z = z > (int64_t)a.rows ? (int64_t)a.rows : z;
+            first[e] = (uint32_t)b;
+            count[e] = z > b ? (uint32_t)(z - b) : 0;
+            order[e] = (uint16_t)e;
+        }
+        __syncthreads();
+        if constexpr (P == Product::kGradMatrix) {
+            for (uint32_t e = tid; e < a.experts; e += THREADS) {
+                const uint32_t mine = count[e];
+                uint32_t rank = 0;
+                for (uint32_t j = 0; j < a.experts; ++j) rank += count[j] > mine || (count[j] == mine && j < e);
+                order[rank] = (uint16_t)e;
+            }
+            __syncthreads();
+        }
+        uint32_t before = 0;
+        for (uint32_t base = 0; base < a.experts; base += THREADS) {
+            const uint32_t i = base + tid;
+            uint32_t tiles = 0;
+            if (i < a.experts) tiles = nt * (P == Product::kGradMatrix ? (a.m + TM - 1) / TM : (count[order[i]] + TM - 1) / TM);
+            const uint32_t sum = wave_inclusive_scan(tiles, SumOp());
+            if (lane_id() == kWave - 1) wave_sum[tid / kWave] = sum;
+            __syncthreads();
+            uint32_t s = before + sum - tiles;
+            for (uint32_t w = 0; w < THREADS / kWave; ++w) {
+                if (w < tid / kWave) s += wave_sum[w];
+                before += wave_sum[w];
+            }
+            if (i < a.experts) start[i] = s;
+            __syncthreads();
+        }
+        if (tid == 0) start[a.experts] = all = before;
+        __syncthreads();
+        if constexpr (P == Product::kGradMatrix) {
+            const uint32_t side = gridDim.x / kXcds, chunks = (before + side - 1) / side;
+            if (chunks <= kChunks && tid < kWave) {
+                // a lane for each XCD holds what it has to do; a stage and a tile's end take about 64 rows' time each
+                const uint32_t lane = lane_id();
+                uint32_t load = lane < kXcds ? 0 : 0xFFFFFFFFu, e = 0, n = 0;
+                for (uint32_t c = 0; c < chunks; ++c) {
+                    while (start[e + 1] <= c * side) ++e;
+                    const uint32_t key = lane < kXcds ? load << 3 | lane : 0xFFFFFFFFu;
+                    const uint32_t xcd = wave_reduce_dpp(key, MinOp()) & 7;
+                    if (lane == xcd) load += (count[order[e]] + 63) / 64 + 6;
+                    if (xcd == blockIdx.x % kXcds) mine[n++] = (uint16_t)c;
+                }
+                mine_count = n;
+            }
+            __syncthreads();
+        }
+    }
+    // The workgroup's tile number `turn`, which may not be there.
+    __device__ __forceinline__ Tile get(const ProductArgs &a, uint32_t turn) const
+    {
+        Tile t = {};
+        const uint32_t xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds, side = gridDim.x / kXcds;
+        const uint32_t total = __builtin_amdgcn_readfirstlane(all);
+        uint32_t id;
+        if constexpr (P == Product::kGradMatrix) {
+            const bool listed = (total + side - 1) / side <= kChunks;
+            uint32_t chunk = turn * kXcds + (turn & 1 ? kXcds - 1 - xcd : xcd);
+            if (listed) {
+                if (turn >= __builtin_amdgcn_readfirstlane(mine_count)) return t;
+                chunk = __builtin_amdgcn_readfirstlane(mine[turn]);
+            }
+            id = chunk * side + slot;
+        } else {
+            const uint32_t per = (total + kXcds - 1) / kXcds, in = turn * side + slot;
+            id = in < per ? xcd * per + in : total;
+        }
+        if (id >= total) return t;
+        uint32_t lo = 0, hi = a.experts;  // start[lo] <= id < start[hi]
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (__builtin_amdgcn_readfirstlane(start[mid]) <= id) lo = mid;
+            else hi = mid;
+        }
+        t.expert = __builtin_amdgcn_readfirstlane(order[lo]);
+        t.first = __builtin_amdgcn_readfirstlane(first[t.expert]);
+        t.count = __builtin_amdgcn_readfirstlane(count[t.expert]);
+        const uint32_t nt = (a.n + TN - 1) / TN, mt = ((P == Product::kGradMatrix ? a.m : t.count) + TM - 1) / TM;
+        tile_place(id - __builtin_amdgcn_readfirstlane(start[lo]), mt, nt, t.m, t.n);
+        t.there = true;
+        return t;
+    }
+};
+
+template <class O>
 __device__ __forceinline__ void store_four(O *row, uint32_t col, uint32_t cols, const float (&x)[4])
 {
     if (col + 4 <= cols) store_pack<4>(row + col, x);
@@ -300,33 +378,312 @@ __device__ __forceinline__ void store_four(O *row, uint32_t col, uint32_t cols, 
             if (col + i < cols) row[col + i] = (O)x[i];
 }
 
-// A workgroup of WM x WN waves makes TM x TN outputs.  ALIGNED: chunks are whole and aligned.
-template <class T, class O, Product P, int TM, int TN, int WM, int WN, bool ALIGNED>
+// The operands of a tile, from its first row and column on.
+template <Product P, class E>
+__device__ __forceinline__ void tile_operands(const ProductArgs &a, const Tile &t, uint32_t m0, uint32_t n0, const E *&lp, const E *&rp,
+                                              uint32_t &rows, uint32_t &depth)
+{
+    rows = P == Product::kGradMatrix ? a.m : t.count;  // of the output
+    depth = P == Product::kGradMatrix ? t.count : a.c;
+    lp = static_cast<const E *>(a.l), rp = static_cast<const E *>(a.r);
+    if constexpr (P == Product::kForward) lp += t.expert * a.l_expert + n0 * a.l_stride;
+    else if constexpr (P == Product::kGradRows) lp += t.expert * a.l_expert + n0;
+    else lp += (uint64_t)t.first * a.l_stride + n0;
+    if constexpr (P == Product::kGradMatrix) rp += (uint64_t)t.first * a.r_stride + m0;
+    else rp += (uint64_t)(t.first + m0) * a.r_stride;
+}
+
+// f(0) .. f(N - 1), as integral constants.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each_of(F f)
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        each_of<N, I + 1>(f);
+    }
+}
+
+// Results of 2-byte types.  A lane has column m = lane % 32 of an instruction's result and the rows
+// 8 q + 4 (lane / 32) .. + 4 of n; exchanges between the halves and the quarters of the wave make
+// that eight neighbouring n of one m, four lanes of which fill 64 bytes of a row of the
+// output: chunk (lane / 16) with its bits exchanged, of row lane % 16 and 16 + lane % 16.
+// (With four n a lane, in 16-byte pieces, the requests to the L2 took 10 us for 256 tiles of
+// 256 x 256.)
+template <class O>
+constexpr bool kPacked = sizeof(O) == 2;
+template <class O>
+__device__ __forceinline__ void pack_rows(const f32x16 &acc, u32x4 (&rows)[2])
+{
+    uint32_t p[4][2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        typedef O v4 __attribute__((ext_vector_type(4)));
+        v4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (O)acc[4 * q + k];
+        const uint2 w = __builtin_bit_cast(uint2, v);
+        p[q][0] = w.x, p[q][1] = w.y;
+    }
+    uint32_t half[2][4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const auto w = __builtin_amdgcn_permlane32_swap(p[2 * c][d], p[2 * c + 1][d], false, false);
+            half[c][d] = w[0], half[c][2 + d] = w[1];
+        }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const auto w = __builtin_amdgcn_permlane16_swap(half[0][d], half[1][d], false, false);
+        rows[0][d] = w[0], rows[1][d] = w[1];
+    }
+}
+__device__ __forceinline__ uint32_t packed_chunk()
+{
+    const uint32_t g = lane_id() / 16;
+    return g >> 1 | (g & 1) << 1;
+}
+// 16 bytes to a row, counted by what waits for the loads around them.  (The values have been
+// converted, so no matrix instruction's result is stored directly.)
+template <int OFFSET>
+__device__ __forceinline__ void store_counted(void *p, u32x4 v)
+{
+    asm volatile("global_store_dwordx4 %0, %1, off offset:%2\n\ts_nop 0" ::"v"(p), "v"(v), "n"(OFFSET) : "memory");
+}
+template <class O, int FM, int FN>
+__device__ __forceinline__ void store_whole_tile(O *out, uint64_t stride, const f32x16 (&acc)[FN][FM])
+{
+    O *row = out + lane_id() % 16 * stride + packed_chunk() * 8;
+#pragma unroll
+    for (int j = 0; j < FM; ++j, row += 32 * stride) {
+        each_of<FN>([&](auto i) {
+            u32x4 v[2];
+            pack_rows<O>(acc[decltype(i)::value][j], v);
+            store_counted<decltype(i)::value * 64>(row, v[0]);
+            store_counted<decltype(i)::value * 64>(row + 16 * stride, v[1]);
+        });
+    }
+}
+
+// A lane has column m of the instructions' results and rows 8 q + 4 (lane / 32) .. + 4 of n.
+template <Product P, class O, int FM, int FN>
+__device__ __forceinline__ void store_tile(const ProductArgs &a, const Tile &t, const f32x16 (&acc)[FN][FM], uint32_t m0, uint32_t n0,
+                                           uint32_t rows)
+{
+    O *out = static_cast<O *>(a.o);
+    if constexpr (P == Product::kGradMatrix) out += t.expert * a.o_expert;
+    else out += (uint64_t)t.first * a.o_stride;
+    const uint32_t lane = lane_id();
+    if constexpr (kPacked<O>) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                u32x4 v[2];
+                pack_rows<O>(acc[i][j], v);
+                const uint32_t n = n0 + i * 32 + packed_chunk() * 8;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t m = m0 + j * 32 + h * 16 + lane % 16;
+                    if (m >= rows || n >= a.n) continue;
+                    Octet<O> x;
+                    __builtin_memcpy(&x.v, &v[h], sizeof(x.v));
+                    O *at = out + m * a.o_stride + n;
+                    if (n + kOctet <= a.n) *reinterpret_cast<typename Octet<O>::vec_u *>(at) = x.v;
+                    else
+#pragma unroll
+                        for (uint32_t k = 0; k < kOctet; ++k)
+                            if (n + k < a.n) at[k] = x.v[k];
+                }
+            }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const uint32_t m = m0 + j * 32 + lane % 32;
+        if (m >= rows) continue;
+        O *row = out + m * a.o_stride;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t n = n0 + i * 32 + q * 8 + lane / 32 * 4;
+                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                if (n < a.n) store_four(row, n, a.n, v);
+            }
+    }
+}
+
+// A workgroup of WM x WN waves makes tiles of TM x TN outputs, one after the other, from operands
+// whose chunks are whole and aligned.  The stages of all its tiles are one stream: loads for a
+// tile begin while the one before is multiplied.  Fragments are read one step ahead into the
+// other of two sets of registers, loads and reads are issued between the matrix instructions, and
+// a stage's barrier comes before its last step: by then every wave has that step's fragments, so
+// the stage's place is free for the loads of the stage BUFS later, and the next stage, whose first
+// fragments are read now, has arrived.
+template <class T, class O, Product P, int TM, int TN, int WM, int WN, int BYTES, int BUFS>
 __global__ __launch_bounds__(WM *WN *kWave) void product_kernel(ProductArgs a)
 {
     constexpr uint32_t THREADS = WM * WN * kWave;
+    constexpr int FM = TM / WM / 32, FN = TN / WN / 32, STEPS = BYTES / 32, kProducts = FM * FN;
+    constexpr bool kLeftAcross = P != Product::kForward, kRightAcross = P == Product::kGradMatrix;
+    using Left = Stage<T, TN, BYTES, THREADS, kLeftAcross>;
+    using Right = Stage<T, TM, BYTES, THREADS, kRightAcross>;
+    constexpr uint32_t kBytes = Left::kBytes + Right::kBytes;
+    constexpr int kLoads = Left::kLoads + Right::kLoads, kStores = kPacked<O> ? FM * FN * 2 : 0;
+    static_assert(kStores + (BUFS - 2) * kLoads < 64, "the counter of memory operations");
+    static_assert(BUFS >= 2 && STEPS % 2 == 0, "a stage ahead, and both sets of registers in turn");
+    __shared__ __attribute__((aligned(256))) char lds[BUFS * kBytes];
+    __shared__ Tiles<P, TM, TN, (int)THREADS> tiles;
+
+    tiles.make(a);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t wm = wave % WM * (TM / WM), wn = wave / WM * (TN / WN);
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
+
+    // Load r of a stage belongs to its step `portion`, counted from the step that frees its place: spread over
+    // a stage, or at once where no other stage is on its way.
+    auto portion = [](int r) { return BUFS > 2 ? r * STEPS / kLoads : 0; };
+    // what is loaded next: a stage of a tile that comes later
+    Left left;
+    Right right;
+    uint32_t load_turn = 0, load_from = 0, load_depth = 0;
+    bool load_more = true;
+    // the next stage, of the next tile that has any; past the last one loads give 0
+    auto next_stage = [&] {
+        load_from += Left::kDepth;
+        while (load_from >= load_depth && load_more) {
+            const Tile t = tiles.get(a, load_turn++);
+            load_more = t.there;
+            if (!load_more) break;
+            uint32_t rows;
+            const T *lp, *rp;
+            const uint32_t m0 = t.m * TM, n0 = t.n * TN;
+            tile_operands<P>(a, t, m0, n0, lp, rp, rows, load_depth);
+            load_from = 0;
+            if (load_depth == 0) continue;
+            left.set(lp, a.l_stride, a.n - n0, load_depth);
+            right.set(rp, a.r_stride, rows - m0, load_depth);
+        }
+    };
+    uint32_t turn = 0;
+    Tile t = tiles.get(a, turn++);
+    if (!t.there) return;
+    next_stage();
+    u32x4 w[2][FN], x[2][FM];
+    uint32_t at = 0, load_at = (BUFS - 1) * kBytes;  // of the stage that is multiplied, and loaded, in LDS
+    if (load_more) {
+#pragma unroll
+        for (int s = 0; s < BUFS; ++s) {
+            if (s) next_stage();
+            const u32x4 left_src = left.source(load_from), right_src = right.source(load_from);
+#pragma unroll
+            for (int r = 0; r < kLoads; ++r) {
+                if (s + 1 == BUFS && portion(r) > 0) continue;
+                if (r < (int)Left::kLoads) left.issue_one(r, left_src, load_from, lds0 + s * kBytes);
+                else right.issue_one(r - Left::kLoads, right_src, load_from, lds0 + s * kBytes + Left::kBytes);
+            }
+        }
+        stage_barrier<(BUFS - 2) * kLoads>();
+#pragma unroll
+        for (int j = 0; j < FM; ++j) x[0][j] = Right::fragment(lds + Left::kBytes, wm + j * 32, 0);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) w[0][i] = Left::fragment(lds, wn + i * 32, 0);
+    }
+    bool stores = false;  // this wave's last kStores memory operations are those of a whole tile
+    for (;;) {
+        const uint32_t rows = P == Product::kGradMatrix ? a.m : t.count, depth = P == Product::kGradMatrix ? t.count : a.c;
+        f32x16 acc[FN][FM];
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) acc[i][j] = f32x16{};
+        for (uint32_t s = 0; s < depth; s += Left::kDepth) {
+            const uint32_t next = at + kBytes == BUFS * kBytes ? 0 : at + kBytes;
+            u32x4 left_src = left.source(load_from), right_src = right.source(load_from);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                const bool last = k + 1 == STEPS;
+                if (last) {
+                    // (a tile's stores were issued after the loads of its successor's first stages)
+                    if (stores) stage_barrier<(BUFS - 2) * kLoads + kStores>();
+                    else stage_barrier<(BUFS - 2) * kLoads>();
+                    stores = false;
+                    next_stage();
+                    load_at = at;
+                    left_src = left.source(load_from), right_src = right.source(load_from);
+                }
+                const char *ll = lds + (last ? next : at), *lr = ll + Left::kBytes;
+                const int set = k & 1, other = set ^ 1, step = (k + 1) % STEPS;
+#pragma unroll
+                for (int q = 0; q < kProducts; ++q) {
+                    // what is issued before product q: reads in the first half of the step, loads in the last step
+#pragma unroll
+                    for (int r = 0; r < FM + FN; ++r) {
+                        if (r * kProducts / (2 * (FM + FN)) != q) continue;
+                        if (r < FM) x[other][r] = Right::fragment(lr, wm + r * 32, step);
+                        else w[other][r - FM] = Left::fragment(ll, wn + (r - FM) * 32, step);
+                    }
+#pragma unroll
+                    for (int r = 0; r < kLoads; ++r) {
+                        if (portion(r) != step) continue;
+                        if ((BUFS > 2 ? r * STEPS % kLoads * kProducts / kLoads : r * kProducts / kLoads) != q) continue;
+                        if (r < (int)Left::kLoads) left.issue_one(r, left_src, load_from, lds0 + load_at);
+                        else right.issue_one(r - Left::kLoads, right_src, load_from, lds0 + load_at + Left::kBytes);
+                    }
+                    acc[q / FM][q % FM] = multiply(w[set][q / FM], x[set][q % FM], acc[q / FM][q % FM], T());
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            at = next;
+        }
+        const uint32_t m0 = t.m * TM + wm, n0 = t.n * TN + wn;
+        bool whole = false;
+        if constexpr (kPacked<O> && BUFS == 2) {
+            whole = m0 + TM / WM <= rows && n0 + TN / WN <= a.n;
+            if (whole) {
+                O *out = static_cast<O *>(a.o);
+                if constexpr (P == Product::kGradMatrix) out += t.expert * a.o_expert;
+                else out += (uint64_t)t.first * a.o_stride;
+                store_whole_tile(out + m0 * a.o_stride + n0, a.o_stride, acc);
+            }
+        }
+        if (!whole) store_tile<P, O>(a, t, acc, m0, n0, rows);
+        stores = whole;
+        t = tiles.get(a, turn++);
+        if (!t.there) break;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the zeros past the end)
+}
+
+// Any stride, size and alignment by way of registers, and 8-bit operands: two stages of 128 bytes
+// of c.
+template <class T, class O, Product P, int TM, int TN, int WM, int WN, bool ALIGNED>
+__global__ __launch_bounds__(WM *WN *kWave) void product_simple_kernel(ProductArgs a)
+{
+    constexpr uint32_t THREADS = WM * WN * kWave, BYTES = 128;
     constexpr int FM = TM / WM / 32, FN = TN / WN / 32;
     constexpr bool kQuant = std::is_same_v<T, fp8>;
     using E = std::conditional_t<kQuant, uint8_t, T>;
     constexpr bool kLeftAcross = P != Product::kForward, kRightAcross = P == Product::kGradMatrix;
-    using Left = Stage<E, TN, THREADS, kLeftAcross>;
-    using Right = Stage<E, TM, THREADS, kRightAcross>;
+    using Left = Stage<E, TN, BYTES, THREADS, kLeftAcross>;
+    using Right = Stage<E, TM, BYTES, THREADS, kRightAcross>;
     constexpr uint32_t kBytes = Left::kBytes + Right::kBytes;
     __shared__ __attribute__((aligned(256))) char lds[2 * kBytes];
+    __shared__ Tiles<P, TM, TN, (int)THREADS> tiles;
 
-    Tile t;
-    if (!find_tile<P>(a, TM, TN, t)) return;
+    tiles.make(a);
+    for (uint32_t turn = 0;; ++turn) {
+    const Tile t = tiles.get(a, turn);
+    if (!t.there) return;
     const uint32_t m0 = t.m * TM, n0 = t.n * TN;
-    const uint32_t rows = P == Product::kGradMatrix ? a.m : t.count;  // of the output
-    const uint32_t depth = P == Product::kGradMatrix ? t.count : a.c;
-    const E *lp = static_cast<const E *>(a.l), *rp = static_cast<const E *>(a.r);
-    if constexpr (P == Product::kForward) lp += t.expert * a.l_expert + n0 * a.l_stride;
-    else if constexpr (P == Product::kGradRows) lp += t.expert * a.l_expert + n0;
-    else lp += t.first * a.l_stride + n0;
-    if constexpr (P == Product::kGradMatrix) rp += t.first * a.r_stride + m0;
-    else rp += (t.first + m0) * a.r_stride;
-    const Left left(lp, a.l_stride, a.n - n0, depth);
-    const Right right(rp, a.r_stride, rows - m0, depth);
+    uint32_t rows, depth;
+    const E *lp, *rp;
+    tile_operands<P>(a, t, m0, n0, lp, rp, rows, depth);
+    Left left;
+    Right right;
+    left.set(lp, a.l_stride, a.n - n0, depth);
+    right.set(rp, a.r_stride, rows - m0, depth);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
     const uint32_t wm = wave % WM * (TM / WM), wn = wave / WM * (TN / WN);
 
@@ -434,35 +791,28 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_kernel(ProductArgs a)
         if (s + 1 < stages) finish(s + 1);
     }
 
-    // a lane has column m of the instruction's result and rows 8 q + 4 (lane / 32) .. + 4 of n
-    O *out = static_cast<O *>(a.o);
-    if constexpr (P == Product::kGradMatrix) out += t.expert * a.o_expert;
-    else out += t.first * a.o_stride;
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const uint32_t m = m0 + wm + j * 32 + lane % 32;
-        if (m >= rows) continue;
-        O *row = out + m * a.o_stride;
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t n = n0 + wn + i * 32 + q * 8 + lane / 32 * 4;
-                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                if (n < a.n) store_four<T>(row, n, a.n, v);
-            }
+    store_tile<P, O>(a, t, acc, m0 + wm, n0 + wn, rows);
+    __syncthreads();  // (the next tile's stages take this one's place)
     }
 }
 
-template <class T, class O, Product P, int TM, int TN, int WM, int WN, bool ALIGNED>
-int product_launch_of(const ProductArgs &a, hipStream_t s)
+template <Product P, int TM, int TN, auto kernel>
+int product_launch_of(const ProductArgs &a, int threads, hipStream_t s)
 {
+    static DeviceCache cache;
     // no more tiles of rows than one for each TM of them and one for each expert
     const uint64_t mt = P == Product::kGradMatrix ? a.experts * ceil_div(a.m, TM) : a.rows / TM + std::min<uint64_t>(a.experts, a.rows);
-    const uint64_t tiles = mt * ceil_div(a.n, TN) + 8;  // (each XCD's share is rounded up)
-    if (tiles > 0x7FFFFFFFull) return LCPP_ERR_SIZE_LIMIT;
+    const uint64_t tiles = mt * ceil_div(a.n, TN);
+    if (tiles > 0x3FFFFFFFull) return LCPP_ERR_SIZE_LIMIT;
+    // what the device holds at once, an equal number on every XCD
+    const uint64_t most = (uint64_t)device_cus() * device_cached(cache, [&] {
+                              int n = 0;
+                              const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0);
+                              return e == hipSuccess && n > 0 ? n : 1;
+                          });
+    const uint32_t grid = (uint32_t)(ceil_div(std::min(tiles, most), kXcds) * kXcds);
     const char *name = P == Product::kForward ? "expert_product" : P == Product::kGradRows ? "expert_product_rows" : "expert_product_matrix";
-    LCPP_LAUNCH(name, s, product_kernel<T, O, P, TM, TN, WM, WN, ALIGNED><<<(uint32_t)tiles, WM * WN * kWave, 0, s>>>(a));
+    LCPP_LAUNCH(name, s, kernel<<<grid, threads, 0, s>>>(a));
     LCPP_CHECK_LAUNCH();
     return LCPP_OK;
 }
@@ -479,13 +829,19 @@ int product_launch(const ProductArgs &a, hipStream_t s)
     if (P != Product::kGradMatrix) aligned = aligned && a.c * e % kChunk == 0;
     if (P != Product::kForward) aligned = aligned && a.n * e % kChunk == 0;
     if (P == Product::kGradMatrix) aligned = aligned && a.m * e % kChunk == 0;
-    if (!aligned) return product_launch_of<T, O, P, 128, 128, 2, 2, false>(a, s);
-    if constexpr (P != Product::kGradMatrix) {
-        const uint64_t each = a.rows / a.experts;
-        if (each < 48) return product_launch_of<T, O, P, 32, 128, 1, 4, true>(a, s);
-        if (each < 192) return product_launch_of<T, O, P, 128, 128, 2, 2, true>(a, s);
+    if (!aligned) return product_launch_of<P, 128, 128, product_simple_kernel<T, O, P, 128, 128, 2, 2, false>>(a, 256, s);
+    const uint64_t each = P == Product::kGradMatrix ? 256 : a.rows / a.experts;
+    if constexpr (std::is_same_v<T, fp8>) {
+        if (each < 48) return product_launch_of<P, 32, 128, product_simple_kernel<T, O, P, 32, 128, 1, 4, true>>(a, 256, s);
+        if (each < 192) return product_launch_of<P, 128, 128, product_simple_kernel<T, O, P, 128, 128, 2, 2, true>>(a, 256, s);
+        return product_launch_of<P, 256, 256, product_simple_kernel<T, O, P, 256, 256, 4, 2, true>>(a, 512, s);
+    } else {
+        if constexpr (P != Product::kGradMatrix) {
+            if (each < 48) return product_launch_of<P, 32, 128, product_kernel<T, O, P, 32, 128, 1, 4, 128, 4>>(a, 256, s);
+            if (each < 192) return product_launch_of<P, 128, 128, product_kernel<T, O, P, 128, 128, 2, 2, 128, 2>>(a, 256, s);
+        }
+        return product_launch_of<P, 256, 256, product_kernel<T, O, P, 256, 256, 4, 2, 128, 2>>(a, 512, s);
     }
-    return product_launch_of<T, O, P, 256, 256, 4, 2, true>(a, s);
 }
 
 }  // namespace
@@ -496,7 +852,7 @@ using namespace lcpp;
 namespace {
 int product_sizes(uint64_t rows, uint64_t experts, uint64_t outputs, uint64_t inputs)
 {
-    if (rows > 0x7FFFFFFFull || experts > 0xFFFFFull || outputs > kMaxCols || inputs > kMaxCols) return LCPP_ERR_INVALID_ARG;
+    if (rows > 0x7FFFFFFFull || experts > kProductExperts || outputs > kMaxCols || inputs > kMaxCols) return LCPP_ERR_INVALID_ARG;
     return LCPP_OK;
 }
 }  // namespace
