@@ -94,10 +94,11 @@ struct Stage {
     static_assert(kBytes % (kChunk * THREADS) == 0, "whole loads");
     // Chunk c of a row is kept in place c ^ swizzle(row).  Along: the 16 rows that a read touches at
     // once fill the 256 bytes of all banks, rows of 64 bytes by fours and rows of 128 by twos.  Across:
-    // the four rows of a transposing read have 64 bytes each.
+    // the four rows of a transposing read have 64 bytes each, the two of a 32-bit read, four apart, 128.
     static __device__ __forceinline__ uint32_t swizzle(uint32_t row)
     {
         static_assert(BYTES == 64 || BYTES == 128, "rows of 4 or 8 chunks");
+        if constexpr (ACROSS && sizeof(T) == 4) return (row >> 2 & 1) << 3;
         return ACROSS ? (row & 3) << 2 : BYTES == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
     }
 
@@ -108,7 +109,7 @@ struct Stage {
     // of the thread's chunk 0; the others are kRowStep rows apart and have the same chunk, the rows' swizzles repeating
     // after as many
     static constexpr uint32_t kRowStep = THREADS / kRowChunks;
-    static_assert(THREADS % kRowChunks == 0 && kRowStep % (ACROSS ? 4 : 16) == 0, "the same swizzle");
+    static_assert(THREADS % kRowChunks == 0 && kRowStep % (!ACROSS ? 16 : sizeof(T) == 4 ? 8 : 4) == 0, "the same swizzle");
     uint32_t row, chunk;
     uint32_t off[kLoads];
 
@@ -514,6 +515,38 @@ __device__ __forceinline__ void store_tile(const ProductArgs &a, const Tile &t, 
     }
 }
 
+// The loads of a workgroup's stages, one behind the other over all its tiles.
+template <class T, Product P, int TM, int TN, class Left, class Right, class List>
+struct Loads {
+    Left left;
+    Right right;
+    uint32_t turn = 0, from = 0, depth = 0;
+    bool more = true;
+    // The next stage, of the next tile that has any; past the last one loads give 0.
+    __device__ __forceinline__ void next(const ProductArgs &a, const List &tiles)
+    {
+        from += Left::kDepth;
+        while (from >= depth && more) {
+            const Tile t = tiles.get(a, turn++);
+            more = t.there;
+            if (!more) break;
+            uint32_t rows;
+            const T *lp, *rp;
+            const uint32_t m0 = t.m * TM, n0 = t.n * TN;
+            tile_operands<P>(a, t, m0, n0, lp, rp, rows, depth);
+            from = 0;
+            if (depth == 0) continue;
+            left.set(lp, a.l_stride, a.n - n0, depth);
+            right.set(rp, a.r_stride, rows - m0, depth);
+        }
+    }
+    __device__ __forceinline__ void issue(int r, uint32_t lds) const
+    {
+        if (r < (int)Left::kLoads) left.issue_one(r, left.source(from), from, lds);
+        else right.issue_one(r - Left::kLoads, right.source(from), from, lds + Left::kBytes);
+    }
+};
+
 // A workgroup of WM x WN waves makes tiles of TM x TN outputs, one after the other, from operands
 // whose chunks are whole and aligned.  The stages of all its tiles are one stream: loads for a
 // tile begin while the one before is multiplied.  Fragments are read one step ahead into the
@@ -534,7 +567,8 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_kernel(ProductArgs a)
     static_assert(kStores + (BUFS - 2) * kLoads < 64, "the counter of memory operations");
     static_assert(BUFS >= 2 && STEPS % 2 == 0, "a stage ahead, and both sets of registers in turn");
     __shared__ __attribute__((aligned(256))) char lds[BUFS * kBytes];
-    __shared__ Tiles<P, TM, TN, (int)THREADS> tiles;
+    using List = Tiles<P, TM, TN, (int)THREADS>;
+    __shared__ List tiles;
 
     tiles.make(a);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -544,45 +578,20 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_kernel(ProductArgs a)
     // Load r of a stage belongs to its step `portion`, counted from the step that frees its place: spread over
     // a stage, or at once where no other stage is on its way.
     auto portion = [](int r) { return BUFS > 2 ? r * STEPS / kLoads : 0; };
-    // what is loaded next: a stage of a tile that comes later
-    Left left;
-    Right right;
-    uint32_t load_turn = 0, load_from = 0, load_depth = 0;
-    bool load_more = true;
-    // the next stage, of the next tile that has any; past the last one loads give 0
-    auto next_stage = [&] {
-        load_from += Left::kDepth;
-        while (load_from >= load_depth && load_more) {
-            const Tile t = tiles.get(a, load_turn++);
-            load_more = t.there;
-            if (!load_more) break;
-            uint32_t rows;
-            const T *lp, *rp;
-            const uint32_t m0 = t.m * TM, n0 = t.n * TN;
-            tile_operands<P>(a, t, m0, n0, lp, rp, rows, load_depth);
-            load_from = 0;
-            if (load_depth == 0) continue;
-            left.set(lp, a.l_stride, a.n - n0, load_depth);
-            right.set(rp, a.r_stride, rows - m0, load_depth);
-        }
-    };
+    Loads<T, P, TM, TN, Left, Right, List> loads;
     uint32_t turn = 0;
     Tile t = tiles.get(a, turn++);
     if (!t.there) return;
-    next_stage();
+    loads.next(a, tiles);
     u32x4 w[2][FN], x[2][FM];
     uint32_t at = 0, load_at = (BUFS - 1) * kBytes;  // of the stage that is multiplied, and loaded, in LDS
-    if (load_more) {
+    if (loads.more) {
 #pragma unroll
         for (int s = 0; s < BUFS; ++s) {
-            if (s) next_stage();
-            const u32x4 left_src = left.source(load_from), right_src = right.source(load_from);
+            if (s) loads.next(a, tiles);
 #pragma unroll
-            for (int r = 0; r < kLoads; ++r) {
-                if (s + 1 == BUFS && portion(r) > 0) continue;
-                if (r < (int)Left::kLoads) left.issue_one(r, left_src, load_from, lds0 + s * kBytes);
-                else right.issue_one(r - Left::kLoads, right_src, load_from, lds0 + s * kBytes + Left::kBytes);
-            }
+            for (int r = 0; r < kLoads; ++r)
+                if (s + 1 < BUFS || portion(r) == 0) loads.issue(r, lds0 + s * kBytes);
         }
         stage_barrier<(BUFS - 2) * kLoads>();
 #pragma unroll
@@ -600,7 +609,6 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_kernel(ProductArgs a)
             for (int j = 0; j < FM; ++j) acc[i][j] = f32x16{};
         for (uint32_t s = 0; s < depth; s += Left::kDepth) {
             const uint32_t next = at + kBytes == BUFS * kBytes ? 0 : at + kBytes;
-            u32x4 left_src = left.source(load_from), right_src = right.source(load_from);
 #pragma unroll
             for (int k = 0; k < STEPS; ++k) {
                 const bool last = k + 1 == STEPS;
@@ -609,9 +617,8 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_kernel(ProductArgs a)
                     if (stores) stage_barrier<(BUFS - 2) * kLoads + kStores>();
                     else stage_barrier<(BUFS - 2) * kLoads>();
                     stores = false;
-                    next_stage();
+                    loads.next(a, tiles);
                     load_at = at;
-                    left_src = left.source(load_from), right_src = right.source(load_from);
                 }
                 const char *ll = lds + (last ? next : at), *lr = ll + Left::kBytes;
                 const int set = k & 1, other = set ^ 1, step = (k + 1) % STEPS;
@@ -628,8 +635,7 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_kernel(ProductArgs a)
                     for (int r = 0; r < kLoads; ++r) {
                         if (portion(r) != step) continue;
                         if ((BUFS > 2 ? r * STEPS % kLoads * kProducts / kLoads : r * kProducts / kLoads) != q) continue;
-                        if (r < (int)Left::kLoads) left.issue_one(r, left_src, load_from, lds0 + load_at);
-                        else right.issue_one(r - Left::kLoads, right_src, load_from, lds0 + load_at + Left::kBytes);
+                        loads.issue(r, lds0 + load_at);
                     }
                     acc[q / FM][q % FM] = multiply(w[set][q / FM], x[set][q % FM], acc[q / FM][q % FM], T());
                     __builtin_amdgcn_sched_barrier(0);
@@ -673,43 +679,13 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_simple_kernel(ProductAr
     __shared__ Tiles<P, TM, TN, (int)THREADS> tiles;
 
     tiles.make(a);
-    for (uint32_t turn = 0;; ++turn) {
-    const Tile t = tiles.get(a, turn);
-    if (!t.there) return;
-    const uint32_t m0 = t.m * TM, n0 = t.n * TN;
-    uint32_t rows, depth;
-    const E *lp, *rp;
-    tile_operands<P>(a, t, m0, n0, lp, rp, rows, depth);
-    Left left;
-    Right right;
-    left.set(lp, a.l_stride, a.n - n0, depth);
-    right.set(rp, a.r_stride, rows - m0, depth);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
     const uint32_t wm = wave % WM * (TM / WM), wn = wave / WM * (TN / WN);
-
-    f32x16 acc[FN][FM];
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = f32x16{};
-
     const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
-    const uint32_t stages = (depth + Left::kDepth - 1) / Left::kDepth;
+    Left left;
+    Right right;
     typename Left::Held held_l;
     typename Right::Held held_r;
-    // scales: of the lane's rows of m and of the wave's block of n
-    float scale_m[FM], scale_n = 0.0f;
-    auto scales = [&](uint32_t s) {
-        if constexpr (kQuant) {
-#pragma unroll
-            for (int j = 0; j < FM; ++j) {
-                const uint32_t m = m0 + wm + j * 32 + lane % 32;
-                scale_m[j] = a.r_scales[(t.first + (m < rows ? m : rows - 1)) * a.r_scale_row + s * a.r_scale_col];
-            }
-            const uint32_t n = n0 + wn < a.n ? n0 + wn : a.n - 1;
-            scale_n = a.l_scales[t.expert * a.l_scale_expert + (uint64_t)(n / 128) * a.l_scale_row + s];
-        }
-    };
     auto begin = [&](uint32_t s) {
         if constexpr (ALIGNED) {
             const uint32_t at = lds0 + (s & 1) * kBytes;
@@ -726,73 +702,110 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_simple_kernel(ProductAr
             right.put(held_r, lds + (s & 1) * kBytes + Left::kBytes);
         }
     };
-    if (stages) {
-        begin(0);
-        finish(0);
-        scales(0);
-    }
-    for (uint32_t s = 0; s < stages; ++s) {
-        stage_barrier();
-        float now_m[FM], now_n = scale_n;
-#pragma unroll
-        for (int j = 0; j < FM; ++j) now_m[j] = scale_m[j];
-        if (s + 1 < stages) {
-            begin(s + 1);
-            scales(s + 1);
-        }
-        const char *ll = lds + (s & 1) * kBytes, *lr = ll + Left::kBytes;
+    // scales: of the lane's rows of m and of the wave's block of n
+    float scale_m[FM], scale_n = 0.0f;
+    auto scales = [&](const Tile &t, uint32_t s) {
         if constexpr (kQuant) {
-            static_assert(TN / WN <= 128 && 128 % (TN / WN) == 0, "a wave's columns have one scale");
-            u32x8 x[FM][2];
-            auto wide = [&](const char *p, uint32_t from, uint32_t k) {
-                u32x8 v;
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    const u32x4 q = Left::along(p, from, k * 4 + lane / 32 * 2 + h);
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) v[4 * h + b] = q[b];
-                }
-                return v;
-            };
-#pragma unroll
-            for (int j = 0; j < FM; ++j)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) x[j][k] = wide(lr, wm + j * 32, k);
-#pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                u32x8 w[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) w[k] = wide(ll, wn + i * 32, k);
-#pragma unroll
-                for (int j = 0; j < FM; ++j) {
-                    f32x16 part = {};
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[k], x[j][k], part, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
-                    const float f = now_m[j] * now_n;
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) acc[i][j][q] += part[q] * f;
-                }
+            for (int j = 0; j < FM; ++j) {
+                const uint32_t m = t.m * TM + wm + j * 32 + lane % 32;
+                scale_m[j] = a.r_scales[(t.first + (m < t.count ? m : t.count - 1)) * a.r_scale_row + s * a.r_scale_col];
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                u32x4 x[FM], w[FN];
-#pragma unroll
-                for (int j = 0; j < FM; ++j) x[j] = Right::fragment(lr, wm + j * 32, k);
-#pragma unroll
-                for (int i = 0; i < FN; ++i) w[i] = Left::fragment(ll, wn + i * 32, k);
-#pragma unroll
-                for (int i = 0; i < FN; ++i)
-#pragma unroll
-                    for (int j = 0; j < FM; ++j) acc[i][j] = multiply(w[i], x[j], acc[i][j], T());
-            }
+            const uint32_t at = t.n * TN + wn, n = at < a.n ? at : a.n - 1;
+            scale_n = a.l_scales[t.expert * a.l_scale_expert + (uint64_t)(n / 128) * a.l_scale_row + s];
         }
-        if (s + 1 < stages) finish(s + 1);
-    }
-
-    store_tile<P, O>(a, t, acc, m0 + wm, n0 + wn, rows);
-    __syncthreads();  // (the next tile's stages take this one's place)
+    };
+    uint32_t turn = 0, rows = 0, stages = 0;
+    // the tile's first stage, on its way while the tile before is stored
+    auto enter = [&](const Tile &t) {
+        uint32_t depth;
+        const E *lp, *rp;
+        const uint32_t m0 = t.m * TM, n0 = t.n * TN;
+        tile_operands<P>(a, t, m0, n0, lp, rp, rows, depth);
+        left.set(lp, a.l_stride, a.n - n0, depth);
+        right.set(rp, a.r_stride, rows - m0, depth);
+        stages = (depth + Left::kDepth - 1) / Left::kDepth;
+        if (stages) {
+            begin(0);
+            scales(t, 0);
+        }
+    };
+    Tile t = tiles.get(a, turn++);
+    if (!t.there) return;
+    enter(t);
+    for (;;) {
+        f32x16 acc[FN][FM];
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) acc[i][j] = f32x16{};
+        if (stages) finish(0);
+        for (uint32_t s = 0; s < stages; ++s) {
+            stage_barrier();
+            float now_m[FM], now_n = scale_n;
+#pragma unroll
+            for (int j = 0; j < FM; ++j) now_m[j] = scale_m[j];
+            if (s + 1 < stages) {
+                begin(s + 1);
+                scales(t, s + 1);
+            }
+            const char *ll = lds + (s & 1) * kBytes, *lr = ll + Left::kBytes;
+            if constexpr (kQuant) {
+                static_assert(TN / WN <= 128 && 128 % (TN / WN) == 0, "a wave's columns have one scale");
+                u32x8 x[FM][2];
+                auto wide = [&](const char *p, uint32_t from, uint32_t k) {
+                    u32x8 v;
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        const u32x4 q = Left::along(p, from, k * 4 + lane / 32 * 2 + h);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) v[4 * h + b] = q[b];
+                    }
+                    return v;
+                };
+#pragma unroll
+                for (int j = 0; j < FM; ++j)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) x[j][k] = wide(lr, wm + j * 32, k);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    u32x8 w[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) w[k] = wide(ll, wn + i * 32, k);
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) {
+                        f32x16 part = {};
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[k], x[j][k], part, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+                        const float f = now_m[j] * now_n;
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) acc[i][j][q] += part[q] * f;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    u32x4 x[FM], w[FN];
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) x[j] = Right::fragment(lr, wm + j * 32, k);
+#pragma unroll
+                    for (int i = 0; i < FN; ++i) w[i] = Left::fragment(ll, wn + i * 32, k);
+#pragma unroll
+                    for (int i = 0; i < FN; ++i)
+#pragma unroll
+                        for (int j = 0; j < FM; ++j) acc[i][j] = multiply(w[i], x[j], acc[i][j], T());
+                }
+            }
+            if (s + 1 < stages) finish(s + 1);
+        }
+        __syncthreads();  // (the next tile's stages take this one's place)
+        const Tile done = t;
+        const uint32_t done_rows = rows;
+        t = tiles.get(a, turn++);
+        if (t.there) enter(t);
+        store_tile<P, O>(a, done, acc, done.m * TM + wm, done.n * TN + wn, done_rows);
+        if (!t.there) return;
     }
 }
 
@@ -830,16 +843,25 @@ int product_launch(const ProductArgs &a, hipStream_t s)
     if (P != Product::kForward) aligned = aligned && a.n * e % kChunk == 0;
     if (P == Product::kGradMatrix) aligned = aligned && a.m * e % kChunk == 0;
     if (!aligned) return product_launch_of<P, 128, 128, product_simple_kernel<T, O, P, 128, 128, 2, 2, false>>(a, 256, s);
+    // Tiles by what the device's rounds of them take, in rounds of 256 x 256: some of the experts' last tiles are
+    // empty, and the four products of 128 x 128, two workgroups of which share a CU, take 1.25 times as long as one
+    // of 256 x 256.  (us forward, 256 -> 128: 16 experts of 256 rows, 2048 x 2048 bfloat16 48 -> 42, 2048 x 1024
+    // float32 247 -> 141, 64 of 128 rows, 1408 x 2048 bfloat16 144 -> 109, 16 of 2048 rows, 2816 x 2048 362 -> 459.)
+    const double cus = device_cus(), spare = 0.25 * (double)std::min<uint64_t>(a.experts, a.rows);
+    auto rounds = [&](uint64_t tile, double at_once) {
+        const double mt = P == Product::kGradMatrix ? (double)(a.experts * ceil_div(a.m, tile)) : (double)a.rows / (double)tile + spare;
+        return std::max(1.0, mt * (double)ceil_div(a.n, tile) / at_once);
+    };
+    const bool large = rounds(256, cus) <= rounds(128, 2 * cus) * 0.625;
     const uint64_t each = P == Product::kGradMatrix ? 256 : a.rows / a.experts;
     if constexpr (std::is_same_v<T, fp8>) {
         if (each < 48) return product_launch_of<P, 32, 128, product_simple_kernel<T, O, P, 32, 128, 1, 4, true>>(a, 256, s);
-        if (each < 192) return product_launch_of<P, 128, 128, product_simple_kernel<T, O, P, 128, 128, 2, 2, true>>(a, 256, s);
+        if (!large) return product_launch_of<P, 128, 128, product_simple_kernel<T, O, P, 128, 128, 2, 2, true>>(a, 256, s);
         return product_launch_of<P, 256, 256, product_simple_kernel<T, O, P, 256, 256, 4, 2, true>>(a, 512, s);
     } else {
-        if constexpr (P != Product::kGradMatrix) {
+        if constexpr (P != Product::kGradMatrix)
             if (each < 48) return product_launch_of<P, 32, 128, product_kernel<T, O, P, 32, 128, 1, 4, 128, 4>>(a, 256, s);
-            if (each < 192) return product_launch_of<P, 128, 128, product_kernel<T, O, P, 128, 128, 2, 2, 128, 2>>(a, 256, s);
-        }
+        if (!large) return product_launch_of<P, 128, 128, product_kernel<T, O, P, 128, 128, 2, 2, 128, 2>>(a, 256, s);
         return product_launch_of<P, 256, 256, product_kernel<T, O, P, 256, 256, 4, 2, 128, 2>>(a, 512, s);
     }
 }
