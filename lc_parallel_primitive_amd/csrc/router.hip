@@ -18,8 +18,11 @@
 //
 // A row lies in the registers of 16, 32 or 64 lanes, eight or sixteen neighbouring
 // experts each.  The choice is k rounds of a maximum over the lane's keys and one over
-// the lanes: the lowest lane that holds it is the owner, so ties need no index in the
-// exchange, and each round is 5 to 8 lane exchanges of 32 bits.
+// the lanes, in 32 bits: keys of 2-byte logits without a bias have the expert's number in
+// their lower half, so that the largest one names its expert; others are ties in so far as
+// they are equal, and the lowest lane that holds the largest has the lowest expert.
+//
+// Bound by these rounds' instructions: 28 or 45 each.
 #include <algorithm>
 
 #include "tensor.hpp"
@@ -51,21 +54,27 @@ struct FMax {
 struct UMax {
     __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
 };
-// Fold over the GL lanes of a row's group, in each of them.
+// Fold over the GL lanes of a row's group, in each of them: inside 16 lanes by DPP, between
+// them by exchanging rows of 16 and halves of 32.
 template <int GL, class T, class Op>
 __device__ __forceinline__ T lanes_fold(T x, Op op)
 {
-    if constexpr (GL == kWave) {
-        return wave_reduce_dpp(x, op);
-    } else {
-        static_assert(GL == 16 || GL == 32, "rows of a wave");
-        x = op(x, dpp_perm<kDppQuadXor1>(x));
-        x = op(x, dpp_perm<kDppQuadXor2>(x));
-        x = op(x, dpp_perm<kDppRowHalfMirror>(x));
-        x = op(x, dpp_perm<kDppRowMirror>(x));
-        if constexpr (GL == 32) x = op(x, shfl_xor(x, 16));
-        return x;
+    static_assert(GL == 16 || GL == 32 || GL == kWave, "rows of a wave");
+    x = op(x, dpp_perm<kDppQuadXor1>(x));
+    x = op(x, dpp_perm<kDppQuadXor2>(x));
+    x = op(x, dpp_perm<kDppRowHalfMirror>(x));
+    x = op(x, dpp_perm<kDppRowMirror>(x));
+    if constexpr (GL > 16) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x);
+        const auto w = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+        x = op(__builtin_bit_cast(T, (uint32_t)w[0]), __builtin_bit_cast(T, (uint32_t)w[1]));
     }
+    if constexpr (GL > 32) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x);
+        const auto w = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+        x = op(__builtin_bit_cast(T, (uint32_t)w[0]), __builtin_bit_cast(T, (uint32_t)w[1]));
+    }
+    return x;
 }
 
 // Bits ordered like the value, NaN last of all; both zeros are one.
@@ -75,6 +84,15 @@ __device__ __forceinline__ uint32_t order_bits(float x)
     return x != x ? 0xFFFFFFFFu : b >> 31 ? ~b : b | 0x80000000u;
 }
 constexpr uint32_t kLowest = 0x007FFFFFu;  // order_bits(-infinity)
+// The same of a 2-byte type, in 16 bits: never 0.
+template <class T>
+__device__ __forceinline__ uint32_t order_bits16(T x)
+{
+    const float f = (float)x;
+    uint32_t b = __builtin_bit_cast(uint16_t, x);
+    b = f == 0.0f ? 0u : b;
+    return f != f ? 0xFFFFu : b >> 15 ? 0xFFFFu ^ b : b | 0x8000u;
+}
 
 __device__ __forceinline__ float sigmoid(float x)
 {
@@ -82,11 +100,12 @@ __device__ __forceinline__ float sigmoid(float x)
     const float e = __expf(-fabsf(x)), r = 1.0f / (1.0f + e);
     return x >= 0.0f ? r : e * r;
 }
-__device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.0f) - log1pf(__expf(-fabsf(x))); }
+// (what rounding 1 + exp(-|x|) loses is a rounding of 1, and so of the exponential that follows)
+__device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.0f) - __logf(1.0f + __expf(-fabsf(x))); }
 
-// V logits of a lane, -infinity past the row's end.
+// V logits of a lane, or what stands for them, `past` past the row's end.
 template <class T, int V>
-__device__ __forceinline__ void load_logits(const T *row, uint32_t first, uint32_t n, float (&l)[V])
+__device__ __forceinline__ void load_logits(const T *row, uint32_t first, uint32_t n, float past, float (&l)[V])
 {
 #pragma unroll
     for (int h = 0; h < V; h += kOctet) {
@@ -98,7 +117,7 @@ __device__ __forceinline__ void load_logits(const T *row, uint32_t first, uint32
         } else {
 #pragma unroll
             for (int i = 0; i < kOctet; ++i)
-                l[h + i] = col + i < n ? (float)row[col + i] : -std::numeric_limits<float>::infinity();
+                l[h + i] = col + i < n ? (float)row[col + i] : past;
         }
     }
 }
@@ -149,59 +168,76 @@ __device__ __forceinline__ void choice_weights(const RouterArgs &a, const float 
     }
 }
 
-template <class T, int GL, int V>
+// NAMED: 2-byte logits without a bias, whose keys name their expert.
+template <class T, int GL, int V, int KV, bool NAMED>
 __global__ __launch_bounds__(kRouteThreads) void router_forward_kernel(RouterArgs a)
 {
-    constexpr int RG = kRouteThreads / GL, KV = kMaxChoices / GL;
-    __shared__ int32_t ids[RG][kMaxChoices];
-    __shared__ float logits[RG][kMaxChoices];
+    constexpr int RG = kRouteThreads / GL;
+    constexpr float kNone = -std::numeric_limits<float>::infinity();
+    __shared__ int32_t ids[NAMED ? 1 : RG][KV * GL];
     const uint32_t t = threadIdx.x % GL, group = threadIdx.x / GL;
     const uint64_t row = (uint64_t)blockIdx.x * RG + group;
     const bool live = row < a.tokens;
     const uint32_t first = t * V;
+    const T *in = static_cast<const T *>(a.logits) + (live ? row : 0) * a.logits_stride;
     float l[V];
-    load_logits<T, V>(static_cast<const T *>(a.logits) + (live ? row : 0) * a.logits_stride, first, a.num_experts, l);
+    load_logits<T, V>(in, first, a.num_experts, kNone, l);
     float most = 0.0f, sum = 1.0f;
     if (!a.sigmoid && !a.normalize) soft_sum<GL, V>(l, most, sum);
+    float bias[V] = {};
+    if (!NAMED && a.bias) load_logits<float, V>(a.bias, first, a.num_experts, 0.0f, bias);
     uint32_t key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        float x = l[i];
-        if (a.bias && first + i < a.num_experts) x += a.bias[first + i];
-        const uint32_t k = order_bits(x);
-        key[i] = l[i] == -std::numeric_limits<float>::infinity() || k <= kLowest ? 0u : k;
+        if constexpr (NAMED) {
+            const uint32_t k = order_bits16((T)l[i]);  // (back to the type it came from: exact)
+            key[i] = l[i] == kNone ? 0u : k << 16 | (0xFFFFu - (first + i));
+        } else {
+            const uint32_t k = order_bits(a.bias ? l[i] + bias[i] : l[i]);
+            key[i] = l[i] == kNone || k <= kLowest ? 0u : k;
+        }
     }
-    const uint32_t base = lane_id() / GL * GL;  // of the group in its wave
+    int32_t id[KV];
+#pragma unroll
+    for (int i = 0; i < KV; ++i) id[i] = -1;
     for (uint32_t j = 0; j < a.choices; ++j) {
         uint32_t mine = key[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) mine = UMax()(mine, key[i]);
         const uint32_t best = lanes_fold<GL>(mine, UMax());
-        uint64_t holds = ballot(mine == best) >> base;
-        if constexpr (GL < kWave) holds &= (1ull << (GL % kWave)) - 1;
-        if ((uint32_t)__builtin_ctzll(holds) == t) {
-            int at = 0;
-            float x = 0.0f;
+        if constexpr (NAMED) {
 #pragma unroll
-            for (int i = V - 1; i >= 0; --i)
-                if (key[i] == best) at = i, x = l[i];
+            for (int i = 0; i < V; ++i) key[i] = key[i] == best ? 0u : key[i];
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i == at) key[i] = 0;
-            ids[group][j] = best ? (int32_t)(first + at) : -1;
-            logits[group][j] = x;
+            for (int i = 0; i < KV; ++i)
+                if (t + i * GL == j) id[i] = best ? (int32_t)(0xFFFFu - (best & 0xFFFFu)) : -1;
+        } else {
+            uint64_t holds = ballot(mine == best) >> (lane_id() / GL * GL);
+            if constexpr (GL < kWave) holds &= (1ull << (GL % kWave)) - 1;
+            bool own = (uint32_t)__builtin_ctzll(holds) == t && best;
+            uint32_t at = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const bool take = own && key[i] == best;
+                key[i] = take ? 0u : key[i];
+                at = take ? first + i : at;
+                own = own && !take;
+            }
+            if ((uint32_t)__builtin_ctzll(holds) == t) ids[group][j] = best ? (int32_t)at : -1;
         }
     }
-    wave_lds_sync();  // (a group is within a wave)
+    if constexpr (!NAMED) {
+        wave_lds_sync();  // (a group is within a wave)
+#pragma unroll
+        for (int i = 0; i < KV; ++i)
+            if (t + i * GL < a.choices) id[i] = ids[group][t + i * GL];
+    }
     float x[KV], p[KV];
     bool has[KV];
-    int32_t id[KV];
 #pragma unroll
     for (int i = 0; i < KV; ++i) {
-        const uint32_t j = t + i * GL;
-        id[i] = j < a.choices ? ids[group][j] : -1;
-        x[i] = j < a.choices ? logits[group][j] : 0.0f;
         has[i] = id[i] >= 0;
+        x[i] = has[i] ? (float)in[id[i]] : 0.0f;  // (from the caches)
     }
     choice_weights<GL, KV>(a, x, has, most, sum, p);
     if (!live) return;
@@ -215,10 +251,10 @@ __global__ __launch_bounds__(kRouteThreads) void router_forward_kernel(RouterArg
 }
 
 // The gradient's coefficients of the chosen experts meet the row in LDS.
-template <class T, int GL, int V>
+template <class T, int GL, int V, int KV>
 __global__ __launch_bounds__(kRouteThreads) void router_backward_kernel(RouterArgs a)
 {
-    constexpr int RG = kRouteThreads / GL, KV = kMaxChoices / GL;
+    constexpr int RG = kRouteThreads / GL;
     __shared__ float coef[RG][GL * V];
     const uint32_t t = threadIdx.x % GL, group = threadIdx.x / GL;
     const uint64_t row = (uint64_t)blockIdx.x * RG + group;
@@ -228,7 +264,7 @@ __global__ __launch_bounds__(kRouteThreads) void router_backward_kernel(RouterAr
     const bool dense = !a.sigmoid && !a.normalize;  // every expert has a gradient
     float l[V], most = 0.0f, sum = 1.0f;
     if (dense) {
-        load_logits<T, V>(in, first, a.num_experts, l);
+        load_logits<T, V>(in, first, a.num_experts, -std::numeric_limits<float>::infinity(), l);
         soft_sum<GL, V>(l, most, sum);
     }
 #pragma unroll
@@ -281,15 +317,20 @@ __global__ __launch_bounds__(kRouteThreads) void router_backward_kernel(RouterAr
     }
 }
 
-// f(lanes of a row, experts of a lane) as integral constants: the fewest lanes that hold
-// the row.
+// f(lanes of a row, experts of a lane, choices of a lane) as integral constants: the fewest
+// lanes that hold the row, and one choice a lane where that is enough.
 template <class F>
-int router_shape(uint32_t experts, F f)
+int router_shape(uint32_t experts, uint32_t choices, F f)
 {
-    if (experts <= 128) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
-    if (experts <= 256) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
-    if (experts <= 512) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
-    return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
+    auto of = [&](auto lanes, auto values) {
+        constexpr int GL = decltype(lanes)::value;
+        if (choices <= GL) return f(lanes, values, std::integral_constant<int, 1>{});
+        return f(lanes, values, std::integral_constant<int, kMaxChoices / GL>{});
+    };
+    if (experts <= 128) return of(std::integral_constant<int, 16>{}, std::integral_constant<int, 8>{});
+    if (experts <= 256) return of(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
+    if (experts <= 512) return of(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+    return of(std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
 }
 
 int router_args(lcpp_dtype t, lcpp_score score, int normalize, float scale, uint64_t tokens, uint64_t experts, uint64_t choices,
@@ -327,10 +368,17 @@ extern "C" int lcpp_router_forward(lcpp_dtype t, lcpp_score score, int normalize
     hipStream_t s = static_cast<hipStream_t>(stream);
     return float_dispatch(t, [&](auto x) -> int {
         using T = decltype(x);
-        return router_shape(a.num_experts, [&](auto gl, auto v) -> int {
-            constexpr int GL = decltype(gl)::value, V = decltype(v)::value;
+        return router_shape(a.num_experts, a.choices, [&](auto gl, auto v, auto kv) -> int {
+            constexpr int GL = decltype(gl)::value, V = decltype(v)::value, KV = decltype(kv)::value;
             const uint32_t grid = (uint32_t)ceil_div(a.tokens, kRouteThreads / GL);
-            LCPP_LAUNCH("router_forward", s, router_forward_kernel<T, GL, V><<<grid, kRouteThreads, 0, s>>>(a));
+            if constexpr (sizeof(T) == 2) {
+                if (!a.bias) {
+                    LCPP_LAUNCH("router_forward", s, router_forward_kernel<T, GL, V, KV, true><<<grid, kRouteThreads, 0, s>>>(a));
+                    LCPP_CHECK_LAUNCH();
+                    return LCPP_OK;
+                }
+            }
+            LCPP_LAUNCH("router_forward", s, router_forward_kernel<T, GL, V, KV, false><<<grid, kRouteThreads, 0, s>>>(a));
             LCPP_CHECK_LAUNCH();
             return LCPP_OK;
         });
@@ -354,10 +402,10 @@ extern "C" int lcpp_router_backward(lcpp_dtype t, lcpp_score score, int normaliz
     hipStream_t s = static_cast<hipStream_t>(stream);
     return float_dispatch(t, [&](auto x) -> int {
         using T = decltype(x);
-        return router_shape(a.num_experts, [&](auto gl, auto v) -> int {
-            constexpr int GL = decltype(gl)::value, V = decltype(v)::value;
+        return router_shape(a.num_experts, a.choices, [&](auto gl, auto v, auto kv) -> int {
+            constexpr int GL = decltype(gl)::value, V = decltype(v)::value, KV = decltype(kv)::value;
             const uint32_t grid = (uint32_t)ceil_div(a.tokens, kRouteThreads / GL);
-            LCPP_LAUNCH("router_backward", s, router_backward_kernel<T, GL, V><<<grid, kRouteThreads, 0, s>>>(a));
+            LCPP_LAUNCH("router_backward", s, router_backward_kernel<T, GL, V, KV><<<grid, kRouteThreads, 0, s>>>(a));
             LCPP_CHECK_LAUNCH();
             return LCPP_OK;
         });

@@ -11,8 +11,9 @@
 //
 // Bound by memory.  A wave takes one token's chunk of 64 octets (one or two 16-byte
 // accesses a lane and row), so the positions and weights are scalars and a pair without a
-// row costs nothing; a token's row is read once for all its pairs.  With dots a token
-// belongs to one wave or to four.
+// row costs nothing; a token's row is read once for all its pairs.  Of rows of fewer
+// octets a wave takes two to eight tokens at once.  With dots a token belongs to no more
+// than one wave or to four.
 #include <algorithm>
 
 #include "tensor.hpp"
@@ -65,7 +66,9 @@ template <class T>
 __device__ __forceinline__ void store_place(T *row, const Place &p, const float (&x)[kOctet])
 {
     if (p.lo == 0 && p.hi == kOctet) {
-        store_pack_nt<kOctet>(row + p.col, x);
+        // (two accesses of a 4-byte type's octet meet in the L2: 8192 tokens x 4 x 2048 with weights 118 us past it, 70 so)
+        if constexpr (sizeof(T) == 4) store_pack<kOctet>(row + p.col, x);
+        else store_pack_nt<kOctet>(row + p.col, x);
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < kOctet; ++i)
@@ -74,11 +77,12 @@ __device__ __forceinline__ void store_place(T *row, const Place &p, const float 
 }
 
 // The pairs first .. first + kBatch of a token: their rows (-1: none) and weights, the same
-// in all lanes.
+// in all lanes where LT, the lanes of a token, are a wave.
 struct Pairs {
     int64_t row[kBatch];
     float w[kBatch];
 };
+template <int LT>
 __device__ __forceinline__ Pairs token_pairs(const TokenArgs &a, uint64_t token, uint32_t first)
 {
     Pairs p;
@@ -88,7 +92,8 @@ __device__ __forceinline__ Pairs token_pairs(const TokenArgs &a, uint64_t token,
         p.w[j] = 1.0f;
         if (first + j >= a.choices) continue;
         const uint64_t at = token * a.choices + first + j;
-        const int32_t row = __builtin_amdgcn_readfirstlane(a.positions[at]);
+        int32_t row = a.positions[at];
+        if constexpr (LT == kWave) row = __builtin_amdgcn_readfirstlane(row);
         if (row >= 0 && (uint64_t)row < a.many_rows) p.row[j] = row;
         if (a.weights) p.w[j] = a.weights[at];
     }
@@ -96,14 +101,38 @@ __device__ __forceinline__ Pairs token_pairs(const TokenArgs &a, uint64_t token,
 }
 
 // ---------------------------------------------------------------- without dots
-template <class T>
+// What a wave works on: a chunk of one token's row, or, with fewer lanes LT for a token,
+// the whole rows of several.
+template <int LT>
+struct Items {
+    uint64_t at;
+    __device__ __forceinline__ Items(const TokenArgs &)
+        : at((uint64_t)blockIdx.x * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave))
+    {
+    }
+    __device__ __forceinline__ bool more(const TokenArgs &a) const
+    {
+        return LT == kWave ? at < a.tokens * a.chunks : at * (kWave / LT) < a.tokens;
+    }
+    __device__ __forceinline__ void next() { at += (uint64_t)gridDim.x * kRowWaves; }
+    __device__ __forceinline__ uint64_t token(const TokenArgs &a) const
+    {
+        return LT == kWave ? at / a.chunks : at * (kWave / LT) + lane_id() / LT;
+    }
+    // the lane's part of the row, in octets or vectors
+    __device__ __forceinline__ uint32_t part(const TokenArgs &a, uint64_t token) const
+    {
+        return LT == kWave ? (uint32_t)(at - token * a.chunks) * kWave + lane_id() : lane_id() % LT;
+    }
+};
+
+template <class T, int LT>
 __global__ __launch_bounds__(kRowThreads) void token_sum_kernel(TokenArgs a)
 {
-    const uint64_t items = a.tokens * a.chunks;
-    uint64_t item = (uint64_t)blockIdx.x * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    for (; item < items; item += (uint64_t)gridDim.x * kRowWaves) {
-        const uint64_t token = item / a.chunks;
-        const Place at = octet_place((uint32_t)(item - token * a.chunks) * kWave + lane_id(), a.cols);
+    Items<LT> item(a);
+    for (; item.more(a); item.next()) {
+        const uint64_t token = item.token(a);
+        const Place at = octet_place(item.part(a, token), token < a.tokens ? a.cols : 0);
         float acc[kOctet] = {};
         if (a.residual && at.active) {
             const Octet<T> r = load_place(static_cast<const T *>(a.residual) + token * a.residual_stride, at);
@@ -111,7 +140,8 @@ __global__ __launch_bounds__(kRowThreads) void token_sum_kernel(TokenArgs a)
             for (int i = 0; i < kOctet; ++i) acc[i] = r[i];
         }
         for (uint32_t first = 0; first < a.choices; first += kBatch) {
-            const Pairs p = token_pairs(a, token, first);
+            if (LT < kWave && !at.active) continue;
+            const Pairs p = token_pairs<LT>(a, token, first);
             if (!at.active) continue;
             Octet<T> x[kBatch];
 #pragma unroll
@@ -127,18 +157,18 @@ __global__ __launch_bounds__(kRowThreads) void token_sum_kernel(TokenArgs a)
     }
 }
 
-template <class T>
+template <class T, int LT>
 __global__ __launch_bounds__(kRowThreads) void token_spread_kernel(TokenArgs a)
 {
-    const uint64_t items = a.tokens * a.chunks;
-    uint64_t item = (uint64_t)blockIdx.x * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    for (; item < items; item += (uint64_t)gridDim.x * kRowWaves) {
-        const uint64_t token = item / a.chunks;
-        const Place at = octet_place((uint32_t)(item - token * a.chunks) * kWave + lane_id(), a.cols);
+    Items<LT> item(a);
+    for (; item.more(a); item.next()) {
+        const uint64_t token = item.token(a);
+        const Place at = octet_place(item.part(a, token), token < a.tokens ? a.cols : 0);
         Octet<T> x;
         if (at.active) x = load_place(static_cast<const T *>(a.few) + token * a.few_stride, at);
         for (uint32_t first = 0; first < a.choices; first += kBatch) {
-            const Pairs p = token_pairs(a, token, first);
+            if (LT < kWave && !at.active) continue;
+            const Pairs p = token_pairs<LT>(a, token, first);
             if (!at.active) continue;
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
@@ -153,18 +183,17 @@ __global__ __launch_bounds__(kRowThreads) void token_spread_kernel(TokenArgs a)
 }
 
 // Rows of any type as they are: V elements of U a lane, 16 bytes.
-template <class U>
+template <class U, int LT>
 __global__ __launch_bounds__(kRowThreads) void token_copy_kernel(TokenArgs a)
 {
     constexpr uint32_t V = 16 / sizeof(U);
     typedef U vec __attribute__((ext_vector_type(V)));
     typedef vec vec_u __attribute__((aligned(sizeof(U))));
-    const uint64_t items = a.tokens * a.chunks;
-    uint64_t item = (uint64_t)blockIdx.x * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    for (; item < items; item += (uint64_t)gridDim.x * kRowWaves) {
-        const uint64_t token = item / a.chunks;
-        uint32_t col = ((uint32_t)(item - token * a.chunks) * kWave + lane_id()) * V;
-        const bool active = col < a.cols, whole = a.cols >= V;
+    Items<LT> item(a);
+    for (; item.more(a); item.next()) {
+        const uint64_t token = item.token(a);
+        uint32_t col = item.part(a, token) * V;
+        const bool active = col < a.cols && token < a.tokens, whole = a.cols >= V;
         if (active && whole && col + V > a.cols) col = a.cols - V;  // (copied twice, the same values)
         const U *in = static_cast<const U *>(a.few) + token * a.few_stride + col;
         vec x = {};
@@ -176,7 +205,8 @@ __global__ __launch_bounds__(kRowThreads) void token_copy_kernel(TokenArgs a)
                     if (i < a.cols) x[i] = in[i];
         }
         for (uint32_t first = 0; first < a.choices; first += kBatch) {
-            const Pairs p = token_pairs(a, token, first);
+            if (LT < kWave && !active) continue;
+            const Pairs p = token_pairs<LT>(a, token, first);
             if (!active) continue;
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
@@ -193,15 +223,29 @@ __global__ __launch_bounds__(kRowThreads) void token_copy_kernel(TokenArgs a)
 }
 
 // ---------------------------------------------------------------- with dots
-// NT threads for a token, B batches of its pairs at a time, so that the sums of their dots
+// Sum over the LT lanes of a token, in each of them (LT 8 to 64).
+template <int LT>
+__device__ __forceinline__ float lanes_total(float x)
+{
+    if constexpr (LT == kWave) return wave_reduce_dpp(x, SumOp());
+    x += dpp_perm<kDppQuadXor1>(x);
+    x += dpp_perm<kDppQuadXor2>(x);
+    x += dpp_perm<kDppRowHalfMirror>(x);
+    if constexpr (LT > 8) x += dpp_perm<kDppRowMirror>(x);
+    if constexpr (LT > 16) x += shfl_xor(x, 16);
+    return x;
+}
+// NT threads (8 to 256) for a token, B batches of its pairs at a time, so that the sums of their dots
 // stay in registers while its columns are gone through.  SPREAD: many_out[pos] = w few as
 // well (where it is wanted), else few_out = sum of w many, of all pairs at once.
 template <class T, int NT, int B, bool SPREAD>
 __global__ __launch_bounds__(kRowThreads) void token_dots_kernel(TokenArgs a)
 {
-    constexpr int RG = kRowThreads / NT, GW = NT / kWave;
-    __shared__ float lds[2][kRowWaves][B * kBatch];
-    const uint32_t t = threadIdx.x % NT, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), group = wave / GW;
+    constexpr int RG = kRowThreads / NT, GW = NT > kWave ? NT / kWave : 1, LT = NT < kWave ? NT : kWave;
+    __shared__ float lds[2][kRowThreads / LT][B * kBatch];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t t = threadIdx.x % NT, group = NT < kWave ? threadIdx.x / NT : wave / GW;
+    const uint32_t part = NT < kWave ? group : wave;  // of the workgroup, that sums its dots
     const uint32_t octets = (a.cols + kOctet - 1) / kOctet;
     int slot = 0;
     auto some_pairs = [&](uint64_t token, uint32_t first) {
@@ -214,7 +258,7 @@ __global__ __launch_bounds__(kRowThreads) void token_dots_kernel(TokenArgs a)
                 float acc[kOctet] = {};
 #pragma unroll
                 for (int b = 0; b < B; ++b) {
-                    const Pairs p = token_pairs(a, token, first + b * kBatch);
+                    const Pairs p = token_pairs<LT>(a, token, first + b * kBatch);
                     Octet<T> y[kBatch];
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j)
@@ -242,19 +286,20 @@ __global__ __launch_bounds__(kRowThreads) void token_dots_kernel(TokenArgs a)
 #pragma unroll
         for (int b = 0; b < B; ++b)
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) dot[b][j] = wave_reduce_dpp(dot[b][j], SumOp());
-        if (lane_id() == 0)
+            for (int j = 0; j < kBatch; ++j) dot[b][j] = lanes_total<LT>(dot[b][j]);
+        if (lane_id() % LT == 0)
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) lds[slot][wave][b * kBatch + j] = dot[b][j];
+                for (int j = 0; j < kBatch; ++j) lds[slot][part][b * kBatch + j] = dot[b][j];
         if constexpr (GW > 1) __syncthreads();
         else wave_lds_sync();
-        if (live && t < B * kBatch && first + t < a.choices) {
+        for (uint32_t j = t; j < B * kBatch; j += NT) {
+            if (!live || first + j >= a.choices) break;
             float d = 0.0f;
 #pragma unroll
-            for (int w = 0; w < GW; ++w) d += lds[slot][group * GW + w][t];
-            a.dots[token * a.choices + first + t] = d;
+            for (int w = 0; w < GW; ++w) d += lds[slot][group * GW + w][j];
+            a.dots[token * a.choices + first + j] = d;
         }
         slot ^= 1;
     };
@@ -287,19 +332,35 @@ bool row_sizes(uint64_t tokens, uint64_t choices, uint64_t cols, uint64_t rows)
 {
     return tokens <= 0x7FFFFFFFull && choices <= kMaxPairs && tokens * choices <= 0x7FFFFFFFull && cols <= kMaxCols && rows <= 0x7FFFFFFFull;
 }
-uint32_t row_grid(uint64_t items, int waves) { return (uint32_t)std::min(ceil_div(items, waves), kMaxRowGroups); }
+uint32_t row_grid(uint64_t items, int each) { return (uint32_t)std::min(ceil_div(items, each), kMaxRowGroups); }
 bool pointer_or_null(const void *p, size_t size) { return !p || elem_ok(p, size); }
 
-// A token in one wave where its columns are few.
+// f(lanes) as an integral constant: as few as hold a token's row of so many parts, 8 to 64.
+template <class F>
+int lanes_of(uint64_t parts, F f)
+{
+    if (parts <= 8) return f(std::integral_constant<int, 8>{});
+    if (parts <= 16) return f(std::integral_constant<int, 16>{});
+    if (parts <= 32) return f(std::integral_constant<int, 32>{});
+    return f(std::integral_constant<int, 64>{});
+}
+// A token in one wave or less where its columns are few, else in four.
 template <class T, int B, bool SPREAD>
 int dots_launch_of(const TokenArgs &a, const char *name, hipStream_t s)
 {
-    if (a.cols <= 1024)
-        LCPP_LAUNCH(name, s, token_dots_kernel<T, kWave, B, SPREAD><<<row_grid(a.tokens, kRowWaves), kRowThreads, 0, s>>>(a));
-    else
+    const uint64_t octets = ceil_div(a.cols, kOctet);
+    if (octets > 128) {
         LCPP_LAUNCH(name, s, token_dots_kernel<T, kRowThreads, B, SPREAD><<<row_grid(a.tokens, 1), kRowThreads, 0, s>>>(a));
-    LCPP_CHECK_LAUNCH();
-    return LCPP_OK;
+        LCPP_CHECK_LAUNCH();
+        return LCPP_OK;
+    }
+    return lanes_of(octets, [&](auto lanes) -> int {
+        constexpr int LT = decltype(lanes)::value;
+        LCPP_LAUNCH(name, s,
+                    token_dots_kernel<T, LT, B, SPREAD><<<row_grid(a.tokens, kRowThreads / LT), kRowThreads, 0, s>>>(a));
+        LCPP_CHECK_LAUNCH();
+        return LCPP_OK;
+    });
 }
 template <bool SPREAD>
 int dots_launch(lcpp_dtype t, const TokenArgs &a, const char *name, hipStream_t s)
@@ -338,18 +399,26 @@ extern "C" int lcpp_token_spread(lcpp_dtype t, const void *in, uint64_t in_strid
     if (weights)
         return float_dispatch(t, [&](auto x) -> int {
             using T = decltype(x);
-            a.chunks = (uint32_t)ceil_div(cols, kWave * kOctet);
-            LCPP_LAUNCH("token_spread", s, token_spread_kernel<T><<<row_grid(tokens * a.chunks, kRowWaves), kRowThreads, 0, s>>>(a));
-            LCPP_CHECK_LAUNCH();
-            return LCPP_OK;
+            return lanes_of(ceil_div(cols, kOctet), [&](auto lanes) -> int {
+                constexpr int LT = decltype(lanes)::value;
+                a.chunks = (uint32_t)ceil_div(cols, LT * kOctet);
+                LCPP_LAUNCH("token_spread", s,
+                            token_spread_kernel<T, LT>
+                            <<<row_grid(tokens * a.chunks, kRowThreads / LT), kRowThreads, 0, s>>>(a));
+                LCPP_CHECK_LAUNCH();
+                return LCPP_OK;
+            });
         });
-    a.chunks = (uint32_t)ceil_div(cols, kWave * 16 / e);
-    const uint32_t grid = row_grid(tokens * a.chunks, kRowWaves);
-    if (e == 4) LCPP_LAUNCH("token_copy", s, token_copy_kernel<uint32_t><<<grid, kRowThreads, 0, s>>>(a));
-    else if (e == 2) LCPP_LAUNCH("token_copy", s, token_copy_kernel<uint16_t><<<grid, kRowThreads, 0, s>>>(a));
-    else LCPP_LAUNCH("token_copy", s, token_copy_kernel<uint8_t><<<grid, kRowThreads, 0, s>>>(a));
-    LCPP_CHECK_LAUNCH();
-    return LCPP_OK;
+    return lanes_of(ceil_div(cols, 16 / e), [&](auto lanes) -> int {
+        constexpr int LT = decltype(lanes)::value;
+        a.chunks = (uint32_t)ceil_div(cols, LT * 16 / e);
+        const uint32_t grid = row_grid(tokens * a.chunks, kRowThreads / LT);
+        if (e == 4) LCPP_LAUNCH("token_copy", s, token_copy_kernel<uint32_t, LT><<<grid, kRowThreads, 0, s>>>(a));
+        else if (e == 2) LCPP_LAUNCH("token_copy", s, token_copy_kernel<uint16_t, LT><<<grid, kRowThreads, 0, s>>>(a));
+        else LCPP_LAUNCH("token_copy", s, token_copy_kernel<uint8_t, LT><<<grid, kRowThreads, 0, s>>>(a));
+        LCPP_CHECK_LAUNCH();
+        return LCPP_OK;
+    });
 }
 
 extern "C" int lcpp_token_sum(lcpp_dtype t, const void *in, uint64_t in_stride, uint64_t rows, const int32_t *positions,
@@ -383,9 +452,13 @@ extern "C" int lcpp_token_sum(lcpp_dtype t, const void *in, uint64_t in_stride, 
     }
     return float_dispatch(t, [&](auto x) -> int {
         using T = decltype(x);
-        a.chunks = (uint32_t)ceil_div(cols, kWave * kOctet);
-        LCPP_LAUNCH("token_sum", s, token_sum_kernel<T><<<row_grid(tokens * a.chunks, kRowWaves), kRowThreads, 0, s>>>(a));
-        LCPP_CHECK_LAUNCH();
-        return LCPP_OK;
+        return lanes_of(ceil_div(cols, kOctet), [&](auto lanes) -> int {
+            constexpr int LT = decltype(lanes)::value;
+            a.chunks = (uint32_t)ceil_div(cols, LT * kOctet);
+            LCPP_LAUNCH("token_sum", s,
+                        token_sum_kernel<T, LT><<<row_grid(tokens * a.chunks, kRowThreads / LT), kRowThreads, 0, s>>>(a));
+            LCPP_CHECK_LAUNCH();
+            return LCPP_OK;
+        });
     });
 }
