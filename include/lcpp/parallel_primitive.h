@@ -737,6 +737,195 @@ class DeviceGatedRecurrence : public LuisaModule {
     }
 };
 
+/* ---- RMS norm, expert router, tokens sorted by expert, experts' products (no counterpart in the reference; see
+ * lcpp_amd.h) */
+
+/* Rows in 8-bit floating point (type LCPP_FLOAT8_E4M3 or _E5M2) with a scale for each row's `group` columns
+ * (0: the whole row). */
+struct EightBits {
+    lcpp_dtype type = LCPP_FLOAT8_E4M3;
+    void *d_quant = nullptr;
+    size_t stride = 0;
+    float *d_scales = nullptr;
+    size_t scale_row_stride = 0, scale_group_stride = 1;
+    uint group = 128;
+};
+
+class DeviceRMSNorm : public LuisaModule {
+  public:
+    template <class T>
+    static size_t GetBackwardTempStorageBytes(size_t rows, size_t cols)
+    {
+        size_t b = 0;
+        lcpp_rms_norm_backward_temp_bytes(activation_dtype_of<T>(), rows, cols, &b);
+        return b;
+    }
+    /* d_weight, d_rstd may be null; d_out may be a view of null where `quant` has rows */
+    template <class T, class W>
+    void Forward(CommandList &cmdlist, RowsView<T> d_in, RowsView<T> d_out, const W *d_weight, float eps, float *d_rstd,
+                 size_t rows, size_t cols, const EightBits &quant = {})
+    {
+        AddForward<T, W>(cmdlist, d_in, {}, {}, d_out, d_weight, eps, d_rstd, rows, cols, quant);
+    }
+    template <class T, class W>
+    void AddForward(CommandList &cmdlist, RowsView<T> d_in, RowsView<T> d_residual, RowsView<T> d_sum, RowsView<T> d_out,
+                    const W *d_weight, float eps, float *d_rstd, size_t rows, size_t cols, const EightBits &quant = {})
+    {
+        check(lcpp_rms_norm_forward(activation_dtype_of<T>(), activation_dtype_of<W>(), d_in.data(), d_in.stride,
+                                    d_residual.data(), d_residual.stride, d_weight, eps, d_sum.data(), d_sum.stride,
+                                    d_out.data(), d_out.stride, d_rstd, quant.type, quant.d_quant, quant.stride,
+                                    quant.d_scales, quant.scale_row_stride, quant.scale_group_stride, quant.group, rows, cols,
+                                    cmdlist.stream),
+              "DeviceRMSNorm::Forward", cmdlist.stream);
+    }
+    /* d_grad_sum: a view of null for none; d_grad_weight may be null */
+    template <class T, class W>
+    void Backward(CommandList &cmdlist, BufferView<uint> temp_storage, RowsView<T> d_grad_out, RowsView<T> d_grad_sum,
+                  RowsView<T> d_in, const W *d_weight, const float *d_rstd, RowsView<T> d_grad_in, W *d_grad_weight,
+                  size_t rows, size_t cols)
+    {
+        check(lcpp_rms_norm_backward(activation_dtype_of<T>(), activation_dtype_of<W>(), temp_storage.data(),
+                                     temp_storage.size_bytes(), d_grad_out.data(), d_grad_out.stride, d_grad_sum.data(),
+                                     d_grad_sum.stride, d_in.data(), d_in.stride, d_weight, d_rstd, d_grad_in.data(),
+                                     d_grad_in.stride, d_grad_weight, rows, cols, cmdlist.stream),
+              "DeviceRMSNorm::Backward", cmdlist.stream, rows && cols ? temp_storage : BufferView<uint>{});
+    }
+};
+
+/* How a router makes weights of its logits. */
+struct RouterScore {
+    lcpp_score score = LCPP_SCORE_SOFTMAX;
+    bool normalize = true;
+    float scale = 1.0f;
+};
+
+class DeviceExpertRouter : public LuisaModule {
+  public:
+    /* d_bias may be null */
+    template <class T>
+    void Forward(CommandList &cmdlist, RowsView<T> d_logits, const float *d_bias, int32_t *d_experts, float *d_weights,
+                 const RouterScore &how, size_t tokens, size_t experts, size_t choices)
+    {
+        check(lcpp_router_forward(activation_dtype_of<T>(), how.score, how.normalize, how.scale, d_logits.data(),
+                                  d_logits.stride, d_bias, d_experts, d_weights, tokens, experts, choices, cmdlist.stream),
+              "DeviceExpertRouter::Forward", cmdlist.stream);
+    }
+    template <class T>
+    void Backward(CommandList &cmdlist, RowsView<T> d_logits, const int32_t *d_experts, const float *d_grad_weights,
+                  RowsView<T> d_grad_logits, const RouterScore &how, size_t tokens, size_t experts, size_t choices)
+    {
+        check(lcpp_router_backward(activation_dtype_of<T>(), how.score, how.normalize, how.scale, d_logits.data(),
+                                   d_logits.stride, d_experts, d_grad_weights, d_grad_logits.data(), d_grad_logits.stride,
+                                   tokens, experts, choices, cmdlist.stream),
+              "DeviceExpertRouter::Backward", cmdlist.stream);
+    }
+};
+
+class DeviceTokenSort : public LuisaModule {
+  public:
+    static size_t GetTempStorageBytes(size_t tokens, size_t choices, size_t experts)
+    {
+        size_t b = 0;
+        lcpp_token_sort_temp_bytes(tokens, choices, experts, &b);
+        return b;
+    }
+    /* d_sources may be null */
+    void Sort(CommandList &cmdlist, BufferView<uint> temp_storage, const int32_t *d_experts, size_t tokens, size_t choices,
+              size_t experts, int32_t *d_positions, int32_t *d_offsets, int32_t *d_sources = nullptr)
+    {
+        check(lcpp_token_sort(temp_storage.data(), temp_storage.size_bytes(), d_experts, tokens, choices, experts, d_positions,
+                              d_offsets, d_sources, cmdlist.stream),
+              "DeviceTokenSort::Sort", cmdlist.stream, temp_storage);
+    }
+    /* `rows` are those of the pairs' matrix; d_weights may be null */
+    template <class T>
+    void Dispatch(CommandList &cmdlist, RowsView<T> d_in, const int32_t *d_positions, const float *d_weights, RowsView<T> d_out,
+                  size_t rows, size_t tokens, size_t choices, size_t cols)
+    {
+        check(lcpp_token_spread(activation_dtype_of<T>(), d_in.data(), d_in.stride, d_positions, d_weights, d_out.data(),
+                                d_out.stride, nullptr, 0, nullptr, rows, tokens, choices, cols, cmdlist.stream),
+              "DeviceTokenSort::Dispatch", cmdlist.stream);
+    }
+    /* d_in and d_grad_weights of null where the weights' gradient is not wanted */
+    template <class T>
+    void DispatchBackward(CommandList &cmdlist, RowsView<T> d_grad_out, const int32_t *d_positions, const float *d_weights,
+                          RowsView<T> d_grad_in, RowsView<T> d_in, float *d_grad_weights, size_t rows, size_t tokens,
+                          size_t choices, size_t cols)
+    {
+        check(lcpp_token_sum(activation_dtype_of<T>(), d_grad_out.data(), d_grad_out.stride, rows, d_positions, d_weights,
+                             nullptr, 0, d_grad_in.data(), d_grad_in.stride, d_in.data(), d_in.stride, d_grad_weights, tokens,
+                             choices, cols, cmdlist.stream),
+              "DeviceTokenSort::DispatchBackward", cmdlist.stream);
+    }
+    /* d_residual: a view of null for none */
+    template <class T>
+    void Combine(CommandList &cmdlist, RowsView<T> d_in, const int32_t *d_positions, const float *d_weights, RowsView<T> d_out,
+                 RowsView<T> d_residual, size_t rows, size_t tokens, size_t choices, size_t cols)
+    {
+        check(lcpp_token_sum(activation_dtype_of<T>(), d_in.data(), d_in.stride, rows, d_positions, d_weights,
+                             d_residual.data(), d_residual.stride, d_out.data(), d_out.stride, nullptr, 0, nullptr, tokens,
+                             choices, cols, cmdlist.stream),
+              "DeviceTokenSort::Combine", cmdlist.stream);
+    }
+    /* d_grad_in or d_grad_weights of null where it is not wanted */
+    template <class T>
+    void CombineBackward(CommandList &cmdlist, RowsView<T> d_grad_out, RowsView<T> d_in, const int32_t *d_positions,
+                         const float *d_weights, RowsView<T> d_grad_in, float *d_grad_weights, size_t rows, size_t tokens,
+                         size_t choices, size_t cols)
+    {
+        check(lcpp_token_spread(activation_dtype_of<T>(), d_grad_out.data(), d_grad_out.stride, d_positions, d_weights,
+                                d_grad_in.data(), d_grad_in.stride, d_in.data(), d_in.stride, d_grad_weights, rows, tokens,
+                                choices, cols, cmdlist.stream),
+              "DeviceTokenSort::CombineBackward", cmdlist.stream);
+    }
+};
+
+/* One matrix of `outputs` rows of `inputs` values for each expert, `row_stride` and `expert_stride` apart. */
+template <class T>
+struct MatricesView {
+    T *ptr = nullptr;
+    size_t row_stride = 0, expert_stride = 0;
+    [[nodiscard]] T *data() const noexcept { return ptr; }
+};
+
+class DeviceExpertProduct : public LuisaModule {
+  public:
+    template <class T>
+    void Forward(CommandList &cmdlist, RowsView<T> d_in, MatricesView<T> d_weight, const int32_t *d_offsets, RowsView<T> d_out,
+                 size_t rows, size_t experts, size_t outputs, size_t inputs)
+    {
+        check(lcpp_expert_product(activation_dtype_of<T>(), d_in.data(), d_in.stride, d_weight.data(), d_weight.row_stride,
+                                  d_weight.expert_stride, d_offsets, activation_dtype_of<T>(), d_out.data(), d_out.stride,
+                                  nullptr, 0, 0, nullptr, rows, experts, outputs, inputs, cmdlist.stream),
+              "DeviceExpertProduct::Forward", cmdlist.stream);
+    }
+    /* 8-bit rows and matrices (LCPP_FLOAT8_E4M3) with a scale for 128 inputs, and for 128 outputs x 128 inputs */
+    template <class O>
+    void Forward(CommandList &cmdlist, const EightBits &in, MatricesView<const uint8_t> d_weight, const float *d_weight_scales,
+                 const int32_t *d_offsets, RowsView<O> d_out, size_t rows, size_t experts, size_t outputs, size_t inputs)
+    {
+        check(in.group != 128 ? LCPP_ERR_INVALID_ARG
+                              : lcpp_expert_product(in.type, in.d_quant, in.stride, d_weight.data(), d_weight.row_stride,
+                                                    d_weight.expert_stride, d_offsets, activation_dtype_of<O>(), d_out.data(),
+                                                    d_out.stride, in.d_scales, in.scale_row_stride, in.scale_group_stride,
+                                                    d_weight_scales, rows, experts, outputs, inputs, cmdlist.stream),
+              "DeviceExpertProduct::Forward", cmdlist.stream);
+    }
+    /* d_grad_in or d_grad_weight of null where it is not wanted; G is T or float */
+    template <class T, class G>
+    void Backward(CommandList &cmdlist, RowsView<T> d_grad_out, RowsView<T> d_in, MatricesView<T> d_weight,
+                  const int32_t *d_offsets, RowsView<T> d_grad_in, MatricesView<G> d_grad_weight, size_t rows, size_t experts,
+                  size_t outputs, size_t inputs)
+    {
+        check(lcpp_expert_product_backward(activation_dtype_of<T>(), d_grad_out.data(), d_grad_out.stride, d_in.data(),
+                                           d_in.stride, d_weight.data(), d_weight.row_stride, d_weight.expert_stride,
+                                           d_offsets, d_grad_in.data(), d_grad_in.stride, activation_dtype_of<G>(),
+                                           d_grad_weight.data(), d_grad_weight.row_stride, d_grad_weight.expert_stride, rows,
+                                           experts, outputs, inputs, cmdlist.stream),
+              "DeviceExpertProduct::Backward", cmdlist.stream);
+    }
+};
+
 }  // namespace luisa::parallel_primitive
 
 #endif /* LCPP_PARALLEL_PRIMITIVE_H */

@@ -45,7 +45,7 @@ def _pairs(t, what: str):
 def _rows(t, rows, cols: int, dtype, what: str, output: bool = False):
     """(address, row stride) of a matrix of this type and so many columns, and rows (None: any)."""
     if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows) or t.dtype != dtype:
-        _unlike(t, ("any" if rows is None else rows, cols), dtype, what)
+        _unlike(t, (t.shape[0] if rows is None and t.dim() else rows, cols), dtype, what)
     return t.data_ptr(), (_like_out if output else _like)(t, t.shape, dtype, what)
 
 
