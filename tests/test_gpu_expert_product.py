@@ -165,3 +165,44 @@ def test_nothing(gpu):
     five = torch.tensor([0, 2, 2, 4], dtype=torch.int32, device="cuda")
     m.Forward(torch.empty(5, 0, device="cuda"), torch.empty(3, 8, 0, device="cuda"), five, out)
     assert torch.all(out[:4] == 0) and torch.all(out[4:] == 5.0)
+
+
+@pytest.mark.parametrize("offsets", [(-5, 3, 3, 1000000), (0, 9, 2, 20), (30, 40, 50, 60), (-9, -8, -7, -6),
+                                     (-(2**31), 2**31 - 1, 20, 20)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float8_e4m3fn])
+def test_offsets_out_of_range(gpu, offsets, dtype):
+    """Offsets are cut to the rows that are there, and one that falls leaves its expert without rows."""
+    log(f"products: offsets {offsets} {dtype}")
+    import lc_parallel_primitive_amd as m
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    rows, outputs, inputs = 20, 48, 64
+    # (small whole numbers: every product and sum is exact)
+    x = torch.randint(-2, 3, (rows, inputs), generator=g, device="cuda").float()
+    w = torch.randint(-2, 3, (3, outputs, inputs), generator=g, device="cuda").float()
+    quant = dtype == torch.float8_e4m3fn
+    out = torch.bfloat16 if quant else dtype
+    y = torch.full((rows, outputs), -77.0, device="cuda", dtype=out)
+    off = torch.tensor(offsets, dtype=torch.int64).to(torch.int32).cuda()
+    product = m.DeviceExpertProduct()
+    scales = (torch.ones(rows, 1, device="cuda"), torch.ones(3, 1, 1, device="cuda")) if quant else ()
+    product.Forward(x.to(dtype), w.to(dtype), off, y, *scales)
+    cut = [min(max(o, 0), rows) for o in offsets]
+    owners = [[e for e in range(3) if cut[e] <= r < cut[e + 1]] for r in range(rows)]
+    got = y.float().cpu()
+    for r, of in enumerate(owners):
+        wants = [(w[e] @ x[r]).to(out).float().cpu() for e in of] or [torch.full((outputs,), -77.0).to(out).float()]
+        assert any(torch.equal(got[r], v) for v in wants), (r, of)
+    if quant:
+        return
+    dx, dw = torch.full_like(x.to(dtype), -77.0), torch.full_like(w.to(dtype), -77.0)
+    dy = torch.randint(-2, 3, (rows, outputs), generator=g, device="cuda").to(dtype)
+    product.Backward(dy, x.to(dtype), w.to(dtype), off, dx, dw)
+    for e in range(3):
+        b, z = cut[e], max(cut[e], cut[e + 1])
+        want = (dy[b:z].float().t() @ x[b:z]).to(dtype)
+        assert torch.equal(dw[e], want), e
+    for r, of in enumerate(owners):
+        if not of:
+            assert bool((dx[r] == torch.full((), -77.0).to(dtype).item()).all())
