@@ -11,6 +11,11 @@
 // there are no atomics whose order could matter.  Up to one workgroup's worth of pairs is
 // one launch; more are two: the tiles' counts, then every workgroup sums the counts of
 // the tiles before its own (and of all, for the experts' offsets) and ranks its tile.
+//
+// Bound by latency: 48 x 8 pairs of 128 experts take 4.0 us, a launch and six barriers;
+// 32768 x 8 of 256 take 2.6 + 10.2 (3 MB): the tiles' counts, a chunk's experts, its
+// ranks and its places one after the other.  (Tiles at most and 64s of a wave in a chunk, both
+// launches: 128 and 2 12.0 us, 64 and 4 15.4, 32 and 4 19, 32 and 2 21, 64 and 2 16.)
 #include <algorithm>
 
 #include "common.hpp"
