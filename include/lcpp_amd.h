@@ -536,7 +536,7 @@ int lcpp_token_sum(lcpp_dtype t, const void *in, uint64_t in_stride, uint64_t ro
 /* Rows offsets[e] .. offsets[e + 1] of in times the transpose of expert e's matrix, weight + e *
  * weight_expert_stride, of `outputs` rows of `inputs` values, weight_stride apart: out[r][o] = the sum
  * over i of in[r][i] * weight[e][o][i], in 32 bits, rounded once to out_t, which is t.  No offset is
- * less than the one before (a row of two experts would have either's product); those outside 0 .. rows
+ * less than the one before (a row of two experts would have values of either); those outside 0 .. rows
  * are taken as 0 or rows; rows outside all of them are left alone.  experts <= 1024, rows < 2^31.
  * t may be LCPP_FLOAT8_E4M3, with scales and out_t any of the three types: in_scales[r *
  * in_scale_row_stride + g * in_scale_group_stride] for each row's 128 inputs and weight_scales

@@ -193,7 +193,8 @@ def test_offsets_out_of_range(gpu, offsets, dtype):
     got = y.float().cpu()
     for r, of in enumerate(owners):
         wants = [(w[e] @ x[r]).to(out).float().cpu() for e in of] or [torch.full((outputs,), -77.0).to(out).float()]
-        assert any(torch.equal(got[r], v) for v in wants), (r, of)
+        # (two experts' workgroups write a row that both have in pieces, in any order: each value is one of theirs)
+        assert bool(torch.stack([got[r] == v for v in wants]).any(0).all()), (r, of)
     if quant:
         return
     dx, dw = torch.full_like(x.to(dtype), -77.0), torch.full_like(w.to(dtype), -77.0)
