@@ -781,21 +781,32 @@ __global__ __launch_bounds__(WM *WN *kWave) void product_simple_kernel(ProductAr
                 for (int j = 0; j < FM; ++j)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) x[j][k] = wide(lr, wm + j * 32, k);
+                // (a product is added to the sums while the matrix cores make the next one)
+                u32x8 w[2];
+                f32x16 part[2];
 #pragma unroll
-                for (int i = 0; i < FN; ++i) {
-                    u32x8 w[2];
+                for (int q = 0; q <= FM * FN; ++q) {
+                    const int i = q / FM, j = q % FM;
+                    if (q < FM * FN) {
+                        if (q == 0)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) w[k] = wide(ll, wn + i * 32, k);
-#pragma unroll
-                    for (int j = 0; j < FM; ++j) {
-                        f32x16 part = {};
+                            for (int k = 0; k < 2; ++k) w[k] = wide(ll, wn, k);
+                        part[q & 1] = f32x16{};
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
-                            part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[k], x[j][k], part, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
-                        const float f = now_m[j] * now_n;
+                            part[q & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[k], x[j][k], part[q & 1], 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+                        if (j == FM - 1 && i + 1 < FN)
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) acc[i][j][q] += part[q] * f;
+                            for (int k = 0; k < 2; ++k) w[k] = wide(ll, wn + (i + 1) * 32, k);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (q > 0) {
+                        const int before = q - 1;
+                        const float f = now_m[before % FM] * now_n;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[before / FM][before % FM][r] += part[before & 1][r] * f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
 #pragma unroll
