@@ -505,7 +505,8 @@ int lcpp_router_forward(lcpp_dtype t, lcpp_score score, int normalize, float sca
                         uint64_t logits_stride, const float *bias, int32_t *experts, float *weights, uint64_t tokens,
                         uint64_t num_experts, uint64_t choices, void *stream);
 /* The gradient of the logits from that of the weights, for the experts that the forward call chose
- * (others than 0 .. num_experts - 1 have none).  grad_logits may lie over logits. */
+ * (others than 0 .. num_experts - 1 have none; one that is named twice has the sum).  grad_logits may
+ * lie over logits. */
 int lcpp_router_backward(lcpp_dtype t, lcpp_score score, int normalize, float scale, const void *logits,
                          uint64_t logits_stride, const int32_t *experts, const float *grad_weights, void *grad_logits,
                          uint64_t grad_stride, uint64_t tokens, uint64_t num_experts, uint64_t choices, void *stream);

@@ -296,7 +296,8 @@ __global__ __launch_bounds__(kRouteThreads) void router_backward_kernel(RouterAr
         else if (a.sigmoid) d *= p[i];
         if (a.sigmoid) d *= sigmoid(-x[i]);
         const uint32_t e = (uint32_t)id[i];
-        coef[group][e % V * GL + e / V] = d;
+        // (an expert that the caller's choices name twice has the sum)
+        __hip_atomic_fetch_add(&coef[group][e % V * GL + e / V], d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
     wave_lds_sync();
     if (!live) return;

@@ -149,3 +149,34 @@ def test_gradient_in_place_and_foreign_experts(gpu):
             outs.append(torch.empty_like(l))
             r.Backward(l, which, torch.ones(50, 5, device="cuda"), outs[-1], normalize=normalize)
         assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("normalize", [False, True])
+def test_gradient_of_an_expert_named_twice(gpu, score, normalize):
+    """Choices that were not made by the forward call may name an expert twice: it has the sum, as autograd in float64
+    says.  Logits of at most 2: a share is off by some 200 roundings of 2^-24, a gradient by four times as many and 80
+    more, of terms that are at most twice the largest gradient of a weight: 2 * 880 * 2^-24 = 1.05e-4 of it."""
+    log(f"router: an expert twice, {score} {normalize}")
+    import lc_parallel_primitive_amd as m
+
+    g = torch.Generator()
+    g.manual_seed(9)
+    rows, experts, k = 33, 70, 20
+    logits = torch.rand(rows, experts, generator=g) * 4 - 2
+    ids = torch.randint(0, experts, (rows, k), generator=g, dtype=torch.int32)
+    ids[:, 1] = ids[:, 0]
+    ids[:, 19] = ids[:, 2]
+    dw = torch.randn(rows, k, generator=g)
+    wide = logits.double().requires_grad_()
+    share = torch.sigmoid(wide) if score == "sigmoid" else torch.softmax(wide, 1)
+    w = share.gather(1, ids.long())
+    if normalize:
+        w = w / w.sum(1, keepdim=True)
+    (w * dw.double() * 1.5).sum().backward()
+    got = torch.empty(rows, experts, device="cuda")
+    m.DeviceExpertRouter().Backward(logits.cuda(), ids.cuda(), dw.cuda(), got, score, normalize, 1.5)
+    again = torch.empty_like(got)
+    m.DeviceExpertRouter().Backward(logits.cuda(), ids.cuda(), dw.cuda(), again, score, normalize, 1.5)
+    assert float((got.double().cpu() - wide.grad).abs().max()) <= 1.5 * 1.05e-4 * float(dw.abs().max())
+    assert torch.equal(got, again)
