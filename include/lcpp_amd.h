@@ -473,9 +473,9 @@ int lcpp_recurrence_step(lcpp_dtype t, lcpp_gate g, const void *gate, uint64_t g
  * type wt (t or LCPP_FLOAT32), NULL for 1.  rstd: one value per row for the backward pass, or NULL.
  * quant (NULL: none): out before its rounding to t, in type qt (LCPP_FLOAT8_E4M3 or _E5M2): for each
  * row and `group` columns (32, 64, 128, 256 or 512, the last ones less; 0: the whole row)
- * scale = max(max |out|, 2^-100) / (the type's largest value), quant = out / scale rounded to
- * nearest even; scales[r * scale_row_stride + g * scale_group_stride].  A group with a value that is
- * not finite has the scale NaN and values NaN.  out may be NULL where quant is not.  The square of a
+ * scale = max(max |out|, 2^-100) / (the type's largest value), quant = out / scale, divided in
+ * float32, rounded to nearest even; scales[r * scale_row_stride + g * scale_group_stride].  A group
+ * with a value that is not finite has the scale NaN and values NaN.  out may be NULL where quant is not.  The square of a
  * value passes float32's range from 2^64 on: such a row gives 0 (rstd 0).  quant may not lie over
  * an input. */
 int lcpp_rms_norm_forward(lcpp_dtype t, lcpp_dtype wt, const void *in, uint64_t in_stride, const void *residual,

@@ -6,8 +6,8 @@
 //   rstd = 1 / sqrt(sum(s^2) / n + eps)
 //   y = s rstd w
 //   8 bits: for each group of columns amax = max |y|, scale = max(amax, 2^-100) / m with
-//   m the format's largest value, q = y / scale rounded to nearest even.  A group with a
-//   y that is not finite has the scale NaN and values NaN.
+//   m the format's largest value, q = y / scale, a quotient of 32 bits rounded to nearest
+//   even.  A group with a y that is not finite has the scale NaN and values NaN.
 //
 // With v = dy w the gradients are
 //   ds = rstd (v - s rstd^2 sum(v s) / n)   [+ the gradient that reaches s elsewhere]
@@ -104,19 +104,27 @@ __device__ __forceinline__ Scale make_scale(uint32_t amax, float qmax)
     s.inverse = 1.0f / s.scale;
     return s;
 }
-// x * inverse in 8 bits: no more than the largest value and a rounding, which rounds to it.
+// x / scale rounded to 32 bits.  The product with the rounded reciprocal is off by up to two units in its last place, which
+// turns one of 14 quotients half way between two 8-bit values to the wrong side; what it leaves of x is a number of 32
+// bits, which corrects it.  (The signs are those that keep a zero's.)
+__device__ __forceinline__ float quotient(float x, const Scale &s)
+{
+    const float r = x * s.inverse;
+    return fmaf(-fmaf(r, s.scale, -x), s.inverse, r);
+}
+// Two numbers in 8 bits: no more than the largest value and a rounding of 32 bits, which rounds to it.
 __device__ __forceinline__ uint32_t quant_pair(float x, float y, bool e5m2, uint32_t old, bool high)
 {
     if (e5m2) return high ? __builtin_amdgcn_cvt_pk_bf8_f32(x, y, (int)old, true) : __builtin_amdgcn_cvt_pk_bf8_f32(x, y, (int)old, false);
     return high ? __builtin_amdgcn_cvt_pk_fp8_f32(x, y, (int)old, true) : __builtin_amdgcn_cvt_pk_fp8_f32(x, y, (int)old, false);
 }
-__device__ __forceinline__ void quant_octet(const float (&y)[kOctet], float inverse, bool e5m2, uint8_t (&q)[kOctet])
+__device__ __forceinline__ void quant_octet(const float (&y)[kOctet], const Scale &s, bool e5m2, uint8_t (&q)[kOctet])
 {
     uint32_t w[2] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        w[h] = quant_pair(y[4 * h] * inverse, y[4 * h + 1] * inverse, e5m2, 0, false);
-        w[h] = quant_pair(y[4 * h + 2] * inverse, y[4 * h + 3] * inverse, e5m2, w[h], true);
+        w[h] = quant_pair(quotient(y[4 * h], s), quotient(y[4 * h + 1], s), e5m2, 0, false);
+        w[h] = quant_pair(quotient(y[4 * h + 2], s), quotient(y[4 * h + 3], s), e5m2, w[h], true);
     }
     __builtin_memcpy(q, w, sizeof(w));
 }
@@ -291,7 +299,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ?
                     float y[kOctet];
                     uint8_t b[kOctet];
                     y_octet(k, y);
-                    quant_octet(y, s.inverse, a.e5m2, b);
+                    quant_octet(y, s, a.e5m2, b);
                     store_bytes(q + c.col(k), b);
                     const uint32_t octet = c.t + k * NT;
                     const uint32_t g = a.group ? octet >> a.log2_lanes : 0;
@@ -299,7 +307,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(AHEAD ?
                 }
                 if (c.has_tail()) {
                     const Scale s = make_scale(tail_most, a.qmax);
-                    q[c.tail()] = (uint8_t)quant_pair(y_tail * s.inverse, 0.0f, a.e5m2, 0, false);
+                    q[c.tail()] = (uint8_t)quant_pair(quotient(y_tail, s), 0.0f, a.e5m2, 0, false);
                     // (a group of these columns alone)
                     if (c.t == 0 && octets == tail_group * a.group) scales[tail_group * a.scale_col] = s.scale;
                 }
@@ -380,7 +388,7 @@ __global__ __launch_bounds__(kLongThreads) void rms_forward_long_kernel(RmsArgs 
                 if (col < a.cols) {
                     const Scale sc = make_scale(most, a.qmax);
                     uint8_t b[kOctet];
-                    quant_octet(y, sc.inverse, a.e5m2, b);
+                    quant_octet(y, sc, a.e5m2, b);
                     uint8_t *q = static_cast<uint8_t *>(a.quant) + row * a.quant_stride + col;
                     if (col + kOctet <= a.cols) {
                         store_bytes(q, b);
