@@ -319,6 +319,20 @@ __global__ __launch_bounds__(kRouteThreads) void router_backward_kernel(RouterAr
     }
 }
 
+// A launch of 2^32 threads or more reports success and leaves most of them out, so more rows than these workgroups have
+// take several launches, f(first row, rows).
+constexpr uint64_t kMaxRouteGroups = 1u << 23;
+template <class F>
+int router_launches(uint64_t tokens, int rows_of_group, F f)
+{
+    const uint64_t most = kMaxRouteGroups * rows_of_group;
+    for (uint64_t first = 0; first < tokens; first += most) {
+        const int status = f(first, std::min(tokens - first, most));
+        if (status) return status;
+    }
+    return LCPP_OK;
+}
+
 // f(lanes of a row, experts of a lane, choices of a lane) as integral constants: the fewest
 // lanes that hold the row, and one choice a lane where that is enough.
 template <class F>
@@ -372,17 +386,23 @@ extern "C" int lcpp_router_forward(lcpp_dtype t, lcpp_score score, int normalize
         using T = decltype(x);
         return router_shape(a.num_experts, a.choices, [&](auto gl, auto v, auto kv) -> int {
             constexpr int GL = decltype(gl)::value, V = decltype(v)::value, KV = decltype(kv)::value;
-            const uint32_t grid = (uint32_t)ceil_div(a.tokens, kRouteThreads / GL);
-            if constexpr (sizeof(T) == 2) {
-                if (!a.bias) {
-                    LCPP_LAUNCH("router_forward", s, router_forward_kernel<T, GL, V, KV, true><<<grid, kRouteThreads, 0, s>>>(a));
-                    LCPP_CHECK_LAUNCH();
-                    return LCPP_OK;
+            return router_launches(tokens, kRouteThreads / GL, [&](uint64_t first, uint64_t n) -> int {
+                RouterArgs b = a;
+                b.logits = static_cast<const T *>(logits) + first * logits_stride;
+                b.experts = experts + first * choices, b.weights = weights + first * choices;
+                b.tokens = (uint32_t)n;
+                const uint32_t grid = (uint32_t)ceil_div(n, kRouteThreads / GL);
+                if constexpr (sizeof(T) == 2) {
+                    if (!b.bias) {
+                        LCPP_LAUNCH("router_forward", s, router_forward_kernel<T, GL, V, KV, true><<<grid, kRouteThreads, 0, s>>>(b));
+                        LCPP_CHECK_LAUNCH();
+                        return LCPP_OK;
+                    }
                 }
-            }
-            LCPP_LAUNCH("router_forward", s, router_forward_kernel<T, GL, V, KV, false><<<grid, kRouteThreads, 0, s>>>(a));
-            LCPP_CHECK_LAUNCH();
-            return LCPP_OK;
+                LCPP_LAUNCH("router_forward", s, router_forward_kernel<T, GL, V, KV, false><<<grid, kRouteThreads, 0, s>>>(b));
+                LCPP_CHECK_LAUNCH();
+                return LCPP_OK;
+            });
         });
     });
 }
@@ -406,10 +426,17 @@ extern "C" int lcpp_router_backward(lcpp_dtype t, lcpp_score score, int normaliz
         using T = decltype(x);
         return router_shape(a.num_experts, a.choices, [&](auto gl, auto v, auto kv) -> int {
             constexpr int GL = decltype(gl)::value, V = decltype(v)::value, KV = decltype(kv)::value;
-            const uint32_t grid = (uint32_t)ceil_div(a.tokens, kRouteThreads / GL);
-            LCPP_LAUNCH("router_backward", s, router_backward_kernel<T, GL, V, KV><<<grid, kRouteThreads, 0, s>>>(a));
-            LCPP_CHECK_LAUNCH();
-            return LCPP_OK;
+            return router_launches(tokens, kRouteThreads / GL, [&](uint64_t first, uint64_t n) -> int {
+                RouterArgs b = a;
+                b.logits = static_cast<const T *>(logits) + first * logits_stride;
+                b.chosen = experts + first * choices, b.grad_weights = grad_weights + first * choices;
+                b.grad_logits = static_cast<T *>(grad_logits) + first * grad_stride;
+                b.tokens = (uint32_t)n;
+                const uint32_t grid = (uint32_t)ceil_div(n, kRouteThreads / GL);
+                LCPP_LAUNCH("router_backward", s, router_backward_kernel<T, GL, V, KV><<<grid, kRouteThreads, 0, s>>>(b));
+                LCPP_CHECK_LAUNCH();
+                return LCPP_OK;
+            });
         });
     });
 }
