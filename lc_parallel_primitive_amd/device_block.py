@@ -285,6 +285,8 @@ class DeviceRMSNorm(_BlockModule):
                    d_scales=None, group: int = 128, stream=None):
         """d_sum = d_residual + d_in, and the RMS norm of d_sum as it is stored; d_sum may be d_residual or d_in, but
         not d_out."""
+        if d_residual is None or d_sum is None:
+            raise ValueError(f"{'d_residual' if d_residual is None else 'd_sum'}: must be given")
         self._forward(d_in, d_residual, d_sum, d_out, d_weight, eps, d_rstd, d_quant, d_scales, group, stream)
 
     def Backward(self, temp_storage, d_grad_out, d_in, d_weight, d_rstd, d_grad_in, d_grad_weight=None, d_grad_sum=None,
