@@ -258,6 +258,8 @@ class DeviceRMSNorm(_BlockModule):
         return _query(lib().lcpp_rms_norm_backward_temp_bytes, float_code(dtype), rows, cols)
 
     def _forward(self, d_in, d_residual, d_sum, d_out, d_weight, eps, d_rstd, d_quant, d_scales, group, stream):
+        if d_quant is None and d_scales is not None:
+            raise ValueError("d_scales goes with d_quant")
         dtype = d_in.dtype
         code = float_code(dtype)
         shape, rows, cols, si = _matrix(d_in, "d_in")
