@@ -71,7 +71,12 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kOutside = 0xFFFFFF00u;
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t voff, uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc) : "memory");
+    // (m0 is put back: the compiler, which has no way to be told that it changes, may keep an index there)
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(rsrc)
+                 : "memory");
 }
 __device__ __forceinline__ u32x4 stage_rsrc(const void *p)
 {
