@@ -550,7 +550,8 @@ int lcpp_expert_product(lcpp_dtype t, const void *in, uint64_t in_stride, const 
                         uint64_t in_scale_group_stride, const float *weight_scales, uint64_t rows, uint64_t experts,
                         uint64_t outputs, uint64_t inputs, void *stream);
 /* The gradients of in and of the matrices (each NULL if not wanted; the latter of type t or
- * LCPP_FLOAT32, 0 for experts without rows) from that of out.  The same bits at every call. */
+ * LCPP_FLOAT32, 0 for experts without rows) from that of out.  The matrices' gradients lie one behind
+ * the other or side by side in the rows of one another.  The same bits at every call. */
 int lcpp_expert_product_backward(lcpp_dtype t, const void *grad_out, uint64_t grad_out_stride, const void *in,
                                  uint64_t in_stride, const void *weight, uint64_t weight_stride,
                                  uint64_t weight_expert_stride, const int32_t *offsets, void *grad_in,

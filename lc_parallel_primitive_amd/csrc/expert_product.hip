@@ -959,9 +959,10 @@ extern "C" int lcpp_expert_product_backward(lcpp_dtype t, const void *grad_out, 
         return LCPP_ERR_INVALID_ARG;
     if (grad_weight && outputs) {
         if (!elem_ok(grad_weight, we) || (rows && !elem_ok(in, e)) || !rows_apart(grad_weight_stride, outputs, inputs)) return LCPP_ERR_INVALID_ARG;
-        // (matrices one behind the other, or side by side within the rows of one another)
-        const uint64_t span = (outputs - 1) * grad_weight_stride + inputs;
-        if (experts > 1 && grad_weight_expert_stride < span) return LCPP_ERR_INVALID_ARG;
+        // matrices one behind the other, or side by side within the rows of one another
+        const bool behind = grad_weight_expert_stride >= (outputs - 1) * grad_weight_stride + inputs;
+        const bool beside = grad_weight_expert_stride >= inputs && grad_weight_stride >= (experts - 1) * grad_weight_expert_stride + inputs;
+        if (experts > 1 && !behind && !beside) return LCPP_ERR_INVALID_ARG;
     }
     if (same_place(grad_in, grad_weight) || same_place(grad_in, grad_out) || same_place(grad_in, weight) ||
         same_place(grad_weight, in) || same_place(grad_weight, grad_out))

@@ -190,7 +190,9 @@ def _matrices(t, what: str, output: bool = False):
     (experts, outputs, inputs), (se, so, si) = t.shape, t.stride()
     if si != 1 and inputs > 1:
         raise ValueError(f"{what}: the values of a matrix's row must be adjacent, got strides {(se, so, si)}")
-    if output and ((so < inputs and outputs > 1) or (experts > 1 and se < (outputs - 1) * so + inputs)):
+    if output and ((so < inputs and outputs > 1) or (experts > 1 and se < (outputs - 1) * so + inputs
+                                                     and (se < inputs or so < (experts - 1) * se + inputs))):
+        # (one behind the other, or side by side in the rows of one another)
         raise ValueError(f"{what}: the matrices of an output must not overlap, got strides {(se, so, si)}")
     if not t.is_cuda:
         _off_gpu(t, what)
