@@ -15,7 +15,7 @@ on the GPU, and no call waits for them.
 """
 from __future__ import annotations
 
-from ._capi import LCPP_SCORES, _float_codes, float_code, lib, quant_code
+from ._capi import LCPP_FLOAT8_E4M3, LCPP_FLOAT16, LCPP_FLOAT32, LCPP_SCORES, _float_codes, float_code, lib, quant_code
 from .device import _ptr, _query, _stream
 from .device_block import _BlockModule, _float_vector, _like, _like_out, _matrix, _off_gpu, _temp, _unlike
 
@@ -271,17 +271,12 @@ class DeviceExpertProduct(_BlockModule):
                    inputs)
 
 
-_COPIED = {"int32": 0, "uint32": 1, "uint8": 8, "int8": 8, "int16": 7}
+_COPIED = {1: LCPP_FLOAT8_E4M3, 2: LCPP_FLOAT16, 4: LCPP_FLOAT32}
 
 
 def _row_code(dtype) -> int:
     """An lcpp_dtype of as many bytes as the elements of rows that are copied."""
-    code = _float_codes.get(dtype)
-    if code is not None:
-        return code
-    name = str(dtype).replace("torch.", "")
-    if name in _COPIED:
-        return _COPIED[name]
-    if name.startswith("float8"):
-        return quant_code(dtype)
-    return float_code(dtype)
+    code = _COPIED.get(dtype.itemsize)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}: rows that are copied have elements of 1, 2 or 4 bytes")
+    return code
