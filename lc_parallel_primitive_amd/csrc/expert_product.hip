@@ -884,14 +884,19 @@ int product_launch(const ProductArgs &a, hipStream_t s)
         return std::max(1.0, mt * (double)ceil_div(a.n, tile) / at_once);
     };
     const bool large = rounds(256, cus) <= rounds(128, 2 * cus) * 0.625;
-    const uint64_t each = P == Product::kGradMatrix ? 256 : a.rows / a.experts;
+    // Rows of 32 where an expert has no more on average: one such tile holds them, and reads the matrices as fast as can be; a
+    // second tile reads them once more.  (us forward, 128 x 128 -> 32 x 128: 128 experts of 2048 x 1024 with 3, 32, 40 and 64 rows
+    // each bfloat16 99 -> 91, 107 -> 98, 111 -> 133, 118 -> 138, e4m3 49 -> 41, 58 -> 49, 60 -> 79, 68 -> 91; 64 of 1408 x 2048
+    // bfloat16 97 -> 80, 101 -> 85, 102 -> 94, 105 -> 99; 16 of 4096 x 2048 43 -> 40, 44 -> 41, 44 -> 51, 45 -> 54; uneven
+    // ones with 24 and 40 rows on average 105 -> 108 and 123 -> 131, 98 -> 82 and 101 -> 87, 68 -> 54 and 46 -> 57.)
+    const bool few = P != Product::kGradMatrix && a.rows / a.experts <= 32;
     if constexpr (std::is_same_v<T, fp8>) {
-        if (each < 48) return product_launch_of<P, 32, 128, product_simple_kernel<T, O, P, 32, 128, 1, 4, true>>(a, 256, s);
+        if (few) return product_launch_of<P, 32, 128, product_simple_kernel<T, O, P, 32, 128, 1, 4, true>>(a, 256, s);
         if (!large) return product_launch_of<P, 128, 128, product_simple_kernel<T, O, P, 128, 128, 2, 2, true>>(a, 256, s);
         return product_launch_of<P, 256, 256, product_simple_kernel<T, O, P, 256, 256, 4, 2, true>>(a, 512, s);
     } else {
         if constexpr (P != Product::kGradMatrix)
-            if (each < 48) return product_launch_of<P, 32, 128, product_kernel<T, O, P, 32, 128, 1, 4, 128, 4>>(a, 256, s);
+            if (few) return product_launch_of<P, 32, 128, product_kernel<T, O, P, 32, 128, 1, 4, 128, 4>>(a, 256, s);
         if (!large) return product_launch_of<P, 128, 128, product_kernel<T, O, P, 128, 128, 2, 2, 128, 2>>(a, 256, s);
         return product_launch_of<P, 256, 256, product_kernel<T, O, P, 256, 256, 4, 2, 128, 2>>(a, 512, s);
     }

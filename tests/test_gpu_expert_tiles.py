@@ -47,7 +47,7 @@ def uneven(experts, rows, seed):
     return [v for pair in zip(lengths, some) for v in pair] + lengths[len(some):] + some[len(lengths):]
 
 
-# What the host's rule takes on 256 CUs (tiles of 128 x 128 past 819 are large ones; below 48 rows an expert 32 x 128).
+# What the host's rule takes on 256 CUs (tiles of 128 x 128 past 819 are large ones; up to 32 rows an expert 32 x 128).
 # name: (lengths, columns of the results, [sums])
 WAYS = {
     "256, whole columns": (uneven(12, 11000, 1), 2048, [64, 200]),
