@@ -821,6 +821,23 @@ class DeviceExpertRouter : public LuisaModule {
     }
 };
 
+template <class T>
+constexpr bool is_activation()
+{
+    using U = std::remove_cv_t<T>;
+    return std::is_same_v<U, float> || std::is_same_v<U, bfloat16> || std::is_same_v<U, float16>;
+}
+/* The type of rows that may be copied only: an activation's own, else one of as many bytes. */
+template <class T>
+constexpr lcpp_dtype row_dtype_of()
+{
+    if constexpr (is_activation<T>()) return activation_dtype_of<T>();
+    else if constexpr (sizeof(T) == 1) return LCPP_FLOAT8_E4M3;
+    else if constexpr (sizeof(T) == 2) return LCPP_FLOAT16;
+    else if constexpr (sizeof(T) == 4) return LCPP_FLOAT32;
+    else static_assert(sizeof(T) == 0, "rows are of types of 1, 2 or 4 bytes");
+}
+
 class DeviceTokenSort : public LuisaModule {
   public:
     static size_t GetTempStorageBytes(size_t tokens, size_t choices, size_t experts)
@@ -837,13 +854,16 @@ class DeviceTokenSort : public LuisaModule {
                               d_offsets, d_sources, cmdlist.stream),
               "DeviceTokenSort::Sort", cmdlist.stream, temp_storage);
     }
-    /* `rows` are those of the pairs' matrix; d_weights may be null */
+    /* `rows` are those of the pairs' matrix; d_weights may be null.  Without weights rows of any type of 1, 2 or 4 bytes are
+     * copied (8-bit ones: uint8_t) */
     template <class T>
     void Dispatch(CommandList &cmdlist, RowsView<T> d_in, const int32_t *d_positions, const float *d_weights, RowsView<T> d_out,
                   size_t rows, size_t tokens, size_t choices, size_t cols)
     {
-        check(lcpp_token_spread(activation_dtype_of<T>(), d_in.data(), d_in.stride, d_positions, d_weights, d_out.data(),
-                                d_out.stride, nullptr, 0, nullptr, rows, tokens, choices, cols, cmdlist.stream),
+        check(d_weights && !is_activation<T>()
+                  ? LCPP_ERR_UNSUPPORTED_DTYPE
+                  : lcpp_token_spread(row_dtype_of<T>(), d_in.data(), d_in.stride, d_positions, d_weights, d_out.data(),
+                                      d_out.stride, nullptr, 0, nullptr, rows, tokens, choices, cols, cmdlist.stream),
               "DeviceTokenSort::Dispatch", cmdlist.stream);
     }
     /* d_in and d_grad_weights of null where the weights' gradient is not wanted */
