@@ -22,8 +22,9 @@
 // their lower half, so that the largest one names its expert; others are ties in so far as
 // they are equal, and the lowest lane that holds the largest has the lowest expert.
 //
-// Bound by these rounds' instructions: 28 or 45 each.  32768 x 256 float32, 8 chosen: 17 us
-// forward (35 MB, 7 us of a copy), 12 backward (4.7 TB/s); 48 x 128: 3.1, the launch.
+// Bound by these rounds' instructions: 28 or 45 each.  32768 x 256, 8 chosen: float32 16 us
+// forward (35 MB, 7 us of a copy), 12 backward (4.7 TB/s); bfloat16 13 without a bias (3.4 of a
+// copy) and 15.5 with one, 7 backward; 48 x 128: 3.1, the launch.
 #include <algorithm>
 
 #include "tensor.hpp"
